@@ -24,6 +24,11 @@ ROWS_U8 = 8
 ROWS_Q8 = 16
 METRIC_IP = 32
 
+# the token cache: codes, and the types of rows, queries and outputs
+CODES_I8, CODES_E4M3 = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+PLAN_NO_BLOCKS, PLAN_TABLE_FULL, PLAN_SLOTS_FULL, PLAN_BAD_LENGTH = 1, 2, 4, 8
+
 _u32p = C.POINTER(C.c_uint32)
 _f32p = C.POINTER(C.c_float)
 _i32p = C.POINTER(C.c_int32)
@@ -36,6 +41,11 @@ class FlatGraphC(C.Structure):
     _fields_ = [("n", C.c_uint32), ("d", C.c_uint32), ("nlayers", C.c_uint32), ("deg0", C.c_uint32), ("degu", C.c_uint32),
                 ("adj0", _u32p), ("cnt0", _u32p), ("up_off", _u32p), ("up_order", _u32p), ("up_down", _u32p),
                 ("up_cnt", _u32p), ("up_adj_slot", _u32p), ("up_adj_order", _u32p), ("ep_slot", _u32p), ("ep_order", _u32p)]
+
+
+class TokenCacheC(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_blocks", C.c_uint32), ("n_heads", C.c_uint32), ("block_tokens", C.c_uint32), ("dim", C.c_uint32), ("codes", C.c_uint32)]
 
 
 # every symbol include/hnsw_amd.h declares: name -> (restype, argtypes)
@@ -76,6 +86,19 @@ SYMBOLS = {
     "hnsw_amd_gather_ceiling_device": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, _f32p, C.POINTER(C.c_uint64)]),
     "hnsw_amd_last_launch_info": (C.c_int, [C.c_void_p, _u32p, _u32p, _u32p]),
     "hnsw_amd_vector_data": (C.c_int, [C.c_void_p, C.POINTER(_f32p)]),
+    "hnsw_amd_cache_plan_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32,
+                                             C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "hnsw_amd_cache_append_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                                               C.c_void_p, C.c_int, C.c_void_p]),
+    "hnsw_amd_cache_read_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "hnsw_amd_cache_attend_workspace": (C.c_uint64, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "hnsw_amd_cache_attend_found_workspace": (C.c_uint64, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "hnsw_amd_cache_attend_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_int64, C.c_int64, C.c_uint32, C.c_void_p, C.c_uint32,
+                                               C.c_void_p, C.c_uint32, C.c_void_p, C.c_int, C.c_float, C.c_uint32, C.c_void_p, C.c_void_p,
+                                               C.c_void_p, C.c_uint64, C.c_int, C.c_void_p]),
+    "hnsw_amd_cache_attend_found_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_int64, C.c_int64, C.c_uint32, C.c_void_p,
+                                                     C.c_uint32, C.c_void_p, C.c_uint32, C.c_void_p, C.c_int, C.c_void_p, C.c_uint32, C.c_uint32,
+                                                     C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_int, C.c_void_p]),
     "hnsw_amd_get_info": (C.c_int, [C.c_void_p, _i32p, _i32p, _i32p, _i32p, _u32p, _i32p, _i32p, _u32p]),
 }
 

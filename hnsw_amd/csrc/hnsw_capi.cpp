@@ -22,6 +22,18 @@ float bruteforce_knn(const float* d_base, uint32_t n, const float* d_queries, ui
                      uint32_t id_offset, uint32_t* d_out_ids, float* d_out_dist, void* stream_v);
 void merge_topk(const float* d_dist, const uint32_t* d_ids, const uint32_t* shard_offset, uint32_t S, uint32_t nq, uint32_t k,
                 uint32_t out_k, size_t shard_stride, uint32_t* d_out_ids, float* d_out_dist, void* stream);
+void cache_plan(const int32_t* lens, const int32_t* grow, uint32_t n_requests, int32_t* table, uint32_t width, int32_t* ring, uint32_t n_blocks,
+                const int64_t* state, uint32_t block_tokens, uint32_t n_slots, int64_t* slots, int32_t* cu_new, int32_t* lens_out,
+                int64_t* state_out, int32_t* status, int device, void* stream);
+void cache_append(const hnsw_amd_token_cache* c, const void* k, const void* v, uint32_t n_rows, uint32_t row_type, int64_t k_row_stride,
+                  int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, const int64_t* slots, int device, void* stream);
+void cache_read(const hnsw_amd_token_cache* c, const int64_t* slots, uint32_t n_rows, uint32_t row_type, void* k, void* v, int device, void* stream);
+uint64_t attend_workspace(const hnsw_amd_token_cache* c, uint32_t n_rows, uint32_t q_heads, uint32_t n_requests, uint32_t width, uint32_t max_len);
+uint64_t attend_found_workspace(const hnsw_amd_token_cache* c, uint32_t n_rows, uint32_t q_heads, uint32_t id_heads, uint32_t n_ids);
+void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows, uint32_t q_heads, int64_t q_row_stride, int64_t q_head_stride,
+                  uint32_t row_type, const int32_t* table, uint32_t width, const int32_t* lens, uint32_t n_requests, const int32_t* cu_q,
+                  bool found, const int32_t* ids, uint32_t n_ids, uint32_t id_heads, int causal, float scale, uint32_t max_len, void* out, float* lse,
+                  void* workspace, uint64_t workspace_bytes, int device, void* stream);
 }
 
 struct hnsw_amd_index {
@@ -477,6 +489,73 @@ int hnsw_amd_get_info(hnsw_amd_index* h, int32_t* M, int32_t* Mmax, int32_t* Mma
         if (max_node_count) *max_node_count = h->host.max_node_count_;
         if (actual_node_count) *actual_node_count = h->host.actual_node_count_;
         if (nlayers) *nlayers = (uint32_t)h->host.layers_.size();
+    });
+}
+
+int hnsw_amd_cache_plan_device(const int32_t* d_lens, const int32_t* d_grow, uint32_t n_requests, int32_t* d_table, uint32_t width, int32_t* d_ring,
+                               uint32_t n_blocks, const int64_t* d_state, uint32_t block_tokens, uint32_t n_slots, int64_t* d_slots, int32_t* d_cu_new,
+                               int32_t* d_lens_out, int64_t* d_state_out, int32_t* d_status, int device, void* stream)
+{
+    return guarded([&] {
+        REQUIRE(d_lens && d_grow && d_table && d_ring && d_state && (d_slots || n_slots == 0) && d_cu_new && d_lens_out && d_state_out && d_status,
+                "cache_plan: NULL argument");
+        cache_plan(d_lens, d_grow, n_requests, d_table, width, d_ring, n_blocks, d_state, block_tokens, n_slots, d_slots, d_cu_new, d_lens_out,
+                   d_state_out, d_status, device, stream);
+    });
+}
+
+int hnsw_amd_cache_append_device(const hnsw_amd_token_cache* cache, const void* d_k, const void* d_v, uint32_t n_rows, uint32_t row_type,
+                                 int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, const int64_t* d_slots,
+                                 int device, void* stream)
+{
+    return guarded([&] {
+        REQUIRE(n_rows == 0 || (d_k && d_v && d_slots), "cache_append: NULL argument");
+        cache_append(cache, d_k, d_v, n_rows, row_type, k_row_stride, k_head_stride, v_row_stride, v_head_stride, d_slots, device, stream);
+    });
+}
+
+int hnsw_amd_cache_read_device(const hnsw_amd_token_cache* cache, const int64_t* d_slots, uint32_t n_rows, uint32_t row_type, void* d_k, void* d_v,
+                               int device, void* stream)
+{
+    return guarded([&] {
+        REQUIRE(n_rows == 0 || d_slots, "cache_read: NULL argument");
+        cache_read(cache, d_slots, n_rows, row_type, d_k, d_v, device, stream);
+    });
+}
+
+uint64_t hnsw_amd_cache_attend_workspace(const hnsw_amd_token_cache* cache, uint32_t n_rows, uint32_t n_q_heads, uint32_t n_requests, uint32_t width,
+                                         uint32_t max_len)
+{
+    return cache ? attend_workspace(cache, n_rows, n_q_heads, n_requests, width, max_len) : 0;
+}
+
+uint64_t hnsw_amd_cache_attend_found_workspace(const hnsw_amd_token_cache* cache, uint32_t n_rows, uint32_t n_q_heads, uint32_t id_heads, uint32_t n_ids)
+{
+    return cache ? attend_found_workspace(cache, n_rows, n_q_heads, id_heads, n_ids) : 0;
+}
+
+int hnsw_amd_cache_attend_device(const hnsw_amd_token_cache* cache, const void* d_q, uint32_t n_rows, uint32_t n_q_heads, int64_t q_row_stride,
+                                 int64_t q_head_stride, uint32_t row_type, const int32_t* d_table, uint32_t width, const int32_t* d_lens,
+                                 uint32_t n_requests, const int32_t* d_cu_q, int causal, float scale, uint32_t max_len, void* d_out, float* d_lse,
+                                 void* d_workspace, uint64_t workspace_bytes, int device, void* stream)
+{
+    return guarded([&] {
+        REQUIRE(d_table && d_lens && (n_rows == 0 || (d_q && d_out)), "cache_attend: NULL argument");
+        cache_attend(cache, d_q, n_rows, n_q_heads, q_row_stride, q_head_stride, row_type, d_table, width, d_lens, n_requests, d_cu_q, false, nullptr, 0, 0,
+                     causal, scale, max_len, d_out, d_lse, d_workspace, workspace_bytes, device, stream);
+    });
+}
+
+int hnsw_amd_cache_attend_found_device(const hnsw_amd_token_cache* cache, const void* d_q, uint32_t n_rows, uint32_t n_q_heads, int64_t q_row_stride,
+                                       int64_t q_head_stride, uint32_t row_type, const int32_t* d_table, uint32_t width, const int32_t* d_lens,
+                                       uint32_t n_requests, const int32_t* d_cu_q, int causal, const uint32_t* d_ids, uint32_t id_heads,
+                                       uint32_t n_ids, float scale, void* d_out, float* d_lse, void* d_workspace, uint64_t workspace_bytes,
+                                       int device, void* stream)
+{
+    return guarded([&] {
+        REQUIRE(d_table && d_lens && (n_rows == 0 || (d_q && d_out && (d_ids || n_ids == 0))), "cache_attend_found: NULL argument");
+        cache_attend(cache, d_q, n_rows, n_q_heads, q_row_stride, q_head_stride, row_type, d_table, width, d_lens, n_requests, d_cu_q,
+                     true, reinterpret_cast<const int32_t*>(d_ids), n_ids, id_heads, causal, scale, 0, d_out, d_lse, d_workspace, workspace_bytes, device, stream);
     });
 }
 

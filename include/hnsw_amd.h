@@ -283,6 +283,93 @@ int hnsw_amd_last_launch_info(hnsw_amd_index* h, uint32_t* lds_bytes_per_query, 
  * valid until the next init / load_graph / import_flat / destroy. */
 int hnsw_amd_vector_data(hnsw_amd_index* h, const float** out);
 
+/* ---- The token cache ------------------------------------------------------------------------------------------------
+ * No counterpart in the reference, which indexes vectors.  The other half of using an index as a language model's memory:
+ * the search says WHICH earlier tokens a query needs, the cache holds what the model reads from them.  Keys and values are
+ * held in 8 bits, in blocks of block_tokens tokens, with one scale for each block and head:
+ *
+ *   codes [n_blocks][n_heads][block_tokens][dim] bytes (16-byte aligned),  scale [n_blocks][n_heads],  value = code * scale
+ *
+ * Requests own blocks through a table [n_requests][width] of block numbers: token p of request b lies in block
+ * table[b][p / block_tokens], its *slot* is that block * block_tokens + p % block_tokens.  Free blocks wait in a ring of
+ * n_blocks entries: ring[head % n_blocks] .. ring[(tail - 1) % n_blocks], state = {head, tail}.
+ *
+ * All pointers below (but the descriptor itself) are device memory of `device`.  The calls are asynchronous on `stream` (a hipStream_t of
+ * that device, NULL = its default stream), allocate nothing, wait for nothing and can be captured into a graph; calls that
+ * touch different buffers may overlap.  What lies in device memory cannot be refused by the host: each call says what it
+ * does with block numbers, slots and lengths that are out of range (none of them reads or writes outside the buffers). */
+enum { HNSW_AMD_CODES_I8 = 0,         /* signed bytes, -127..127 */
+       HNSW_AMD_CODES_E4M3 = 1 };     /* 8-bit floats (4 exponent, 3 mantissa bits; largest 448, no infinities) */
+enum { HNSW_AMD_TYPE_F32 = 0, HNSW_AMD_TYPE_F16 = 1, HNSW_AMD_TYPE_BF16 = 2 };   /* of rows, queries and outputs */
+typedef struct {
+    void *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    uint32_t n_blocks, n_heads;
+    uint32_t block_tokens;            /* 16, 32, 64, 128 or 256 */
+    uint32_t dim;                     /* multiple of 16, up to 256 */
+    uint32_t codes;                   /* HNSW_AMD_CODES_* */
+} hnsw_amd_token_cache;
+
+/* Block tables and slots from request lengths, one launch.  Request b holds lens[b] tokens and grows by grow[b] >= 0, or
+ * ends (grow[b] == -1: its blocks go back to the ring).  Blocks are taken off the ring's head in the order of the requests
+ * and entered into the table behind those the request holds; blocks given back go behind the tail and can be taken by later
+ * calls.  Writes slots[0 .. n_slots) (the new tokens of request 0, then 1, ...; -1 behind the last one), cu_new[0 .. n_requests]
+ * (new tokens before each request), lens_out and state_out, which may not be the inputs' buffers: a call that is repeated
+ * with the same inputs gives the same results.  (A request's table row keeps its entries when it ends.)  *status is 0, or
+ * says with HNSW_AMD_PLAN_* bits why nothing was done: then slots are -1, cu_new 0, lengths, state, table and ring as before.
+ * n_requests <= 8192. */
+enum { HNSW_AMD_PLAN_NO_BLOCKS = 1,   /* the ring holds fewer blocks than are needed */
+       HNSW_AMD_PLAN_TABLE_FULL = 2,  /* a request would outgrow its table row (width blocks) */
+       HNSW_AMD_PLAN_SLOTS_FULL = 4,  /* more than n_slots new tokens */
+       HNSW_AMD_PLAN_BAD_LENGTH = 8 };/* a negative length, grow < -1, or a ring state that cannot be */
+int hnsw_amd_cache_plan_device(const int32_t* d_lens, const int32_t* d_grow, uint32_t n_requests, int32_t* d_table, uint32_t width, int32_t* d_ring,
+                               uint32_t n_blocks, const int64_t* d_state, uint32_t block_tokens, uint32_t n_slots, int64_t* d_slots, int32_t* d_cu_new,
+                               int32_t* d_lens_out, int64_t* d_state_out, int32_t* d_status, int device, void* stream);
+
+/* Quantises n_rows new tokens (k, v: [n_rows][n_heads][dim] of row_type, strides in elements, the last dimension contiguous)
+ * into their slots.  A block's scale is the least power of two 2^e (-100 <= e <= 121) for which the largest finite value fits
+ * the codes' range; it never shrinks while the block holds earlier tokens, and where a new token raises it the earlier codes
+ * are rounded to the new scale.  Rows whose run begins at a block's first slot start the block afresh.  Codes round to
+ * nearest, ties to even; infinities become the largest code, NaN becomes 0.  Slots outside the cache are skipped.  The rows
+ * of one block must lie next to each other with ascending slots (as cache_plan lays them out): a block that is named in two
+ * separate places of one call ends with unspecified codes and scale. */
+int hnsw_amd_cache_append_device(const hnsw_amd_token_cache* cache, const void* d_k, const void* d_v, uint32_t n_rows, uint32_t row_type,
+                                 int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, const int64_t* d_slots,
+                                 int device, void* stream);
+
+/* The values of n_rows slots, [n_rows][n_heads][dim] of row_type (16-byte aligned); either output may be NULL.  In 32 bits the stored
+ * keys are what an index over them is built from.  A slot outside the cache gives zeros. */
+int hnsw_amd_cache_read_device(const hnsw_amd_token_cache* cache, const int64_t* d_slots, uint32_t n_rows, uint32_t row_type, void* d_k, void* d_v,
+                               int device, void* stream);
+
+/* Softmax attention over the cache: out[i][h] = sum_t p_t v_t / sum_t p_t with p_t = exp(scale * q[i][h] . k_t), the key head
+ * of query head h being h / (n_q_heads / n_heads).  q: n_rows rows of n_q_heads heads (strides in elements, the last dimension
+ * contiguous), out: [n_rows][n_q_heads][dim] of row_type, lse (may be NULL): [n_rows][n_q_heads] f32, log sum_t p_t.
+ * cu_q NULL: one row for each request.  Else request b's rows are cu_q[b] .. cu_q[b + 1] (n_requests + 1 ascending entries
+ * from 0, none above n_rows); rows behind the last request are left as they are.  The rows of a request are its last tokens
+ * (lens counts them): with `causal`, row i of n sees the tokens 0 .. lens - n + i; without, all of lens.  A row that sees
+ * nothing gives zeros and -infinity.  Lengths are taken within 0 .. width * block_tokens, tokens of a block number outside
+ * the cache do not exist.  max_len: a hint, the longest length (0: not known), which sets how the work is split; results do
+ * not depend on it beyond rounding.  workspace: at least hnsw_amd_cache_attend_workspace(...) bytes, 16-byte aligned, not
+ * shared with a call that may run at the same time (NULL if that is 0). */
+uint64_t hnsw_amd_cache_attend_workspace(const hnsw_amd_token_cache* cache, uint32_t n_rows, uint32_t n_q_heads, uint32_t n_requests, uint32_t width,
+                                         uint32_t max_len);
+int hnsw_amd_cache_attend_device(const hnsw_amd_token_cache* cache, const void* d_q, uint32_t n_rows, uint32_t n_q_heads, int64_t q_row_stride,
+                                 int64_t q_head_stride, uint32_t row_type, const int32_t* d_table, uint32_t width, const int32_t* d_lens,
+                                 uint32_t n_requests, const int32_t* d_cu_q, int causal, float scale, uint32_t max_len, void* d_out, float* d_lse,
+                                 void* d_workspace, uint64_t workspace_bytes, int device, void* stream);
+
+/* The same over listed tokens: row i and list head g (query heads g * n_q_heads / id_heads and on; id_heads is a multiple of
+ * n_heads and divides n_q_heads) see the tokens ids[i][g][0 .. n_ids), positions in their request — the node_orders that a search of
+ * an index over that request's keys returns, whose padding (0xFFFFFFFF), like any other position at or behind the row's last
+ * visible token, is skipped.  A position that is listed twice counts twice. */
+uint64_t hnsw_amd_cache_attend_found_workspace(const hnsw_amd_token_cache* cache, uint32_t n_rows, uint32_t n_q_heads, uint32_t id_heads, uint32_t n_ids);
+int hnsw_amd_cache_attend_found_device(const hnsw_amd_token_cache* cache, const void* d_q, uint32_t n_rows, uint32_t n_q_heads, int64_t q_row_stride,
+                                       int64_t q_head_stride, uint32_t row_type, const int32_t* d_table, uint32_t width, const int32_t* d_lens,
+                                       uint32_t n_requests, const int32_t* d_cu_q, int causal, const uint32_t* d_ids, uint32_t id_heads,
+                                       uint32_t n_ids, float scale, void* d_out, float* d_lse, void* d_workspace, uint64_t workspace_bytes,
+                                       int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
