@@ -24,78 +24,602 @@ struct AttendArgs {
 
 namespace {
 
-// The simplest form: one workgroup per query row and head, 256 tokens at a time.
-template <class T, int CODES>
-__global__ __launch_bounds__(256) void attend_simple_kernel(AttendArgs a)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWaves = 4;                 // wavefronts of a workgroup
+constexpr uint32_t kTile = 32;            // tokens a wavefront takes at a time
+constexpr uint32_t kScanTokens = 4096;    // of one table of block entries in LDS (all tokens), and
+constexpr uint32_t kListTokens = 1024;    // of one table of token entries (listed tokens)
+constexpr float kPScale = 32768.0f;       // probabilities are multiplied by this before they become 16-bit floats, see below
+
+template <class T> constexpr int kQTerms = sizeof(T) == 4 ? 2 : 1;                  // 16-bit floats that a query element is split into
+template <class T> constexpr int kPTerms = std::is_same_v<T, bf16> ? 1 : 2;         // and a probability
+
+__device__ __forceinline__ float max_over_groups(float x)       // over the four lanes that share lane & 15
 {
-    __shared__ float q_s[256], p_s[256], red[4];
-    __shared__ uint64_t at_s[256];
-    __shared__ float sv_s[256];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, head = blockIdx.x % a.q_heads, row = blockIdx.x / a.q_heads;
-    const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
-    if (b >= a.n_requests) return;
-    const uint32_t kv = head / (a.q_heads / a.n_heads);
-    const int64_t cap = (int64_t)a.width * a.block_tokens;
-    int64_t len = a.lens[b];
-    if (len < 0) len = 0;
-    if (len > cap) len = cap;
-    int64_t seen = len;
-    if (a.cu_q && a.causal) seen = len - (a.cu_q[b + 1] - a.cu_q[b]) + (int64_t)(row - a.cu_q[b]) + 1;
-    if (seen > len) seen = len;
-    const int64_t items = a.found ? (int64_t)a.n_ids : seen;
-    const int32_t* ids = a.found ? a.ids + ((size_t)row * a.id_heads + head / (a.q_heads / a.id_heads)) * a.n_ids : nullptr;
-    if (tid < a.dim) q_s[tid] = to_float(((const T*)a.q)[(int64_t)row * a.q_row_stride + (int64_t)head * a.q_head_stride + tid]);
-    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
-    for (int64_t t0 = 0; t0 < items; t0 += 256) {
-        __syncthreads();
-        float s = -__builtin_inff();
-        uint64_t at = ~0ull;
-        float sv = 0.0f;
-        if (t0 + tid < items) {
-            const int64_t t = a.found ? (int64_t)(uint32_t)ids[t0 + tid] : t0 + tid;
-            const int32_t blk = t < seen ? a.table[(size_t)b * a.width + t / a.block_tokens] : -1;
-            if ((uint32_t)blk < a.n_blocks) {
-                const uint64_t bh = (uint64_t)blk * a.n_heads + kv;
-                at = (bh * a.block_tokens + t % a.block_tokens) * a.dim;
-                float dot = 0.0f;
-                for (uint32_t i = 0; i < a.dim / 4; i++) {
-                    float x[4];
-                    decode4<CODES>(*reinterpret_cast<const uint32_t*>(a.k_codes + at + 4 * i), x);
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float x)
+{
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ f16x2 as_f16x2(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+
+// Two signed bytes, each in the low half of a 16-bit lane of w (the high halves are 0), as 16-bit floats: with its sign bit turned a
+// byte is code + 128, and 0x6400 | b is the 16-bit float 1024 + b, so 1152 less is the code, exactly.
+__device__ __forceinline__ f16x2 bytes_to_f16(uint32_t w)
+{
+    return as_f16x2(w ^ 0x64806480u) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
+}
+
+// Eight consecutive codes of a row as 16-bit floats (exact for both kinds of codes).  Signed bytes come out in the order
+// 0 2 1 3 4 6 5 7, which the queries are laid out to match.
+template <int CODES> __device__ __forceinline__ f16x8 decode8(uint32_t w0, uint32_t w1)
+{
+    union { f16x8 v; f16x2 h[4]; } u;
+    if constexpr (CODES == HNSW_AMD_CODES_I8) {
+        u.h[0] = bytes_to_f16(w0 & 0x00ff00ffu);
+        u.h[1] = bytes_to_f16((w0 >> 8) & 0x00ff00ffu);
+        u.h[2] = bytes_to_f16(w1 & 0x00ff00ffu);
+        u.h[3] = bytes_to_f16((w1 >> 8) & 0x00ff00ffu);
+    } else {
+        u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
+        u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
+        u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
+        u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
+    }
+    return u.v;
+}
+constexpr int kOrderI8[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+
+// Byte b of eight rows' words (one word of each of two times four rows), as 16-bit floats: a column of the values.
+template <int CODES> __device__ __forceinline__ void decode_columns(const uint32_t (&w)[8], f16x8 (&out)[4])
+{
+    union U { f16x8 v; f16x2 h[4]; };
+    U u[4];
+    if constexpr (CODES == HNSW_AMD_CODES_I8) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) dot = __builtin_fmaf(x[j], q_s[4 * i + j], dot);
-                }
-                s = dot * a.k_scale[bh] * a.scale;
-                sv = a.v_scale[bh];
+        for (int b = 0; b < 4; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                u[b].h[j] = bytes_to_f16(__builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x0c000c00u | ((4u + b) << 16) | (uint32_t)b));
+    } else {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t* x = &w[4 * half];
+            const uint32_t a0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), a1 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+            const uint32_t c0 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u), c1 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+            const uint32_t t[4] = {__builtin_amdgcn_perm(c0, a0, 0x05040100u), __builtin_amdgcn_perm(c0, a0, 0x07060302u),
+                                   __builtin_amdgcn_perm(c1, a1, 0x05040100u), __builtin_amdgcn_perm(c1, a1, 0x07060302u)};
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                u[b].h[2 * half] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(t[b], 1.0f, false);
+                u[b].h[2 * half + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(t[b], 1.0f, true);
             }
         }
-        float top = s;
-#pragma unroll
-        for (int o2 = 32; o2 >= 1; o2 >>= 1) top = fmaxf(top, __shfl_xor(top, o2));
-        if (lane == 0) red[tid >> 6] = top;
-        __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]))), ref = mn == -__builtin_inff() ? 0.0f : mn;
-        const float p = expf(s - ref), shrink = expf(m - ref);
-        p_s[tid] = p; at_s[tid] = at; sv_s[tid] = sv;
-        float sum = p;
-#pragma unroll
-        for (int o2 = 32; o2 >= 1; o2 >>= 1) sum += __shfl_xor(sum, o2);
-        __syncthreads();
-        if (lane == 0) red[tid >> 6] = sum;
-        __syncthreads();
-        l = l * shrink + (red[0] + red[1] + red[2] + red[3]);
-        m = mn;
-        o *= shrink;
-        if (tid < a.dim)
-            for (int j = 0; j < 256; j++)
-                if (at_s[j] != ~0ull) {
-                    float x[4];
-                    decode4<CODES>(*reinterpret_cast<const uint32_t*>(a.v_codes + at_s[j] + (tid & ~3u)), x);
-                    o += p_s[j] * sv_s[j] * x[tid & 3];
-                }
     }
-    const size_t to = (size_t)row * a.q_heads + head;
-    if (tid < a.dim) ((T*)a.out)[to * a.dim + tid] = from_float<T>(l > 0.0f ? o / l : (l == 0.0f ? 0.0f : l));
-    if (tid == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : m + logf(l);
+#pragma unroll
+    for (int b = 0; b < 4; b++) out[b] = u[b].v;
+}
+
+// Where a request's rows lie among the query rows, kept within n_rows whatever cu_q holds.
+struct Span { uint32_t first, count; };
+__device__ __forceinline__ Span rows_of(const AttendArgs& a, uint32_t b)
+{
+    if (!a.cu_q) return {b, 1};
+    const int64_t lo = min(max((int64_t)a.cu_q[b], (int64_t)0), (int64_t)a.n_rows), hi = min(max((int64_t)a.cu_q[b + 1], lo), (int64_t)a.n_rows);
+    return {(uint32_t)lo, (uint32_t)(hi - lo)};
+}
+__device__ __forceinline__ uint32_t length_of(const AttendArgs& a, uint32_t b)
+{
+    const int64_t cap = (int64_t)a.width * a.block_tokens;
+    return (uint32_t)min(max((int64_t)a.lens[b], (int64_t)0), cap);
+}
+// tokens that row i of a request's n rows sees
+__device__ __forceinline__ uint32_t seen_by(const AttendArgs& a, uint32_t len, uint32_t n, uint32_t i)
+{
+    if (!a.causal) return len;
+    const int64_t s = (int64_t)len - n + i + 1;
+    return (uint32_t)min(max(s, (int64_t)0), (int64_t)len);
+}
+
+// Unit u of the rows cut into tiles of `tile` (row, head) pairs, request after request: its request and the tile within it; false
+// when there are fewer units.
+__device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_t group, uint32_t tile, uint32_t lane, uint32_t& request, uint32_t& part)
+{
+    if (!a.cu_q) {
+        const uint32_t per = (group + tile - 1) / tile;
+        request = u / per;
+        part = u - request * per;
+        return request < a.n_requests;
+    }
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.n_requests; b0 += 64) {
+        uint32_t n = 0;
+        if (b0 + lane < a.n_requests) n = (uint32_t)(((uint64_t)rows_of(a, b0 + lane).count * group + tile - 1) / tile);
+        uint32_t upto = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(upto, off);
+            if (lane >= (uint32_t)off) upto += y;
+        }
+        const unsigned long long m = __ballot(before + upto > u);
+        if (m) {
+            const int at = __builtin_ctzll(m);
+            request = b0 + at;
+            part = u - before - (__shfl(upto, at) - __shfl(n, at));
+            return true;
+        }
+        before += __shfl(upto, 63);
+    }
+    return false;
+}
+
+struct Partials {
+    float* out;        // [n_rows][q_heads][n_splits][dim], divided by the split's sum
+    float* lse;        // [n_rows][q_heads][n_splits], in base 2
+    uint32_t n_splits, chunk;
+};
+
+// Attention of few query rows over many tokens: for single tokens the codes are read once and that is the time.
+//
+// The workgroup takes one key head of one request (or one list), up to 16 * MT rows of queries and one chunk of the tokens; its
+// four wavefronts take tiles of 32 tokens in turn, each with a softmax of its own, and join at the end.  Scores are computed
+// transposed, S^T = K Q^T, with v_mfma_f32_16x16x32_f16: the lane that then holds scores of query (lane & 15) is the one that needs
+// their probabilities as the operand of O^T = V^T P^T, so that nothing is exchanged between lanes, and the softmax's maximum and
+// sum are scalars of a lane.  Codes go from memory to registers as the matrix instructions want them, without LDS:
+//   keys    lane (m, g): row m of 16, 16-byte pieces g, g + 4, ... (the order of the dims is free as long as the queries have it too)
+//   values  lane (m, g): the same DP / 16 bytes of rows 4g .. 4g + 3 of both halves of the tile; a byte of eight rows is an operand
+// and the next tile is under way while one is computed.  Codes become 16-bit floats, which hold both kinds exactly.
+// Queries are scaled by a power of two to just under 2^15 and rounded to 16-bit floats (nothing is lost of bf16 and f16 but what
+// lies 2^-29 under the row's largest element); 32-bit queries are split into two terms.  A block's key scale multiplies the
+// scores; its value scale, over the largest of the table's, multiplies the probabilities, which as 16-bit floats in units of 2^-15
+// reach down to 2^-39 of the largest: 2^-11 of each is rounded away for bf16 rows (whose outputs keep 2^-8), and a second term
+// takes that up for the others.  Sums, maxima and outputs are in 32 bits.
+template <class T, int CODES, int DP, int MT, bool FOUND>
+__global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
+{
+    constexpr int KS = DP / 32, KW = DP / 64, VW = DP / 64, VB = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
+    constexpr uint32_t kEntries = FOUND ? kListTokens + kTile : kScanTokens / 16 + 2;
+    constexpr int kOutLd = DP + 4;
+    __shared__ uint32_t ent_row[kEntries];                      // first row of a block's (a token's) codes, in rows of dim bytes; ~0: there is none
+    __shared__ __align__(16) float ent_k[kEntries], ent_v[kEntries];         // its scales (values: see pw below)
+    __shared__ __align__(16) float join[2][16 * MT][kOutLd];
+    __shared__ float join_m[kWaves][16 * MT], join_l[kWaves][16 * MT], red[kWaves];
+    __shared__ uint32_t red_n[kWaves];
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t head = blockIdx.x % heads, unit = blockIdx.x / heads, split = blockIdx.y;
+    const uint32_t dim = a.dim, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs);
+    const uint32_t group = a.q_heads / heads;                   // rows of a token: query heads that share this key head, or list
+    const uint32_t kv = FOUND ? head / (heads / a.n_heads) : head;
+
+    // which rows: `first` + r / group is the query row of row r, head * group + r % group its head
+    uint32_t b, first, count, r0;
+    if constexpr (FOUND) {
+        const uint32_t per = (group + 16 * MT - 1) / (16 * MT);
+        first = unit / per;
+        r0 = (unit - first * per) * 16 * MT;
+        if (first >= a.n_rows) return;
+        b = a.cu_q ? request_of(a.cu_q, a.n_requests, first) : first;
+        if (b >= a.n_requests) return;
+        count = 1;
+    } else {
+        uint32_t part;
+        if (!unit_of(a, unit, group, 16 * MT, lane, b, part)) return;
+        const Span s = rows_of(a, b);
+        first = s.first;
+        count = s.count;
+        r0 = part * 16 * MT;
+    }
+    const uint32_t n_r = count * group;                         // (fits: n_rows * q_heads < 2^31)
+    if (r0 >= n_r) return;
+    const uint32_t len = length_of(a, b);
+
+    // the rows of this lane's columns, what they see, and the queries
+    uint32_t seen[MT], least = 0xffffffffu, most = 0;
+    f16x8 q[MT][KS][QT];
+    float factor[MT];                                           // of the products: scores in base 2
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;           // (goes into the queries, so that factors are not negative)
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const uint32_t r = r0 + 16 * mt + m;
+        const bool there = r < n_r;
+        uint32_t i = there ? r / group : 0;
+        const uint32_t h = head * group + (there ? r - i * group : 0);
+        if constexpr (FOUND) {
+            const Span s = rows_of(a, b);
+            seen[mt] = seen_by(a, len, s.count, first - s.first);
+        } else {
+            seen[mt] = there ? seen_by(a, len, count, i) : 0;
+        }
+        if (there) { least = min(least, seen[mt]); most = max(most, seen[mt]); }
+        const T* x = (const T*)a.q + (int64_t)(first + i) * a.q_row_stride + (int64_t)h * a.q_head_stride;
+        float v[KS][8], top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const uint32_t col = 64 * (s / 2) + 16 * g + 8 * (s % 2);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[s][j] = 0.0f;
+            if (there && col < dim) {
+                if (q_vec) load8<T, true>(x + col, v[s]);
+                else load8<T, false>(x + col, v[s]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[s][j]));
+        }
+        top = max_over_groups(top);
+        int e = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;      // top * 2^e in [2^14, 2^15)
+        factor[mt] = fabsf(a.scale) * kLog2e;
+        factor[mt] = ldexpf(factor[mt], -e);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = ldexpf(v[s][CODES == HNSW_AMD_CODES_I8 ? kOrderI8[j] : j] * sign, e);
+                const _Float16 hi = (_Float16)y;
+                q[mt][s][0][j] = hi;
+                if constexpr (QT == 2) q[mt][s][1][j] = (_Float16)(y - (float)hi);
+            }
+    }
+    // (over the lanes that share g, i.e. over all rows of the tile)
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+        least = min(least, (uint32_t)__shfl_xor((int)least, off));
+        most = max(most, (uint32_t)__shfl_xor((int)most, off));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+
+    const uint32_t all = FOUND ? a.n_ids : most;                // items: tokens, or list entries
+    const uint32_t begin = split * parts.chunk;
+    if (!FOUND && split > 0 && begin >= all) return;            // (a row that sees no token of a chunk does not ask for its part)
+    const uint32_t end = split + 1 < parts.n_splits ? min(begin + parts.chunk, all) : all;
+
+    f32x4 o[MT][VB];
+    float top[MT], sum[MT], unit_v = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        top[mt] = -__builtin_inff();
+        sum[mt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VB; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    constexpr uint32_t kTable = FOUND ? kListTokens : kScanTokens;
+    for (uint32_t c0 = begin; c0 < end; c0 += kTable) {
+        const uint32_t c1 = min(end - c0, kTable) + c0;
+        uint32_t n = c1 - c0, e0 = 0;                           // items in the table
+        float largest = 0.0f;
+        if (c0 != begin) __syncthreads();                       // the table's last readers are done
+        if constexpr (FOUND) {
+            // listed tokens that the row sees and that exist, moved together (in order): entries, then 32 or less that weigh nothing
+            const int32_t* ids = a.ids + ((size_t)first * heads + head) * a.n_ids;
+            uint32_t kept = 0;
+            for (uint32_t i0 = 0; i0 < n; i0 += 256) {
+                const uint32_t i = i0 + tid;
+                uint32_t row = ~0u;
+                float sk = 0.0f, sv = 0.0f;
+                if (i < n) {
+                    const uint32_t t = (uint32_t)ids[c0 + i];
+                    if (t < seen[0]) {
+                        const uint32_t blk = (uint32_t)a.table[(size_t)b * a.width + (t >> bs_log)];
+                        if (blk < a.n_blocks) {
+                            const uint32_t bh = blk * a.n_heads + kv;
+                            row = (bh << bs_log) + (t & (bs - 1));
+                            sk = a.k_scale[bh];
+                            sv = a.v_scale[bh];
+                        }
+                    }
+                }
+                const unsigned long long mine = __ballot(row != ~0u);
+                if (i0) __syncthreads();
+                if (lane == 0) red_n[wave] = (uint32_t)__popcll(mine);
+                __syncthreads();
+                uint32_t at = kept + (uint32_t)__popcll(mine & ((1ull << lane) - 1));
+                for (uint32_t w = 0; w < kWaves; w++) {
+                    if (w < wave) at += red_n[w];
+                    kept += red_n[w];
+                }
+                if (row != ~0u) { ent_row[at] = row; ent_k[at] = sk; ent_v[at] = sv; largest = fmaxf(largest, sv); }
+            }
+            n = kept;
+            __syncthreads();
+            if (tid < kTile && n > 0) { ent_row[n + tid] = ent_row[n - 1]; ent_k[n + tid] = 0.0f; ent_v[n + tid] = 0.0f; }
+        } else {
+            e0 = c0 >> bs_log;
+            const uint32_t n_e = ((c1 - 1) >> bs_log) - e0 + 1;
+            for (uint32_t i = tid; i < n_e; i += 256) {
+                const uint32_t blk = (uint32_t)a.table[(size_t)b * a.width + e0 + i];
+                uint32_t row = ~0u;
+                float sk = 0.0f, sv = 0.0f;
+                if (blk < a.n_blocks) {
+                    const uint32_t bh = blk * a.n_heads + kv;
+                    row = bh << bs_log;
+                    sk = a.k_scale[bh];
+                    sv = a.v_scale[bh];
+                }
+                ent_row[i] = row; ent_k[i] = sk; ent_v[i] = sv;
+                largest = fmaxf(largest, sv);
+            }
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
+        if (lane == 0) red[wave] = largest;
+        __syncthreads();
+        largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
+        if (largest > 0.0f) {
+            if (unit_v > 0.0f && unit_v != largest) {           // outputs so far are in units of the last table's largest scale
+                const float change = unit_v / largest;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < VB; i++) o[mt][i] *= change;
+            }
+            unit_v = largest;
+        }
+
+        // a tile's codes: where they are, and the loads
+        struct Tile { u32x4 k[2][KW]; uint32_t v[8][VW]; uint32_t row[2]; };
+        const uint32_t k_col = min(16 * g, dim - 16), v_col = VB * m;
+        auto fetch = [&](uint32_t j, Tile& t) {
+            const uint32_t i0 = 32 * j;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t row_k, row_v[4];
+                const uint8_t *kb = a.k_codes, *vb = a.v_codes;
+                if constexpr (FOUND) {
+                    row_k = ent_row[i0 + 16 * h + m];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) row_v[r] = ent_row[i0 + 16 * h + 4 * g + r];
+                    t.row[h] = 0;
+                } else {
+                    const uint32_t last = c1 - 1, start = min(c0 + i0 + 16 * h, last);
+                    uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
+                    t.row[h] = base;
+                    if (base == ~0u) base = 0;                  // (loads stay inside, the values are dropped)
+                    const uint64_t at = (uint64_t)(base + (start & (bs - 1))) * dim;
+                    kb += at;
+                    vb += at;
+                    row_k = min(m, last - start);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) row_v[r] = min(4 * g + r, last - start);
+                }
+                auto offset = [&](uint32_t row) { if constexpr (FOUND) return (uint64_t)row * dim; else return row * dim; };
+#pragma unroll
+                for (int i = 0; i < KW; i++)
+                    t.k[h][i] = *reinterpret_cast<const u32x4*>(kb + offset(row_k) + (64 * i + 16 * g < dim ? 64 * i + 16 * g : k_col));
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint8_t* p = vb + offset(row_v[r]);
+                    if constexpr (VW == 2) {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(p + (v_col + 8 <= dim ? v_col : 0));
+                        t.v[4 * h + r][0] = w[0]; t.v[4 * h + r][1] = w[1];
+                    } else if constexpr (VW == 4) {
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(p + (v_col + 16 <= dim ? v_col : 0));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) t.v[4 * h + r][i] = w[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VW; i++) t.v[4 * h + r][i] = *reinterpret_cast<const uint32_t*>(p + (v_col + 4 * i + 4 <= dim ? v_col + 4 * i : 0));
+                    }
+                }
+            }
+        };
+        auto take = [&](uint32_t j, Tile& t) {
+            const uint32_t i0 = 32 * j;
+            f32x4 s[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const f16x8 k = decode8<CODES>(t.k[h][ks / 2][2 * (ks % 2)], t.k[h][ks / 2][2 * (ks % 2) + 1]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int qt = 0; qt < QT; qt++) s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], s[mt][h], 0, 0, 0);
+                }
+            float fk[2][4], pw[2][4];                           // the scales of this lane's tokens 4g + r of both halves
+            bool gone[2] = {false, false}, ragged;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if constexpr (FOUND) {
+                    const float4 x = *reinterpret_cast<const float4*>(&ent_k[i0 + 16 * h + 4 * g]), y = *reinterpret_cast<const float4*>(&ent_v[i0 + 16 * h + 4 * g]);
+                    fk[h][0] = x.x; fk[h][1] = x.y; fk[h][2] = x.z; fk[h][3] = x.w;
+                    pw[h][0] = y.x * per_v; pw[h][1] = y.y * per_v; pw[h][2] = y.z * per_v; pw[h][3] = y.w * per_v;
+                } else {
+                    const uint32_t e = (min(c0 + i0 + 16 * h, c1 - 1) >> bs_log) - e0;
+                    const float x = ent_k[e], y = ent_v[e] * per_v;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) { fk[h][r] = x; pw[h][r] = y; }
+                    gone[h] = t.row[h] == ~0u;
+                }
+            }
+            if constexpr (FOUND) ragged = i0 + 32 > n;
+            else ragged = c0 + i0 + 32 > least || c0 + i0 + 32 > c1 || gone[0] || gone[1];
+            f16x8 p[MT][PT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                float x[2][4], local = -__builtin_inff();
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[h][r] = s[mt][h][r] * (fk[h][r] * factor[mt]);
+                if (ragged) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const uint32_t i = i0 + 16 * h + 4 * g + r;
+                            const bool sees = FOUND ? i < n : (c0 + i < min(seen[mt], c1) && !gone[h]);
+                            x[h][r] = sees ? x[h][r] : -__builtin_inff();
+                        }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) local = fmaxf(local, x[h][r]);
+                if (__ballot(local > top[mt])) {                // rare after the first tiles: a new maximum
+                    const float now = fmaxf(top[mt], max_over_groups(local));
+                    const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
+                    top[mt] = now;
+                    sum[mt] *= shrink;
+#pragma unroll
+                    for (int i = 0; i < VB; i++) o[mt][i] *= shrink;
+                }
+                const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float y = __builtin_amdgcn_exp2f(x[h][r] - ref);
+                        sum[mt] += y;
+                        const float w = y * pw[h][r];
+                        const _Float16 hi = (_Float16)w;
+                        p[mt][0][4 * h + r] = hi;
+                        if constexpr (PT == 2) p[mt][1][4 * h + r] = (_Float16)(w - (float)hi);
+                    }
+            }
+            if constexpr (!FOUND) {
+                if (gone[0] || gone[1]) {
+#pragma unroll
+                    for (int r = 0; r < 8; r++)
+#pragma unroll
+                        for (int i = 0; i < VW; i++) t.v[r][i] = gone[r / 4] ? 0u : t.v[r][i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VW; i++) {
+                uint32_t w[8];
+                f16x8 v[4];
+#pragma unroll
+                for (int r = 0; r < 8; r++) w[r] = t.v[r][i];
+                decode_columns<CODES>(w, v);
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int pt = 0; pt < PT; pt++) o[mt][4 * i + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p[mt][pt], o[mt][4 * i + c], 0, 0, 0);
+            }
+        };
+        const uint32_t tiles = (n + kTile - 1) / kTile;
+        if (wave < tiles) {
+            Tile t[2];
+            fetch(wave, t[0]);
+            for (uint32_t j = wave; j < tiles; j += 2 * kWaves) {
+                if (j + kWaves < tiles) fetch(j + kWaves, t[1]);
+                take(j, t[0]);
+                if (j + kWaves >= tiles) break;
+                if (j + 2 * kWaves < tiles) fetch(j + 2 * kWaves, t[0]);
+                take(j + kWaves, t[1]);
+            }
+        }
+    }
+
+    // the four wavefronts' softmaxes become one
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        sum[mt] = sum_over_groups(sum[mt]);
+        if (g == 0) { join_m[wave][16 * mt + m] = top[mt]; join_l[wave][16 * mt + m] = sum[mt]; }
+    }
+    __syncthreads();
+    auto ref_of = [&](uint32_t r) {
+        const float x = fmaxf(fmaxf(join_m[0][r], join_m[1][r]), fmaxf(join_m[2][r], join_m[3][r]));
+        return x == -__builtin_inff() ? 0.0f : x;
+    };
+    auto put = [&](bool add) {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            const float f = __builtin_amdgcn_exp2f(top[mt] - ref_of(16 * mt + m));
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int i = 0; i < VB; i += 4) {
+                    float4* to = reinterpret_cast<float4*>(&join[wave & 1][16 * mt + m][(4 * g + r) * VB + i]);
+                    float4 x = make_float4(o[mt][i][r] * f, o[mt][i + 1][r] * f, o[mt][i + 2][r] * f, o[mt][i + 3][r] * f);
+                    if (add) { const float4 y = *to; x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); }
+                    *to = x;
+                }
+        }
+    };
+    if (wave >= 2) put(false);
+    __syncthreads();
+    if (wave < 2) put(true);
+    __syncthreads();
+    const float unit_o = unit_v / kPScale;
+    for (uint32_t r = wave; r < 16 * MT && r0 + r < n_r; r += kWaves) {
+        const uint32_t i = (r0 + r) / group;
+        const size_t to = (size_t)(first + i) * a.q_heads + head * group + (r0 + r - i * group);
+        const float ref = ref_of(r);
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) l += join_l[w][r] * __builtin_amdgcn_exp2f(join_m[w][r] - ref);
+        const float inv = l == 0.0f ? 0.0f : unit_o / l;
+        if (parts.n_splits == 1) {
+            for (uint32_t d = lane; d < dim; d += 64) ((T*)a.out)[to * dim + d] = from_float<T>((join[0][r][d] + join[1][r][d]) * inv);
+            if (lane == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        } else {
+            const size_t at = to * parts.n_splits + split;
+            for (uint32_t d = lane; d < dim; d += 64) parts.out[at * dim + d] = (join[0][r][d] + join[1][r][d]) * inv;
+            if (lane == 0) parts.lse[at] = l == 0.0f ? -__builtin_inff() : ref + __builtin_amdgcn_logf(l);
+        }
+    }
+}
+
+// The chunks' outputs of a row and head become one: weights 2^(lse - largest).  One wavefront each.
+template <class T>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials parts)
+{
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t to = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (to >= (uint64_t)a.n_rows * a.q_heads) return;
+    const uint32_t row = (uint32_t)(to / a.q_heads);
+    const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
+    if (b >= a.n_requests) return;
+    uint32_t n = parts.n_splits;
+    if (!a.found) {
+        const Span s = rows_of(a, b);
+        const uint32_t sees = seen_by(a, length_of(a, b), s.count, row - s.first);
+        n = min(n, (uint32_t)(((uint64_t)sees + parts.chunk - 1) / parts.chunk));
+    }
+    const float* lse = parts.lse + to * parts.n_splits;
+    const float* x = parts.out + to * parts.n_splits * a.dim;
+    float top = -__builtin_inff();
+    for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, lse[i]);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.0f;
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+        const float w = i0 + lane < n ? __builtin_amdgcn_exp2f(lse[i0 + lane] - ref) : 0.0f;
+        l += w;
+        const uint32_t here = min(n - i0, 64u);
+        for (uint32_t i = 0; i < here; i++) {
+            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (lane + 64 * c < a.dim) o[c] += f * x[(size_t)(i0 + i) * a.dim + lane + 64 * c];
+        }
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+        if (lane + 64 * c < a.dim) ((T*)a.out)[to * a.dim + lane + 64 * c] = from_float<T>(o[c] * inv);
+    if (lane == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 }  // namespace
@@ -108,14 +632,61 @@ static void check_attend(const hnsw_amd_token_cache* c, const AttendArgs& a, con
     if (a.n_requests < 1) throw std::invalid_argument(w + ": no requests");
     if (a.width < 1 || (uint64_t)a.width * c->block_tokens > 0x7fffffffull) throw std::invalid_argument(w + ": the table's width in tokens must be 1..2^31 - 1");
     if (!a.cu_q && a.n_rows != a.n_requests) throw std::invalid_argument(w + ": without cu_q there is one query row for each request");
-    if (a.n_rows > 0x7fffffffu || (uint64_t)a.n_rows * a.q_heads > 0x7fffffffull) throw std::invalid_argument(w + ": too many rows and heads for one call");
+    if (a.n_rows > 0x7fffffffu || (uint64_t)a.n_rows * a.q_heads >= 1ull << 26) throw std::invalid_argument(w + ": too many rows and heads for one call");
     if (a.found && (a.id_heads < 1 || a.id_heads % c->n_heads || a.q_heads % a.id_heads))
         throw std::invalid_argument(w + ": the lists' heads must be a multiple of the cache's heads and divide the query heads");
     if (!(a.scale == a.scale) || a.scale - a.scale != 0.0f) throw std::invalid_argument(w + ": scale must be finite");
 }
 
-uint64_t attend_workspace(const hnsw_amd_token_cache*, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) { return 0; }
-uint64_t attend_found_workspace(const hnsw_amd_token_cache*, uint32_t, uint32_t, uint32_t, uint32_t) { return 0; }
+// How a call's work is cut: units (rows) x heads x chunks of the items (tokens, or list entries).
+struct Cut { uint32_t mt, units, heads, chunk, n_splits; };
+
+static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_requests, uint32_t heads, uint32_t items, bool by_request, bool ragged)
+{
+    Cut c{};
+    c.heads = heads;
+    const uint32_t group = q_heads / heads;
+    // one tile of 16 rows, or two where that many rows share the tokens: the codes are decoded once for both (beyond 128 dims two
+    // tiles' outputs do not fit the registers)
+    const double rows = (double)group * (by_request ? (double)n_rows / n_requests : 1.0);
+    c.mt = rows > 16.0 && dim <= 128 ? 2 : 1;
+    const uint32_t tile = 16 * c.mt;
+    if (by_request && ragged) c.units = n_requests + (uint32_t)((uint64_t)n_rows * group / tile);
+    else c.units = (by_request ? n_requests : n_rows) * ((group + tile - 1) / tile);
+    // chunks: enough workgroups to fill the GPU twice over, none shorter than 128 items
+    const uint64_t wanted = 1024, have = (uint64_t)c.units * heads;
+    uint64_t splits = have ? (wanted + have - 1) / have : 1;
+    const uint64_t step = (uint64_t)kWaves * kTile;
+    uint64_t chunk = (((uint64_t)items + splits - 1) / splits + step - 1) / step * step;
+    if (chunk < step) chunk = step;
+    c.chunk = (uint32_t)chunk;
+    splits = ((uint64_t)items + chunk - 1) / chunk;
+    c.n_splits = splits ? (uint32_t)splits : 1;
+    return c;
+}
+
+static uint64_t workspace_of(const Cut& c, uint32_t n_rows, uint32_t q_heads, uint32_t dim)
+{
+    return c.n_splits == 1 ? 0 : (uint64_t)n_rows * q_heads * c.n_splits * (dim + 1) * 4;
+}
+
+static uint32_t items_of(uint32_t width, uint32_t block_tokens, uint32_t max_len)
+{
+    const uint64_t cap = (uint64_t)width * block_tokens;
+    return (uint32_t)(max_len && max_len < cap ? max_len : (cap < 0x7fffffffull ? cap : 0x7fffffffull));
+}
+
+uint64_t attend_workspace(const hnsw_amd_token_cache* c, uint32_t n_rows, uint32_t q_heads, uint32_t n_requests, uint32_t width, uint32_t max_len)
+{
+    if (!c->n_heads || !n_requests || !q_heads || q_heads % c->n_heads) return 0;      // (the call itself says what is wrong)
+    return workspace_of(cut_work(c->dim, n_rows, q_heads, n_requests, c->n_heads, items_of(width, c->block_tokens, max_len), true, n_rows != n_requests), n_rows, q_heads, c->dim);
+}
+
+uint64_t attend_found_workspace(const hnsw_amd_token_cache* c, uint32_t n_rows, uint32_t q_heads, uint32_t id_heads, uint32_t n_ids)
+{
+    if (!id_heads || !q_heads || q_heads % id_heads) return 0;
+    return workspace_of(cut_work(c->dim, n_rows, q_heads, n_rows, id_heads, n_ids, false, false), n_rows, q_heads, c->dim);
+}
 
 void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows, uint32_t q_heads, int64_t q_row_stride, int64_t q_head_stride,
                   uint32_t row_type, const int32_t* table, uint32_t width, const int32_t* lens, uint32_t n_requests, const int32_t* cu_q,
@@ -128,13 +699,43 @@ void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows,
                  q, q_row_stride, q_head_stride, n_rows, q_heads, table, lens, cu_q, ids, width, n_requests, n_ids, id_heads, causal, found ? 1 : 0, scale, out, lse};
     check_attend(c, a, who);
     check_row_type(row_type, who);
-    (void)max_len; (void)workspace; (void)workspace_bytes;
     if (n_rows == 0) return;
+    const Cut cut = found ? cut_work(c->dim, n_rows, q_heads, n_rows, id_heads, n_ids, false, false)
+                          : cut_work(c->dim, n_rows, q_heads, n_requests, c->n_heads, items_of(width, c->block_tokens, max_len), true, n_rows != n_requests);
+    const uint64_t need = workspace_of(cut, n_rows, q_heads, c->dim);
+    if (need > workspace_bytes || (need && !workspace)) throw std::invalid_argument(std::string(who) + ": the workspace is too small");
+    if (reinterpret_cast<uintptr_t>(workspace) & 15u) throw std::invalid_argument(std::string(who) + ": the workspace must be aligned to 16 bytes");
+    if ((uint64_t)cut.units * cut.heads >= 1ull << 24 || cut.n_splits > 65535u) throw std::invalid_argument(std::string(who) + ": too much work for one call");
     const OnDevice on(device);
+    Partials parts{(float*)workspace, (float*)workspace + (uint64_t)n_rows * q_heads * cut.n_splits * c->dim, cut.n_splits, cut.chunk};
     by_types(row_type, c->codes, [&](auto t, auto codes) {
-        hipLaunchKernelGGL((attend_simple_kernel<decltype(t), codes.value>), dim3(n_rows * q_heads), dim3(256), 0, (hipStream_t)stream, a);
+        using T = decltype(t);
+        const int64_t step = 16 / (int64_t)sizeof(T);
+        const uint32_t q_vec = (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && q_row_stride % step == 0 && q_head_stride % step == 0;
+        auto go = [&](auto dp, auto mt, auto f) {
+            hipLaunchKernelGGL((attend_rows_kernel<T, codes.value, dp.value, mt.value, f.value>), dim3(cut.units * cut.heads, cut.n_splits), dim3(256), 0,
+                               (hipStream_t)stream, a, parts, cut.heads, q_vec);
+        };
+        auto by_rows = [&](auto dp, auto f) {
+            if constexpr (dp.value <= 128) {
+                if (cut.mt == 2) return go(dp, std::integral_constant<int, 2>{}, f);
+            }
+            go(dp, std::integral_constant<int, 1>{}, f);
+        };
+        auto by_kind = [&](auto dp) {
+            if (found) by_rows(dp, std::true_type{});
+            else by_rows(dp, std::false_type{});
+        };
+        if (c->dim <= 64) by_kind(std::integral_constant<int, 64>{});
+        else if (c->dim <= 128) by_kind(std::integral_constant<int, 128>{});
+        else if (c->dim <= 192) by_kind(std::integral_constant<int, 192>{});
+        else by_kind(std::integral_constant<int, 256>{});
+        check_launch(who);
+        if (cut.n_splits > 1) {
+            hipLaunchKernelGGL((attend_join_kernel<T>), dim3((uint32_t)(((uint64_t)n_rows * q_heads + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a, parts);
+            check_launch(who);
+        }
     });
-    check_launch(who);
 }
 
 }  // namespace hnsw_amd

@@ -358,7 +358,7 @@ void cache_append(const hnsw_amd_token_cache* c, const void* k, const void* v, u
     // prompt): it looks at a block's worth, most of which are one run.
     a.span = (uint64_t)n_rows * c->n_heads <= 16384 ? 1 : c->block_tokens;
     const uint64_t units = (uint64_t)((n_rows + a.span - 1) / a.span) * c->n_heads * 2, groups = (units + 3) / 4;
-    if (groups > 0x7fffffffull) throw std::invalid_argument("cache_append: too many rows and heads for one call");
+    if (groups >= 1ull << 24) throw std::invalid_argument("cache_append: too many rows and heads for one call");
     by_types(row_type, c->codes, [&](auto t, auto codes) {
         using T = decltype(t);
         const int64_t step = 16 / (int64_t)sizeof(T);
@@ -376,7 +376,7 @@ void cache_read(const hnsw_amd_token_cache* c, const int64_t* slots, uint32_t n_
     if (n_rows == 0 || (!k && !v)) return;
     if (!aligned16(k) || !aligned16(v)) throw std::invalid_argument("cache_read: outputs must be aligned to 16 bytes");
     const uint64_t groups = ((uint64_t)n_rows * c->n_heads * (c->dim / 8) + 255) / 256;
-    if (groups > 0x7fffffffull) throw std::invalid_argument("cache_read: too many rows for one call");
+    if (groups >= 1ull << 24) throw std::invalid_argument("cache_read: too many rows for one call");
     const OnDevice on(device);
     const ReadArgs a{{(const uint8_t*)c->k_codes, (const uint8_t*)c->v_codes}, {c->k_scale, c->v_scale}, {k, v}, slots, n_rows, c->n_blocks, c->n_heads, c->block_tokens, c->dim};
     by_types(row_type, c->codes, [&](auto t, auto codes) {
