@@ -161,6 +161,64 @@ __device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_
     return false;
 }
 
+// A query row's operands, eight elements from column col(s) on for step s, and what the products with codes are multiplied by to be
+// scores in base 2.  The row is scaled by the power of two that puts its largest element into [2^14, 2^15).  The four lanes that
+// share a row call this together.
+template <class T, int CODES, int KS, int QT, class Col>
+__device__ __forceinline__ float load_query(const AttendArgs& a, bool there, uint32_t row, uint32_t head, uint32_t vec, Col&& col, f16x8 (&q)[KS][QT])
+{
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;           // (goes into the queries, so that factors are not negative)
+    const T* x = (const T*)a.q + (int64_t)row * a.q_row_stride + (int64_t)head * a.q_head_stride;
+    float v[KS][8], top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const uint32_t c = col(s);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[s][j] = 0.0f;
+        if (there && c < a.dim) {
+            if (vec) load8<T, true>(x + c, v[s]);
+            else load8<T, false>(x + c, v[s]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[s][j]));
+    }
+    top = max_over_groups(top);
+    const int e = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float y = ldexpf(v[s][CODES == HNSW_AMD_CODES_I8 ? kOrderI8[j] : j] * sign, e);
+            const _Float16 hi = (_Float16)y;
+            q[s][0][j] = hi;
+            if constexpr (QT == 2) q[s][1][j] = (_Float16)(y - (float)hi);
+        }
+    return ldexpf(fabsf(a.scale) * kLog2e, -e);
+}
+
+// Block entries of the tokens c0 .. c1 of request b into LDS (whole workgroup): first row of a block's codes in rows of dim bytes, ~0
+// where there is no block, and its scales.  Returns the largest value scale that this thread saw.
+__device__ __forceinline__ float table_entries(const AttendArgs& a, uint32_t b, uint32_t kv, uint32_t bs_log, uint32_t c0, uint32_t c1, uint32_t tid,
+                                               uint32_t threads, uint32_t* ent_row, float* ent_k, float* ent_v)
+{
+    const uint32_t e0 = c0 >> bs_log, n_e = ((c1 - 1) >> bs_log) - e0 + 1;
+    float largest = 0.0f;
+    for (uint32_t i = tid; i < n_e; i += threads) {
+        const uint32_t blk = (uint32_t)a.table[(size_t)b * a.width + e0 + i];
+        uint32_t row = ~0u;
+        float sk = 0.0f, sv = 0.0f;
+        if (blk < a.n_blocks) {
+            const uint32_t bh = blk * a.n_heads + kv;
+            row = bh << bs_log;
+            sk = a.k_scale[bh];
+            sv = a.v_scale[bh];
+        }
+        ent_row[i] = row; ent_k[i] = sk; ent_v[i] = sv;
+        largest = fmaxf(largest, sv);
+    }
+    return largest;
+}
+
 struct Partials {
     float* out;        // [n_rows][q_heads][n_splits][dim], divided by the split's sum
     float* lse;        // [n_rows][q_heads][n_splits], in base 2
@@ -227,13 +285,11 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
     uint32_t seen[MT], least = 0xffffffffu, most = 0;
     f16x8 q[MT][KS][QT];
     float factor[MT];                                           // of the products: scores in base 2
-    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;           // (goes into the queries, so that factors are not negative)
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
         const uint32_t r = r0 + 16 * mt + m;
         const bool there = r < n_r;
-        uint32_t i = there ? r / group : 0;
-        const uint32_t h = head * group + (there ? r - i * group : 0);
+        const uint32_t i = there ? r / group : 0, h = head * group + (there ? r - i * group : 0);
         if constexpr (FOUND) {
             const Span s = rows_of(a, b);
             seen[mt] = seen_by(a, len, s.count, first - s.first);
@@ -241,33 +297,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
             seen[mt] = there ? seen_by(a, len, count, i) : 0;
         }
         if (there) { least = min(least, seen[mt]); most = max(most, seen[mt]); }
-        const T* x = (const T*)a.q + (int64_t)(first + i) * a.q_row_stride + (int64_t)h * a.q_head_stride;
-        float v[KS][8], top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const uint32_t col = 64 * (s / 2) + 16 * g + 8 * (s % 2);
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[s][j] = 0.0f;
-            if (there && col < dim) {
-                if (q_vec) load8<T, true>(x + col, v[s]);
-                else load8<T, false>(x + col, v[s]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[s][j]));
-        }
-        top = max_over_groups(top);
-        int e = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;      // top * 2^e in [2^14, 2^15)
-        factor[mt] = fabsf(a.scale) * kLog2e;
-        factor[mt] = ldexpf(factor[mt], -e);
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = ldexpf(v[s][CODES == HNSW_AMD_CODES_I8 ? kOrderI8[j] : j] * sign, e);
-                const _Float16 hi = (_Float16)y;
-                q[mt][s][0][j] = hi;
-                if constexpr (QT == 2) q[mt][s][1][j] = (_Float16)(y - (float)hi);
-            }
+        factor[mt] = load_query<T, CODES, KS, QT>(a, there, first + i, h, q_vec, [&](int s) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); }, q[mt]);
     }
     // (over the lanes that share g, i.e. over all rows of the tile)
 #pragma unroll
@@ -335,20 +365,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
             if (tid < kTile && n > 0) { ent_row[n + tid] = ent_row[n - 1]; ent_k[n + tid] = 0.0f; ent_v[n + tid] = 0.0f; }
         } else {
             e0 = c0 >> bs_log;
-            const uint32_t n_e = ((c1 - 1) >> bs_log) - e0 + 1;
-            for (uint32_t i = tid; i < n_e; i += 256) {
-                const uint32_t blk = (uint32_t)a.table[(size_t)b * a.width + e0 + i];
-                uint32_t row = ~0u;
-                float sk = 0.0f, sv = 0.0f;
-                if (blk < a.n_blocks) {
-                    const uint32_t bh = blk * a.n_heads + kv;
-                    row = bh << bs_log;
-                    sk = a.k_scale[bh];
-                    sv = a.v_scale[bh];
-                }
-                ent_row[i] = row; ent_k[i] = sk; ent_v[i] = sv;
-                largest = fmaxf(largest, sv);
-            }
+            largest = table_entries(a, b, kv, bs_log, c0, c1, tid, 256, ent_row, ent_k, ent_v);
         }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
@@ -578,14 +595,292 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
     }
 }
 
-// The chunks' outputs of a row and head become one: weights 2^(lse - largest).  One wavefront each.
+// Attention of many query rows: prompts.  The codes of 64 tokens become 16-bit floats once for all 64 * MT rows of the workgroup: in
+// LDS, keys [token][dim], values [dim][token] (the eight tokens of a matrix operand next to each other; rows of an odd number of
+// 16-byte pieces, so that operands are read without bank conflicts), while the next tile's codes are on their way to registers.
+// Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel, but that a block's value scale goes
+// into the exponent instead of being multiplied in: weights are 2^(score - maximum + log2 of the scale over the table's largest), their
+// sum is put right by the inverse per 16 tokens.
+template <class T, int CODES, int DP, int MT, int NBUF>
+__global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
+{
+    constexpr int KS = DP / 32, DT = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
+    constexpr int kTokens = 64, kKeyLd = DP + 8, kValLd = kTokens + 8;          // 16-bit elements
+    constexpr int KL = kTokens * (DP / 16) / 256;                               // 16-byte pieces of keys a thread moves
+    constexpr int kOcts = DP / 4 * (kTokens / 8), VL = (kOcts + 255) / 256;     // (word of 4 dims) x 8 tokens of values
+    constexpr uint32_t kEntries = kScanTokens / 16 + 2;
+    __shared__ uint32_t ent_row[kEntries];
+    __shared__ float ent_k[kEntries], ent_v[kEntries], red[kWaves];
+    __shared__ __align__(16) _Float16 keys[NBUF][kTokens * kKeyLd];
+    __shared__ __align__(16) _Float16 vals[NBUF][DP * kValLd];
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t kv = blockIdx.x % a.n_heads, split = blockIdx.y;
+    const uint32_t unit = gridDim.x / a.n_heads - 1 - blockIdx.x / a.n_heads;   // the last rows of a prompt see the most: first
+    const uint32_t dim = a.dim, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs);
+    const uint32_t group = a.q_heads / a.n_heads;
+    constexpr uint32_t kRows = kWaves * 16 * MT;
+    uint32_t b, part;
+    if (!unit_of(a, unit, group, kRows, lane, b, part)) return;
+    const Span rows = rows_of(a, b);
+    const uint32_t n_r = rows.count * group, r0 = part * kRows + wave * 16 * MT;
+    const uint32_t len = length_of(a, b);
+
+    uint32_t seen[MT], least = 0xffffffffu, most = 0;
+    f16x8 q[MT][KS][QT];
+    float factor[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const uint32_t r = r0 + 16 * mt + m;
+        const bool there = r < n_r;
+        const uint32_t i = there ? r / group : 0, h = kv * group + (there ? r - i * group : 0);
+        seen[mt] = there ? seen_by(a, len, rows.count, i) : 0;
+        if (there) { least = min(least, seen[mt]); most = max(most, seen[mt]); }
+        factor[mt] = load_query<T, CODES, KS, QT>(a, there, rows.first + i, h, q_vec, [&](int s) { return 32 * s + 8 * g; }, q[mt]);
+    }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+        least = min(least, (uint32_t)__shfl_xor((int)least, off));
+        most = max(most, (uint32_t)__shfl_xor((int)most, off));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    // what the workgroup's last row sees
+    const uint32_t last_r = min((part + 1) * kRows, n_r) - 1;
+    const uint32_t all = seen_by(a, len, rows.count, last_r / group);
+    const uint32_t begin = split * parts.chunk;
+    if (split > 0 && begin >= all) return;
+    const uint32_t end = split + 1 < parts.n_splits ? min(begin + parts.chunk, all) : all;
+
+    f32x4 o[MT][DT];
+    float top[MT], sum[MT], unit_v = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        top[mt] = -__builtin_inff();
+        sum[mt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (uint32_t c0 = begin; c0 < end; c0 += kScanTokens) {
+        const uint32_t c1 = min(end - c0, kScanTokens) + c0, e0 = c0 >> bs_log;
+        __syncthreads();                                        // the last table's readers are done
+        float largest = table_entries(a, b, kv, bs_log, c0, c1, tid, 256, ent_row, ent_k, ent_v);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
+        if (lane == 0) red[wave] = largest;
+        __syncthreads();
+        largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        if (largest > 0.0f) {
+            if (unit_v > 0.0f && unit_v != largest) {
+                const float change = unit_v / largest;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < DT; i++) o[mt][i] *= change;
+            }
+            unit_v = largest;
+        }
+        const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
+
+        u32x4 kr[KL];
+        uint32_t vr[VL][8];
+        // token t of the tile at t0: its row of codes (of the nearest token that is there; `gone`: of no block)
+        auto row_of = [&](uint32_t t, bool& gone) {
+            const uint32_t pos = min(t, c1 - 1), base = ent_row[(pos >> bs_log) - e0];
+            gone = base == ~0u;
+            return (uint64_t)((gone ? 0u : base) + (pos & (bs - 1))) * dim;
+        };
+        auto fetch = [&](uint32_t t0) {
+#pragma unroll
+            for (int i = 0; i < KL; i++) {
+                const uint32_t at = tid + 256 * i, t = at / (DP / 16), c = at % (DP / 16) * 16;
+                bool gone;
+                const uint64_t row = row_of(t0 + t, gone);
+                kr[i] = *reinterpret_cast<const u32x4*>(a.k_codes + row + (c < dim ? c : 0));
+                if (c >= dim || gone) kr[i] = u32x4{0u, 0u, 0u, 0u};
+            }
+#pragma unroll
+            for (int i = 0; i < VL; i++) {
+                const uint32_t at = tid + 256 * i, c = at % (DP / 4) * 4, oct = at / (DP / 4);      // octet: 32-token half oct / 4, lanes g = oct % 4
+                if (kOcts % 256 && at >= kOcts) break;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {                   // four rows in a row lie in one block
+                    bool gone;
+                    const uint32_t t = t0 + 32 * (oct / 4) + 16 * h + 4 * (oct % 4);
+                    const uint64_t row = row_of(t, gone);
+                    const uint32_t left = c1 - 1 - min(t, c1 - 1);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(a.v_codes + row + min((uint32_t)r, left) * dim + (c < dim ? c : 0));
+                        if (gone) vr[i][4 * h + r] = 0;
+                    }
+                }
+            }
+        };
+        auto store = [&](int buf) {
+#pragma unroll
+            for (int i = 0; i < KL; i++) {
+                const uint32_t at = tid + 256 * i, t = at / (DP / 16), c = at % (DP / 16) * 16;
+                *reinterpret_cast<f16x8*>(&keys[buf][t * kKeyLd + c]) = decode8<CODES>(kr[i][0], kr[i][1]);
+                *reinterpret_cast<f16x8*>(&keys[buf][t * kKeyLd + c + 8]) = decode8<CODES>(kr[i][2], kr[i][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < VL; i++) {
+                const uint32_t at = tid + 256 * i, c = at % (DP / 4) * 4, oct = at / (DP / 4);
+                if (kOcts % 256 && at >= kOcts) break;
+                f16x8 v[4];
+                decode_columns<CODES>(vr[i], v);
+#pragma unroll
+                for (int j = 0; j < 4; j++) *reinterpret_cast<f16x8*>(&vals[buf][(c + j) * kValLd + 8 * oct]) = v[j];
+            }
+        };
+        auto compute = [&](uint32_t t0, int buf) {
+            if (t0 >= most) return;                             // none of this wavefront's rows sees the tile
+            f32x4 s[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) s[mt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const f16x8 k = *reinterpret_cast<const f16x8*>(&keys[buf][(16 * t + m) * kKeyLd + 32 * ks + 8 * g]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int qt = 0; qt < QT; qt++) s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], s[mt][t], 0, 0, 0);
+                }
+            float fk[4], pw[4];
+            bool gone[4], any_gone = false;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const uint32_t e = (min(t0 + 16 * t, c1 - 1) >> bs_log) - e0;
+                fk[t] = ent_k[e];
+                pw[t] = fmaxf(ent_v[e] * per_v, 0x1p-60f);      // (a scale of 0 next to others: weights that vanish as 16-bit floats)
+                gone[t] = ent_row[e] == ~0u;
+                any_gone |= gone[t];
+            }
+            const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || __ballot(any_gone);
+            f16x8 p[MT][2][PT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                float local = -__builtin_inff(), f[4];
+                if (ragged) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const uint32_t pos = t0 + 16 * t + 4 * g + r;
+                            s[mt][t][r] = pos < min(seen[mt], c1) && !gone[t] ? s[mt][t][r] : -__builtin_inff();
+                        }
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    f[t] = fk[t] * factor[mt];
+                    const float x = fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3]));
+                    local = fmaxf(local, f[t] > 0.0f || x == -__builtin_inff() ? x * fmaxf(f[t], 0x1p-126f) : 0.0f);      // (no 0 * infinity)
+                }
+                if (__ballot(local > top[mt])) {
+                    const float now = fmaxf(top[mt], max_over_groups(local));
+                    const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
+                    top[mt] = now;
+                    sum[mt] *= shrink;
+#pragma unroll
+                    for (int i = 0; i < DT; i++) o[mt][i] *= shrink;
+                }
+                const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const float lift = __builtin_amdgcn_logf(pw[t]) - ref;
+                    float part_sum = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        float arg = __builtin_fmaf(s[mt][t][r], f[t], lift);
+                        if (ragged) arg = s[mt][t][r] == -__builtin_inff() ? -__builtin_inff() : arg;
+                        const float w = __builtin_amdgcn_exp2f(arg);
+                        part_sum += w;
+                        const _Float16 hi = (_Float16)w;
+                        p[mt][t / 2][0][4 * (t % 2) + r] = hi;
+                        if constexpr (PT == 2) p[mt][t / 2][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
+                    }
+                    sum[mt] = __builtin_fmaf(part_sum, __builtin_amdgcn_rcpf(pw[t]), sum[mt]);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < DT; i++) {
+                    const f16x8 v = *reinterpret_cast<const f16x8*>(&vals[buf][(16 * i + m) * kValLd + 32 * h + 8 * g]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int pt = 0; pt < PT; pt++) o[mt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[mt][h][pt], o[mt][i], 0, 0, 0);
+                }
+        };
+
+        fetch(c0);
+        store(0);
+        __syncthreads();
+        int buf = 0;
+        for (uint32_t t0 = c0; t0 < c1; t0 += kTokens) {
+            const bool more = t0 + kTokens < c1;
+            if (more) fetch(t0 + kTokens);
+            compute(t0, buf);
+            if constexpr (NBUF == 1) __syncthreads();           // (the only buffer is about to be overwritten)
+            if (NBUF == 2) buf ^= 1;
+            if (more) store(buf);
+            __syncthreads();
+        }
+    }
+
+    const float unit_o = unit_v / kPScale;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const float l = sum_over_groups(sum[mt]);
+        const uint32_t r = r0 + 16 * mt + m;
+        if (r >= n_r) continue;
+        const uint32_t i = r / group;
+        const size_t to = (size_t)(rows.first + i) * a.q_heads + kv * group + (r - i * group);
+        const float inv = l == 0.0f ? 0.0f : unit_o / l, lse = l == 0.0f ? -__builtin_inff() : top[mt] + __builtin_amdgcn_logf(l);
+        if (parts.n_splits == 1) {
+            T* out = (T*)a.out + to * dim;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+                if (16 * t < (int)dim) {
+                    const uint32_t d = 16 * t + 4 * g;
+                    if constexpr (sizeof(T) == 4) {
+                        *reinterpret_cast<float4*>(out + d) = make_float4(o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
+                    } else {
+                        u32x2 w;
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            w[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(o[mt][t][2 * j] * inv)) | ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(o[mt][t][2 * j + 1] * inv)) << 16);
+                        *reinterpret_cast<u32x2*>(out + d) = w;
+                    }
+                }
+            if (g == 0 && a.lse) a.lse[to] = lse * 0.6931471805599453f;
+        } else {
+            const size_t at = to * parts.n_splits + split;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+                if (16 * t < (int)dim)
+                    *reinterpret_cast<float4*>(parts.out + at * dim + 16 * t + 4 * g) = make_float4(o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
+            if (g == 0) parts.lse[at] = lse;
+        }
+    }
+}
+
+// The chunks' outputs of a row and head become one: weights 2^(lse - largest).  One workgroup each: dim / 4 lanes take a chunk, so that
+// 256 / (dim / 4) chunks are read at a time.
 template <class T>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials parts)
 {
-    const uint32_t lane = threadIdx.x & 63;
-    const uint64_t to = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (to >= (uint64_t)a.n_rows * a.q_heads) return;
-    const uint32_t row = (uint32_t)(to / a.q_heads);
+    __shared__ float red[kWaves], weight[256];
+    __shared__ __align__(16) float4 out_s[256];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, to = blockIdx.x, row = to / a.q_heads;
     const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
     if (b >= a.n_requests) return;
     uint32_t n = parts.n_splits;
@@ -594,32 +889,51 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials
         const uint32_t sees = seen_by(a, length_of(a, b), s.count, row - s.first);
         n = min(n, (uint32_t)(((uint64_t)sees + parts.chunk - 1) / parts.chunk));
     }
-    const float* lse = parts.lse + to * parts.n_splits;
-    const float* x = parts.out + to * parts.n_splits * a.dim;
+    const float* lse = parts.lse + (size_t)to * parts.n_splits;
+    const float* x = parts.out + (size_t)to * parts.n_splits * a.dim;
+    const uint32_t lanes = a.dim / 4, per = 256 / lanes, mine = tid / lanes, d = (tid - mine * lanes) * 4;
     float top = -__builtin_inff();
-    for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, lse[i]);
+    for (uint32_t i = tid; i < n; i += 256) top = fmaxf(top, lse[i]);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    if (lane == 0) red[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float ref = top == -__builtin_inff() ? 0.0f : top;
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.0f;
-    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-        const float w = i0 + lane < n ? __builtin_amdgcn_exp2f(lse[i0 + lane] - ref) : 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+    for (uint32_t i0 = 0; i0 < n; i0 += 256) {
+        const float w = i0 + tid < n ? __builtin_amdgcn_exp2f(lse[i0 + tid] - ref) : 0.0f;
         l += w;
-        const uint32_t here = min(n - i0, 64u);
-        for (uint32_t i = 0; i < here; i++) {
-            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (lane + 64 * c < a.dim) o[c] += f * x[(size_t)(i0 + i) * a.dim + lane + 64 * c];
-        }
+        __syncthreads();
+        weight[tid] = w;
+        __syncthreads();
+        const uint32_t here = min(n - i0, 256u);
+        if (mine < per)
+#pragma unroll 4
+            for (uint32_t i = mine; i < here; i += per) {
+                const float4 y = *reinterpret_cast<const float4*>(x + (size_t)(i0 + i) * a.dim + d);
+                const float f = weight[i];
+                o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
+            }
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-        if (lane + 64 * c < a.dim) ((T*)a.out)[to * a.dim + lane + 64 * c] = from_float<T>(o[c] * inv);
-    if (lane == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    __syncthreads();
+    if (lane == 0) red[tid >> 6] = l;
+    out_s[tid] = o;
+    __syncthreads();
+    l = red[0] + red[1] + red[2] + red[3];
+    if (mine == 0) {
+        for (uint32_t i = 1; i < per; i++) {
+            const float4 y = out_s[tid + i * lanes];
+            o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        T* out = (T*)a.out + (size_t)to * a.dim + d;
+        out[0] = from_float<T>(o.x * inv); out[1] = from_float<T>(o.y * inv); out[2] = from_float<T>(o.z * inv); out[3] = from_float<T>(o.w * inv);
+    }
+    if (tid == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 }  // namespace
@@ -632,31 +946,33 @@ static void check_attend(const hnsw_amd_token_cache* c, const AttendArgs& a, con
     if (a.n_requests < 1) throw std::invalid_argument(w + ": no requests");
     if (a.width < 1 || (uint64_t)a.width * c->block_tokens > 0x7fffffffull) throw std::invalid_argument(w + ": the table's width in tokens must be 1..2^31 - 1");
     if (!a.cu_q && a.n_rows != a.n_requests) throw std::invalid_argument(w + ": without cu_q there is one query row for each request");
-    if (a.n_rows > 0x7fffffffu || (uint64_t)a.n_rows * a.q_heads >= 1ull << 26) throw std::invalid_argument(w + ": too many rows and heads for one call");
+    if (a.n_rows > 0x7fffffffu || (uint64_t)a.n_rows * a.q_heads >= 1ull << 24) throw std::invalid_argument(w + ": too many rows and heads for one call");
     if (a.found && (a.id_heads < 1 || a.id_heads % c->n_heads || a.q_heads % a.id_heads))
         throw std::invalid_argument(w + ": the lists' heads must be a multiple of the cache's heads and divide the query heads");
+    if (reinterpret_cast<uintptr_t>(a.out) & 15u) throw std::invalid_argument(w + ": the output must be aligned to 16 bytes");
     if (!(a.scale == a.scale) || a.scale - a.scale != 0.0f) throw std::invalid_argument(w + ": scale must be finite");
 }
 
 // How a call's work is cut: units (rows) x heads x chunks of the items (tokens, or list entries).
-struct Cut { uint32_t mt, units, heads, chunk, n_splits; };
+struct Cut { bool tiles; uint32_t mt, units, heads, chunk, n_splits; };
 
 static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_requests, uint32_t heads, uint32_t items, bool by_request, bool ragged)
 {
     Cut c{};
     c.heads = heads;
     const uint32_t group = q_heads / heads;
-    // one tile of 16 rows, or two where that many rows share the tokens: the codes are decoded once for both (beyond 128 dims two
-    // tiles' outputs do not fit the registers)
-    const double rows = (double)group * (by_request ? (double)n_rows / n_requests : 1.0);
-    c.mt = rows > 16.0 && dim <= 128 ? 2 : 1;
-    const uint32_t tile = 16 * c.mt;
+    const double rows = (double)group * (by_request ? (double)n_rows / n_requests : 1.0);      // that share the tokens
+    // Many rows: tiles of 128 (64 beyond 128 dims) through LDS.  Few: 16, or 32, in registers; the codes are decoded once for both
+    // halves (beyond 128 dims two halves' outputs do not fit the registers).
+    c.tiles = by_request && ragged && rows > 32.0;
+    c.mt = c.tiles ? (dim <= 128 ? 2 : 1) : rows > 16.0 && dim <= 128 ? 2 : 1;
+    const uint32_t tile = 16 * c.mt * (c.tiles ? kWaves : 1);
     if (by_request && ragged) c.units = n_requests + (uint32_t)((uint64_t)n_rows * group / tile);
     else c.units = (by_request ? n_requests : n_rows) * ((group + tile - 1) / tile);
-    // chunks: enough workgroups to fill the GPU twice over, none shorter than 128 items
-    const uint64_t wanted = 1024, have = (uint64_t)c.units * heads;
+    // chunks: enough workgroups to fill the GPU (twice over where a workgroup is bound by memory), none shorter than 128 items (512 for tiles)
+    const uint64_t wanted = c.tiles ? 512 : 1024, have = (uint64_t)c.units * heads;
     uint64_t splits = have ? (wanted + have - 1) / have : 1;
-    const uint64_t step = (uint64_t)kWaves * kTile;
+    const uint64_t step = c.tiles ? 512 : (uint64_t)kWaves * kTile;
     uint64_t chunk = (((uint64_t)items + splits - 1) / splits + step - 1) / step * step;
     if (chunk < step) chunk = step;
     c.chunk = (uint32_t)chunk;
@@ -716,6 +1032,10 @@ void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows,
             hipLaunchKernelGGL((attend_rows_kernel<T, codes.value, dp.value, mt.value, f.value>), dim3(cut.units * cut.heads, cut.n_splits), dim3(256), 0,
                                (hipStream_t)stream, a, parts, cut.heads, q_vec);
         };
+        auto by_tiles = [&](auto dp, auto mt) {
+            hipLaunchKernelGGL((attend_tile_kernel<T, codes.value, dp.value, mt.value, dp.value <= 128 ? 2 : 1>), dim3(cut.units * cut.heads, cut.n_splits), dim3(256), 0,
+                               (hipStream_t)stream, a, parts, q_vec);
+        };
         auto by_rows = [&](auto dp, auto f) {
             if constexpr (dp.value <= 128) {
                 if (cut.mt == 2) return go(dp, std::integral_constant<int, 2>{}, f);
@@ -723,7 +1043,8 @@ void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows,
             go(dp, std::integral_constant<int, 1>{}, f);
         };
         auto by_kind = [&](auto dp) {
-            if (found) by_rows(dp, std::true_type{});
+            if (cut.tiles) by_tiles(dp, std::integral_constant<int, dp.value <= 128 ? 2 : 1>{});
+            else if (found) by_rows(dp, std::true_type{});
             else by_rows(dp, std::false_type{});
         };
         if (c->dim <= 64) by_kind(std::integral_constant<int, 64>{});
@@ -732,7 +1053,7 @@ void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows,
         else by_kind(std::integral_constant<int, 256>{});
         check_launch(who);
         if (cut.n_splits > 1) {
-            hipLaunchKernelGGL((attend_join_kernel<T>), dim3((uint32_t)(((uint64_t)n_rows * q_heads + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a, parts);
+            hipLaunchKernelGGL((attend_join_kernel<T>), dim3(n_rows * q_heads), dim3(256), 0, (hipStream_t)stream, a, parts);
             check_launch(who);
         }
     });

@@ -344,7 +344,7 @@ int hnsw_amd_cache_read_device(const hnsw_amd_token_cache* cache, const int64_t*
 
 /* Softmax attention over the cache: out[i][h] = sum_t p_t v_t / sum_t p_t with p_t = exp(scale * q[i][h] . k_t), the key head
  * of query head h being h / (n_q_heads / n_heads).  q: n_rows rows of n_q_heads heads (strides in elements, the last dimension
- * contiguous), out: [n_rows][n_q_heads][dim] of row_type, lse (may be NULL): [n_rows][n_q_heads] f32, log sum_t p_t.
+ * contiguous), out: [n_rows][n_q_heads][dim] of row_type (16-byte aligned), lse (may be NULL): [n_rows][n_q_heads] f32, log sum_t p_t.
  * cu_q NULL: one row for each request.  Else request b's rows are cu_q[b] .. cu_q[b + 1] (n_requests + 1 ascending entries
  * from 0, none above n_rows); rows behind the last request are left as they are.  The rows of a request are its last tokens
  * (lens counts them): with `causal`, row i of n sees the tokens 0 .. lens - n + i; without, all of lens.  A row that sees

@@ -15,7 +15,7 @@ def _cache(**kw):
     return capi.TokenCacheC(*[v[n] for n, _ in capi.TokenCacheC._fields_])
 
 
-def _attend(cache, found=False, q=1, rows=2, heads=4, row_type=0, table=1, width=4, lens=1, requests=2, cu=None, ids=1, id_heads=2, n_ids=3, scale=1.0, out=1,
+def _attend(cache, found=False, q=1, rows=2, heads=4, row_type=0, table=1, width=4, lens=1, requests=2, cu=None, ids=1, id_heads=2, n_ids=3, scale=1.0, out=16,
             work=None, nbytes=0):
     L, c = capi.lib(), ctypes.addressof(cache) if cache is not None else None
     if found:
@@ -40,7 +40,7 @@ def test_rows_beyond_32_bits_are_refused():
 
 
 @pytest.mark.parametrize("bad", [dict(heads=3), dict(heads=0), dict(requests=0), dict(width=0), dict(width=1 << 27), dict(rows=3), dict(row_type=3),
-                                 dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=None), dict(table=None), dict(lens=None),
+                                 dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=None), dict(out=24), dict(table=None), dict(lens=None),
                                  dict(rows=1 << 31, cu=1), dict(rows=1 << 30, cu=1)])
 def test_attend_refuses(bad):
     assert _attend(_cache(), **bad) == capi.E_ARG

@@ -322,6 +322,26 @@ def test_attend_found(lens, heads, share, group, block, dim, codes, dtype, k):
     _compare(s, q, out, lse, lambda r, h: (r, ref.visible(ids[r, h // each], lens[r])), dim ** -0.5)
 
 
+def test_work_that_needs_no_splitting_and_more_than_one_table():
+    """So many rows that no chunk is cut, over more tokens (entries of a list) than a workgroup's table of blocks (tokens) holds; scales differ
+    between the tables."""
+    s = Setup([4500, 64], 8, 16, 64, E4)
+    v = s.cache.v_scale.cpu()
+    v[s.table[0, :256].long()] *= 2.0 ** -3
+    s.cache.v_scale.copy_(v)
+    s.v64 = s.cache.v_codes.cpu().double() * v.double()[:, :, None, None]
+    new, cu = [600, 40], [0, 600, 640]
+    q = _queries(640, 8 * 16, 64, BF16)
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=_gpu(cu))
+    _compare(s, q[:, :], out, lse, lambda r, h: (int(r >= 600), np.arange([4500, 64][r >= 600] - [600, 40][r >= 600] + r - cu[int(r >= 600)] + 1)), 64 ** -0.5, pick=[0, 599, 600, 639])
+    lens = [3000] * 64
+    s = Setup(lens, 4, 64, 32, I8)
+    ids = np.stack([np.random.default_rng(i).permutation(3000)[:1500] for i in range(64 * 16)]).reshape(64, 16, 1500).astype(np.int32)
+    q = _queries(64, 16, 32, BF16)
+    out, lse = s.cache.attend_found(q, s.d_table, s.d_lens, _gpu(ids))
+    _compare(s, q, out, lse, lambda r, h: (r, ref.visible(ids[r, h], 3000)), 32 ** -0.5, pick=[0, 31, 63])
+
+
 def test_attend_found_of_many_rows_sees_no_later_token():
     lens, new = [50, 9], [6, 12]
     s = Setup(lens, 1, 16, 64, I8)
