@@ -116,6 +116,10 @@ __device__ __forceinline__ Span rows_of(const AttendArgs& a, uint32_t b)
     const int64_t lo = min(max((int64_t)a.cu_q[b], (int64_t)0), (int64_t)a.n_rows), hi = min(max((int64_t)a.cu_q[b + 1], lo), (int64_t)a.n_rows);
     return {(uint32_t)lo, (uint32_t)(hi - lo)};
 }
+__device__ __forceinline__ Span uniform(Span s)                 // the same in all lanes: say so
+{
+    return {(uint32_t)__builtin_amdgcn_readfirstlane(s.first), (uint32_t)__builtin_amdgcn_readfirstlane(s.count)};
+}
 __device__ __forceinline__ uint32_t length_of(const AttendArgs& a, uint32_t b)
 {
     const int64_t cap = (int64_t)a.width * a.block_tokens;
@@ -153,10 +157,10 @@ __device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_
         if (m) {
             const int at = __builtin_ctzll(m);
             request = b0 + at;
-            part = u - before - (__shfl(upto, at) - __shfl(n, at));
+            part = __builtin_amdgcn_readfirstlane(u - before - (__shfl(upto, at) - __shfl(n, at)));
             return true;
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
@@ -266,20 +270,20 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
         first = unit / per;
         r0 = (unit - first * per) * 16 * MT;
         if (first >= a.n_rows) return;
-        b = a.cu_q ? request_of(a.cu_q, a.n_requests, first) : first;
+        b = __builtin_amdgcn_readfirstlane(a.cu_q ? request_of(a.cu_q, a.n_requests, first) : first);
         if (b >= a.n_requests) return;
         count = 1;
     } else {
         uint32_t part;
         if (!unit_of(a, unit, group, 16 * MT, lane, b, part)) return;
-        const Span s = rows_of(a, b);
+        const Span s = uniform(rows_of(a, b));
         first = s.first;
         count = s.count;
         r0 = part * 16 * MT;
     }
     const uint32_t n_r = count * group;                         // (fits: n_rows * q_heads < 2^31)
     if (r0 >= n_r) return;
-    const uint32_t len = length_of(a, b);
+    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
 
     // the rows of this lane's columns, what they see, and the queries
     uint32_t seen[MT], least = 0xffffffffu, most = 0;
@@ -473,14 +477,11 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
 #pragma unroll
                     for (int r = 0; r < 4; r++) x[h][r] = s[mt][h][r] * (fk[h][r] * factor[mt]);
                 if (ragged) {
+                    const int left = (int)((FOUND ? n : min(seen[mt], c1) - c0) - i0 - 4 * g);
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const uint32_t i = i0 + 16 * h + 4 * g + r;
-                            const bool sees = FOUND ? i < n : (c0 + i < min(seen[mt], c1) && !gone[h]);
-                            x[h][r] = sees ? x[h][r] : -__builtin_inff();
-                        }
+                        for (int r = 0; r < 4; r++) x[h][r] = 16 * h + r < left && !gone[h] ? x[h][r] : -__builtin_inff();
                 }
 #pragma unroll
                 for (int h = 0; h < 2; h++)
@@ -596,8 +597,10 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
 }
 
 // Attention of many query rows: prompts.  The codes of 64 tokens become 16-bit floats once for all 64 * MT rows of the workgroup: in
-// LDS, keys [token][dim], values [dim][token] (the eight tokens of a matrix operand next to each other; rows of an odd number of
-// 16-byte pieces, so that operands are read without bank conflicts), while the next tile's codes are on their way to registers.
+// LDS, keys [token][dim] (rows of an odd number of 16-byte pieces, so that operands are read without bank conflicts), values
+// [dim][token] (the eight tokens of a matrix operand next to each other, the pieces of a row in an order that differs by row to
+// the same end), while the next tile's codes are on their way to registers: each wavefront moves the keys of 16 tokens and a quarter
+// of the values' octets, so that the blocks they lie in are scalars.
 // Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel, but that a block's value scale goes
 // into the exponent instead of being multiplied in: weights are 2^(score - maximum + log2 of the scale over the table's largest), their
 // sum is put right by the inverse per 16 tokens.
@@ -605,14 +608,14 @@ template <class T, int CODES, int DP, int MT, int NBUF>
 __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
 {
     constexpr int KS = DP / 32, DT = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
-    constexpr int kTokens = 64, kKeyLd = DP + 8, kValLd = kTokens + 8;          // 16-bit elements
-    constexpr int KL = kTokens * (DP / 16) / 256;                               // 16-byte pieces of keys a thread moves
-    constexpr int kOcts = DP / 4 * (kTokens / 8), VL = (kOcts + 255) / 256;     // (word of 4 dims) x 8 tokens of values
+    constexpr int kTokens = 64, kKeyLd = DP + 8;                 // 16-bit elements
+    constexpr int KL = DP / 64, VL = (DP + 127) / 128;          // 16-byte pieces of keys, and words x 8 tokens of values, that a thread moves
     constexpr uint32_t kEntries = kScanTokens / 16 + 2;
     __shared__ uint32_t ent_row[kEntries];
-    __shared__ float ent_k[kEntries], ent_v[kEntries], red[kWaves];
+    __shared__ float ent_k[kEntries], ent_v[kEntries], ent_i[kEntries], red[kWaves];
     __shared__ __align__(16) _Float16 keys[NBUF][kTokens * kKeyLd];
-    __shared__ __align__(16) _Float16 vals[NBUF][DP * kValLd];
+    __shared__ __align__(16) _Float16 vals[NBUF][DP * kTokens];
+    auto val_at = [](uint32_t d, uint32_t oct) { return d * kTokens + 8 * (oct ^ ((d >> 1) & 7)); };
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -623,9 +626,9 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     constexpr uint32_t kRows = kWaves * 16 * MT;
     uint32_t b, part;
     if (!unit_of(a, unit, group, kRows, lane, b, part)) return;
-    const Span rows = rows_of(a, b);
+    const Span rows = uniform(rows_of(a, b));
     const uint32_t n_r = rows.count * group, r0 = part * kRows + wave * 16 * MT;
-    const uint32_t len = length_of(a, b);
+    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
 
     uint32_t seen[MT], least = 0xffffffffu, most = 0;
     f16x8 q[MT][KS][QT];
@@ -682,39 +685,50 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
             }
             unit_v = largest;
         }
-        const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
+        // weights get a block's value scale over the largest by way of the exponent (a scale of 0 next to others counts as 2^-60 of it:
+        // weights that vanish as 16-bit floats)
+        for (uint32_t i = tid; i <= ((c1 - 1) >> bs_log) - e0; i += 256) {          // (the entries that this thread wrote)
+            const float w = largest > 0.0f ? fmaxf(ent_v[i] * (kPScale / largest), 0x1p-60f) : 1.0f;
+            ent_v[i] = __builtin_amdgcn_logf(w);
+            ent_i[i] = 1.0f / w;
+        }
+        __syncthreads();
 
         u32x4 kr[KL];
         uint32_t vr[VL][8];
-        // token t of the tile at t0: its row of codes (of the nearest token that is there; `gone`: of no block)
-        auto row_of = [&](uint32_t t, bool& gone) {
-            const uint32_t pos = min(t, c1 - 1), base = ent_row[(pos >> bs_log) - e0];
+        bool v_gone[2];
+        const uint32_t k_row = lane >> 2, oct = 2 * wave + (lane >> 5), v_row = 4 * (oct & 3), v_word = lane & 31;
+        // the codes from token `start` on (16 of them, in one block; those behind the last token are the last one): their first row's
+        // offset, and how many there are
+        auto place = [&](uint32_t start, uint32_t& limit, bool& gone) {
+            const uint32_t pos = min(start, c1 - 1), base = __builtin_amdgcn_readfirstlane(ent_row[(pos >> bs_log) - e0]);
+            limit = min(c1 - 1 - pos, 15u);
             gone = base == ~0u;
             return (uint64_t)((gone ? 0u : base) + (pos & (bs - 1))) * dim;
         };
         auto fetch = [&](uint32_t t0) {
+            uint32_t limit;
+            bool gone;
+            const uint8_t* kb = a.k_codes + place(t0 + 16 * wave, limit, gone);     // (scores of tokens of no block are masked)
+            const uint32_t kr0 = (limit == 15 ? k_row : min(k_row, limit)) * dim;
 #pragma unroll
             for (int i = 0; i < KL; i++) {
-                const uint32_t at = tid + 256 * i, t = at / (DP / 16), c = at % (DP / 16) * 16;
-                bool gone;
-                const uint64_t row = row_of(t0 + t, gone);
-                kr[i] = *reinterpret_cast<const u32x4*>(a.k_codes + row + (c < dim ? c : 0));
-                if (c >= dim || gone) kr[i] = u32x4{0u, 0u, 0u, 0u};
+                const uint32_t c = 64 * i + 16 * (lane & 3);
+                kr[i] = *reinterpret_cast<const u32x4*>(kb + kr0 + (c < dim ? c : 0));
             }
 #pragma unroll
-            for (int i = 0; i < VL; i++) {
-                const uint32_t at = tid + 256 * i, c = at % (DP / 4) * 4, oct = at / (DP / 4);      // octet: 32-token half oct / 4, lanes g = oct % 4
-                if (kOcts % 256 && at >= kOcts) break;
+            for (int h = 0; h < 2; h++) {
+                const uint8_t* vb = a.v_codes + place(t0 + 32 * (wave >> 1) + 16 * h, limit, v_gone[h]);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {                   // four rows in a row lie in one block
-                    bool gone;
-                    const uint32_t t = t0 + 32 * (oct / 4) + 16 * h + 4 * (oct % 4);
-                    const uint64_t row = row_of(t, gone);
-                    const uint32_t left = c1 - 1 - min(t, c1 - 1);
+                for (int i = 0; i < VL; i++) {
+                    const uint32_t c = 4 * (v_word + 32 * i), at = c < dim ? c : 0;
+                    if (limit == 15) {
+                        const uint32_t v0 = v_row * dim + at;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(a.v_codes + row + min((uint32_t)r, left) * dim + (c < dim ? c : 0));
-                        if (gone) vr[i][4 * h + r] = 0;
+                        for (int r = 0; r < 4; r++) vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(vb + (size_t)r * dim + v0);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(vb + min(v_row + r, limit) * dim + at);
                     }
                 }
             }
@@ -722,27 +736,29 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         auto store = [&](int buf) {
 #pragma unroll
             for (int i = 0; i < KL; i++) {
-                const uint32_t at = tid + 256 * i, t = at / (DP / 16), c = at % (DP / 16) * 16;
-                *reinterpret_cast<f16x8*>(&keys[buf][t * kKeyLd + c]) = decode8<CODES>(kr[i][0], kr[i][1]);
-                *reinterpret_cast<f16x8*>(&keys[buf][t * kKeyLd + c + 8]) = decode8<CODES>(kr[i][2], kr[i][3]);
+                _Float16* to = &keys[buf][(16 * wave + k_row) * kKeyLd + 64 * i + 16 * (lane & 3)];
+                *reinterpret_cast<f16x8*>(to) = decode8<CODES>(kr[i][0], kr[i][1]);
+                *reinterpret_cast<f16x8*>(to + 8) = decode8<CODES>(kr[i][2], kr[i][3]);
+            }
+            if (v_gone[0] || v_gone[1]) {
+#pragma unroll
+                for (int i = 0; i < VL; i++)
+#pragma unroll
+                    for (int r = 0; r < 8; r++) vr[i][r] = v_gone[r / 4] ? 0u : vr[i][r];
             }
 #pragma unroll
             for (int i = 0; i < VL; i++) {
-                const uint32_t at = tid + 256 * i, c = at % (DP / 4) * 4, oct = at / (DP / 4);
-                if (kOcts % 256 && at >= kOcts) break;
+                const uint32_t c = 4 * (v_word + 32 * i);
+                if (DP % 128 && c >= DP) break;
                 f16x8 v[4];
                 decode_columns<CODES>(vr[i], v);
 #pragma unroll
-                for (int j = 0; j < 4; j++) *reinterpret_cast<f16x8*>(&vals[buf][(c + j) * kValLd + 8 * oct]) = v[j];
+                for (int j = 0; j < 4; j++) *reinterpret_cast<f16x8*>(&vals[buf][val_at(c + j, oct)]) = v[j];
             }
         };
         auto compute = [&](uint32_t t0, int buf) {
             if (t0 >= most) return;                             // none of this wavefront's rows sees the tile
             f32x4 s[MT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int t = 0; t < 4; t++) s[mt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -751,31 +767,31 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                        for (int qt = 0; qt < QT; qt++) s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], s[mt][t], 0, 0, 0);
+                        for (int qt = 0; qt < QT; qt++)
+                            s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][t] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
                 }
-            float fk[4], pw[4];
+            float fk[4], lift[4], put_right[4];
             bool gone[4], any_gone = false;
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 const uint32_t e = (min(t0 + 16 * t, c1 - 1) >> bs_log) - e0;
                 fk[t] = ent_k[e];
-                pw[t] = fmaxf(ent_v[e] * per_v, 0x1p-60f);      // (a scale of 0 next to others: weights that vanish as 16-bit floats)
-                gone[t] = ent_row[e] == ~0u;
+                lift[t] = ent_v[e];
+                put_right[t] = ent_i[e];
+                gone[t] = __builtin_amdgcn_readfirstlane(ent_row[e]) == ~0u;
                 any_gone |= gone[t];
             }
-            const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || __ballot(any_gone);
+            const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || any_gone;
             f16x8 p[MT][2][PT];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
                 float local = -__builtin_inff(), f[4];
                 if (ragged) {
+                    const int left = (int)(min(seen[mt], c1) - t0 - 4 * g);         // (both are below 2^31)
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const uint32_t pos = t0 + 16 * t + 4 * g + r;
-                            s[mt][t][r] = pos < min(seen[mt], c1) && !gone[t] ? s[mt][t][r] : -__builtin_inff();
-                        }
+                        for (int r = 0; r < 4; r++) s[mt][t][r] = 16 * t + r < left && !gone[t] ? s[mt][t][r] : -__builtin_inff();
                 }
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -794,11 +810,11 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                 const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const float lift = __builtin_amdgcn_logf(pw[t]) - ref;
+                    const float by = lift[t] - ref;
                     float part_sum = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        float arg = __builtin_fmaf(s[mt][t][r], f[t], lift);
+                        float arg = __builtin_fmaf(s[mt][t][r], f[t], by);
                         if (ragged) arg = s[mt][t][r] == -__builtin_inff() ? -__builtin_inff() : arg;
                         const float w = __builtin_amdgcn_exp2f(arg);
                         part_sum += w;
@@ -806,14 +822,14 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                         p[mt][t / 2][0][4 * (t % 2) + r] = hi;
                         if constexpr (PT == 2) p[mt][t / 2][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
                     }
-                    sum[mt] = __builtin_fmaf(part_sum, __builtin_amdgcn_rcpf(pw[t]), sum[mt]);
+                    sum[mt] = __builtin_fmaf(part_sum, put_right[t], sum[mt]);
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < DT; i++) {
-                    const f16x8 v = *reinterpret_cast<const f16x8*>(&vals[buf][(16 * i + m) * kValLd + 32 * h + 8 * g]);
+                    const f16x8 v = *reinterpret_cast<const f16x8*>(&vals[buf][val_at(16 * i + m, 4 * h + g)]);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -970,7 +986,7 @@ static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_
     if (by_request && ragged) c.units = n_requests + (uint32_t)((uint64_t)n_rows * group / tile);
     else c.units = (by_request ? n_requests : n_rows) * ((group + tile - 1) / tile);
     // chunks: enough workgroups to fill the GPU (twice over where a workgroup is bound by memory), none shorter than 128 items (512 for tiles)
-    const uint64_t wanted = c.tiles ? 512 : 1024, have = (uint64_t)c.units * heads;
+    const uint64_t wanted = c.tiles ? 256 : 1024, have = (uint64_t)c.units * heads;
     uint64_t splits = have ? (wanted + have - 1) / have : 1;
     const uint64_t step = c.tiles ? 512 : (uint64_t)kWaves * kTile;
     uint64_t chunk = (((uint64_t)items + splits - 1) / splits + step - 1) / step * step;
