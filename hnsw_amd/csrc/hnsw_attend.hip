@@ -29,7 +29,12 @@ constexpr int kWaves = 4;                 // wavefronts of a workgroup
 constexpr uint32_t kTile = 32;            // tokens a wavefront takes at a time
 constexpr uint32_t kScanTokens = 4096;    // of one table of block entries in LDS (all tokens), and
 constexpr uint32_t kListTokens = 1024;    // of one table of token entries (listed tokens)
-constexpr float kPScale = 32768.0f;       // probabilities are multiplied by this before they become 16-bit floats, see below
+// A softmax's reference is only moved when a score is more than this above it, in base 2: moving it costs as much as a third of a tile
+// (the outputs are multiplied by the change), and over random scores some row of 16 sees a new maximum in every second tile.
+// Probabilities relative to the reference are then up to 2^4, and what they are multiplied by before they become 16-bit floats
+// (largest 2^16) leaves room for that.
+constexpr float kLead = 4.0f;
+constexpr float kPScale = 2048.0f;
 
 template <class T> constexpr int kQTerms = sizeof(T) == 4 ? 2 : 1;                  // 16-bit floats that a query element is split into
 template <class T> constexpr int kPTerms = std::is_same_v<T, bf16> ? 1 : 2;         // and a probability
@@ -241,8 +246,8 @@ struct Partials {
 // and the next tile is under way while one is computed.  Codes become 16-bit floats, which hold both kinds exactly.
 // Queries are scaled by a power of two to just under 2^15 and rounded to 16-bit floats (nothing is lost of bf16 and f16 but what
 // lies 2^-29 under the row's largest element); 32-bit queries are split into two terms.  A block's key scale multiplies the
-// scores; its value scale, over the largest of the table's, multiplies the probabilities, which as 16-bit floats in units of 2^-15
-// reach down to 2^-39 of the largest: 2^-11 of each is rounded away for bf16 rows (whose outputs keep 2^-8), and a second term
+// scores; its value scale, over the largest of the table's, multiplies the probabilities, which as 16-bit floats in units of 2^-11
+// reach down to 2^-35 of the largest: 2^-11 of each is rounded away for bf16 rows (whose outputs keep 2^-8), and a second term
 // takes that up for the others.  Sums, maxima and outputs are in 32 bits.
 template <class T, int CODES, int DP, int MT, bool FOUND>
 __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
@@ -487,7 +492,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) local = fmaxf(local, x[h][r]);
-                if (__ballot(local > top[mt])) {                // rare after the first tiles: a new maximum
+                if (__ballot(local > top[mt] + kLead)) {        // rare after the first tile
                     const float now = fmaxf(top[mt], max_over_groups(local));
                     const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
                     top[mt] = now;
@@ -612,7 +617,8 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     constexpr int KL = DP / 64, VL = (DP + 127) / 128;          // 16-byte pieces of keys, and words x 8 tokens of values, that a thread moves
     constexpr uint32_t kEntries = kScanTokens / 16 + 2;
     __shared__ uint32_t ent_row[kEntries];
-    __shared__ float ent_k[kEntries], ent_v[kEntries], ent_i[kEntries], red[kWaves];
+    __shared__ float ent_k[kEntries], ent_v[kEntries], red[kWaves];
+    __shared__ __align__(16) float4 ent[kEntries];              // key scale, log2 of the weights' factor, its inverse, and ~0 (as bits) where there is no block
     __shared__ __align__(16) _Float16 keys[NBUF][kTokens * kKeyLd];
     __shared__ __align__(16) _Float16 vals[NBUF][DP * kTokens];
     auto val_at = [](uint32_t d, uint32_t oct) { return d * kTokens + 8 * (oct ^ ((d >> 1) & 7)); };
@@ -689,8 +695,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         // weights that vanish as 16-bit floats)
         for (uint32_t i = tid; i <= ((c1 - 1) >> bs_log) - e0; i += 256) {          // (the entries that this thread wrote)
             const float w = largest > 0.0f ? fmaxf(ent_v[i] * (kPScale / largest), 0x1p-60f) : 1.0f;
-            ent_v[i] = __builtin_amdgcn_logf(w);
-            ent_i[i] = 1.0f / w;
+            ent[i] = make_float4(ent_k[i], __builtin_amdgcn_logf(w), 1.0f / w, __uint_as_float(ent_row[i] == ~0u ? ~0u : 0u));
         }
         __syncthreads();
 
@@ -770,15 +775,12 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                         for (int qt = 0; qt < QT; qt++)
                             s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][t] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
                 }
-            float fk[4], lift[4], put_right[4];
+            float4 x[4];
             bool gone[4], any_gone = false;
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                const uint32_t e = (min(t0 + 16 * t, c1 - 1) >> bs_log) - e0;
-                fk[t] = ent_k[e];
-                lift[t] = ent_v[e];
-                put_right[t] = ent_i[e];
-                gone[t] = __builtin_amdgcn_readfirstlane(ent_row[e]) == ~0u;
+                x[t] = ent[(min(t0 + 16 * t, c1 - 1) >> bs_log) - e0];
+                gone[t] = __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].w)) != 0;
                 any_gone |= gone[t];
             }
             const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || any_gone;
@@ -795,11 +797,10 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                 }
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    f[t] = fk[t] * factor[mt];
-                    const float x = fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3]));
-                    local = fmaxf(local, f[t] > 0.0f || x == -__builtin_inff() ? x * fmaxf(f[t], 0x1p-126f) : 0.0f);      // (no 0 * infinity)
+                    f[t] = fmaxf(x[t].x * factor[mt], 0x1p-126f);                   // (not 0, which masked scores would make NaN)
+                    local = fmaxf(local, f[t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
                 }
-                if (__ballot(local > top[mt])) {
+                if (__ballot(local > top[mt] + kLead)) {
                     const float now = fmaxf(top[mt], max_over_groups(local));
                     const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
                     top[mt] = now;
@@ -810,19 +811,17 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                 const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const float by = lift[t] - ref;
+                    const float by = x[t].y - ref;
                     float part_sum = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        float arg = __builtin_fmaf(s[mt][t][r], f[t], by);
-                        if (ragged) arg = s[mt][t][r] == -__builtin_inff() ? -__builtin_inff() : arg;
-                        const float w = __builtin_amdgcn_exp2f(arg);
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][t][r], f[t], by));
                         part_sum += w;
                         const _Float16 hi = (_Float16)w;
                         p[mt][t / 2][0][4 * (t % 2) + r] = hi;
                         if constexpr (PT == 2) p[mt][t / 2][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
                     }
-                    sum[mt] = __builtin_fmaf(part_sum, put_right[t], sum[mt]);
+                    sum[mt] = __builtin_fmaf(part_sum, x[t].z, sum[mt]);
                 }
             }
 #pragma unroll

@@ -110,17 +110,17 @@ def tolerance(out, spread, qk, peak, n, dim, dtype, largest=0.0):
     dim products in 32 bits (each step off by half a step of a partial sum, at most qk: (dim + 8) 2^-24 qk with the query's
     split into halves, the scale and the base-2 logarithm's factor), the exponential adds its argument's rounding and its own, probabilities that meet
     the values as 16-bit floats are off by 2^-11 of themselves, and sums over n tokens by n 2^-24.
-    Those 16-bit floats have a smallest step: a token's weight, its probability (1 at the row's maximum) times its value scale over the
-    largest scale S, is held in units of 2^-15, where the step is never under 2^-24, so it is off by up to half of that, 2^-25 2^-15 =
-    2^-40, whatever its size.  That meets a code of at most C and the unit S: n tokens move the sum by n 2^-40 S C at most (`largest` is
-    S C), and the sum of the probabilities that it is divided by is at least 1."""
+    Those 16-bit floats have a smallest step: a token's weight, its probability (1 at the softmax's reference, which is one of the row's
+    scores) times its value scale over the largest scale S, is held in units of 2^-11, where the step is never under 2^-24, so it is off
+    by up to half of that, 2^-25 2^-11 = 2^-36, whatever its size.  That meets a code of at most C and the unit S: n tokens move the
+    sum by n 2^-36 S C at most (`largest` is S C), and the sum of the probabilities that it is divided by is at least 1."""
     half = torch.finfo(dtype).eps / 2
     score = (dim + 8) * 2.0 ** -24 * qk
     p = 2 * (score + 2.0 ** -22 * (1 + peak)) + 2 * n * 2.0 ** -24 + 2.0 ** -22
     if dtype is not torch.float32:
         p += 2.0 ** -11
     least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps       # values under the smallest normal round by a fixed step
-    return half * out.abs() + (spread * p + n * 2.0 ** -40 * largest) * (1 + half) + least
+    return half * out.abs() + (spread * p + n * 2.0 ** -36 * largest) * (1 + half) + least
 
 
 def lse_tolerance(lse, qk, peak, n, dim):
