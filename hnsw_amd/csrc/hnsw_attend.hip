@@ -205,27 +205,42 @@ __device__ __forceinline__ float load_query(const AttendArgs& a, bool there, uin
     return ldexpf(fabsf(a.scale) * kLog2e, -e);
 }
 
-// Block entries of the tokens c0 .. c1 of request b into LDS (whole workgroup): first row of a block's codes in rows of dim bytes, ~0
-// where there is no block, and its scales.  Returns the largest value scale that this thread saw.
-__device__ __forceinline__ float table_entries(const AttendArgs& a, uint32_t b, uint32_t kv, uint32_t bs_log, uint32_t c0, uint32_t c1, uint32_t tid,
-                                               uint32_t threads, uint32_t* ent_row, float* ent_k, float* ent_v)
+// Block entries of the tokens c0 .. c1 of request b into LDS, by a workgroup of 256 threads: first row of a block's codes (in rows of dim
+// bytes) and its scales.  An entry of no block has the key scale -1 and the row of one that is, so that loads stay among codes of
+// live tokens: weights of 0 do not meet the NaN that stale codes can be.  Returns the largest value scale; false where no entry is of a block.
+struct Reduced { float largest[kWaves]; uint32_t some[kWaves]; };
+__device__ __forceinline__ bool table_entries(const AttendArgs& a, uint32_t b, uint32_t kv, uint32_t bs_log, uint32_t c0, uint32_t c1, uint32_t tid,
+                                              uint32_t* ent_row, float* ent_k, float* ent_v, Reduced& red, float& largest)
 {
-    const uint32_t e0 = c0 >> bs_log, n_e = ((c1 - 1) >> bs_log) - e0 + 1;
-    float largest = 0.0f;
-    for (uint32_t i = tid; i < n_e; i += threads) {
+    const uint32_t e0 = c0 >> bs_log, n_e = ((c1 - 1) >> bs_log) - e0 + 1, lane = tid & 63, wave = tid >> 6;
+    uint32_t some = 0;                                          // a row + 1
+    largest = 0.0f;
+    for (uint32_t i = tid; i < n_e; i += 256) {
         const uint32_t blk = (uint32_t)a.table[(size_t)b * a.width + e0 + i];
-        uint32_t row = ~0u;
-        float sk = 0.0f, sv = 0.0f;
+        uint32_t row = 0;
+        float sk = -1.0f, sv = 0.0f;
         if (blk < a.n_blocks) {
             const uint32_t bh = blk * a.n_heads + kv;
             row = bh << bs_log;
             sk = a.k_scale[bh];
             sv = a.v_scale[bh];
+            some = row + 1;
+            largest = fmaxf(largest, sv);
         }
         ent_row[i] = row; ent_k[i] = sk; ent_v[i] = sv;
-        largest = fmaxf(largest, sv);
     }
-    return largest;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        largest = fmaxf(largest, __shfl_xor(largest, off));
+        some = max(some, (uint32_t)__shfl_xor((int)some, off));
+    }
+    if (lane == 0) { red.largest[wave] = largest; red.some[wave] = some; }
+    __syncthreads();
+    largest = fmaxf(fmaxf(red.largest[0], red.largest[1]), fmaxf(red.largest[2], red.largest[3]));
+    some = __builtin_amdgcn_readfirstlane(max(max(red.some[0], red.some[1]), max(red.some[2], red.some[3])));
+    for (uint32_t i = tid; i < n_e; i += 256)                   // (the entries that this thread wrote)
+        if (ent_k[i] < 0.0f) ent_row[i] = some - 1;
+    return some != 0;
 }
 
 struct Partials {
@@ -255,10 +270,11 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
     constexpr int KS = DP / 32, KW = DP / 64, VW = DP / 64, VB = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
     constexpr uint32_t kEntries = FOUND ? kListTokens + kTile : kScanTokens / 16 + 2;
     constexpr int kOutLd = DP + 4;
-    __shared__ uint32_t ent_row[kEntries];                      // first row of a block's (a token's) codes, in rows of dim bytes; ~0: there is none
+    __shared__ uint32_t ent_row[kEntries];                      // first row of a block's (a token's) codes, in rows of dim bytes
     __shared__ __align__(16) float ent_k[kEntries], ent_v[kEntries];         // its scales (values: see pw below)
     __shared__ __align__(16) float join[2][16 * MT][kOutLd];
-    __shared__ float join_m[kWaves][16 * MT], join_l[kWaves][16 * MT], red[kWaves];
+    __shared__ float join_m[kWaves][16 * MT], join_l[kWaves][16 * MT];
+    __shared__ Reduced red;
     __shared__ uint32_t red_n[kWaves];
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
@@ -372,15 +388,17 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
             n = kept;
             __syncthreads();
             if (tid < kTile && n > 0) { ent_row[n + tid] = ent_row[n - 1]; ent_k[n + tid] = 0.0f; ent_v[n + tid] = 0.0f; }
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
+            if (lane == 0) red.largest[wave] = largest;
+            __syncthreads();
+            largest = fmaxf(fmaxf(red.largest[0], red.largest[1]), fmaxf(red.largest[2], red.largest[3]));
         } else {
             e0 = c0 >> bs_log;
-            largest = table_entries(a, b, kv, bs_log, c0, c1, tid, 256, ent_row, ent_k, ent_v);
+            const bool some = table_entries(a, b, kv, bs_log, c0, c1, tid, ent_row, ent_k, ent_v, red, largest);
+            __syncthreads();
+            if (!some) continue;
         }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
-        if (lane == 0) red[wave] = largest;
-        __syncthreads();
-        largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
         if (largest > 0.0f) {
             if (unit_v > 0.0f && unit_v != largest) {           // outputs so far are in units of the last table's largest scale
@@ -394,7 +412,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
         }
 
         // a tile's codes: where they are, and the loads
-        struct Tile { u32x4 k[2][KW]; uint32_t v[8][VW]; uint32_t row[2]; };
+        struct Tile { u32x4 k[2][KW]; uint32_t v[8][VW]; };
         const uint32_t k_col = min(16 * g, dim - 16), v_col = VB * m;
         auto fetch = [&](uint32_t j, Tile& t) {
             const uint32_t i0 = 32 * j;
@@ -406,12 +424,9 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
                     row_k = ent_row[i0 + 16 * h + m];
 #pragma unroll
                     for (int r = 0; r < 4; r++) row_v[r] = ent_row[i0 + 16 * h + 4 * g + r];
-                    t.row[h] = 0;
                 } else {
                     const uint32_t last = c1 - 1, start = min(c0 + i0 + 16 * h, last);
-                    uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
-                    t.row[h] = base;
-                    if (base == ~0u) base = 0;                  // (loads stay inside, the values are dropped)
+                    const uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
                     const uint64_t at = (uint64_t)(base + (start & (bs - 1))) * dim;
                     kb += at;
                     vb += at;
@@ -468,7 +483,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
                     const float x = ent_k[e], y = ent_v[e] * per_v;
 #pragma unroll
                     for (int r = 0; r < 4; r++) { fk[h][r] = x; pw[h][r] = y; }
-                    gone[h] = t.row[h] == ~0u;
+                    gone[h] = __builtin_amdgcn_readfirstlane(__float_as_uint(x)) >> 31;
                 }
             }
             if constexpr (FOUND) ragged = i0 + 32 > n;
@@ -512,14 +527,6 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a, Partials
                         p[mt][0][4 * h + r] = hi;
                         if constexpr (PT == 2) p[mt][1][4 * h + r] = (_Float16)(w - (float)hi);
                     }
-            }
-            if constexpr (!FOUND) {
-                if (gone[0] || gone[1]) {
-#pragma unroll
-                    for (int r = 0; r < 8; r++)
-#pragma unroll
-                        for (int i = 0; i < VW; i++) t.v[r][i] = gone[r / 4] ? 0u : t.v[r][i];
-                }
             }
 #pragma unroll
             for (int i = 0; i < VW; i++) {
@@ -617,8 +624,9 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     constexpr int KL = DP / 64, VL = (DP + 127) / 128;          // 16-byte pieces of keys, and words x 8 tokens of values, that a thread moves
     constexpr uint32_t kEntries = kScanTokens / 16 + 2;
     __shared__ uint32_t ent_row[kEntries];
-    __shared__ float ent_k[kEntries], ent_v[kEntries], red[kWaves];
-    __shared__ __align__(16) float4 ent[kEntries];              // key scale, log2 of the weights' factor, its inverse, and ~0 (as bits) where there is no block
+    __shared__ float ent_k[kEntries], ent_v[kEntries];
+    __shared__ Reduced red;
+    __shared__ __align__(16) float4 ent[kEntries];              // key scale, log2 of the weights' factor, its inverse; key scale -1: there is no block
     __shared__ __align__(16) _Float16 keys[NBUF][kTokens * kKeyLd];
     __shared__ __align__(16) _Float16 vals[NBUF][DP * kTokens];
     auto val_at = [](uint32_t d, uint32_t oct) { return d * kTokens + 8 * (oct ^ ((d >> 1) & 7)); };
@@ -675,12 +683,8 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     for (uint32_t c0 = begin; c0 < end; c0 += kScanTokens) {
         const uint32_t c1 = min(end - c0, kScanTokens) + c0, e0 = c0 >> bs_log;
         __syncthreads();                                        // the last table's readers are done
-        float largest = table_entries(a, b, kv, bs_log, c0, c1, tid, 256, ent_row, ent_k, ent_v);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
-        if (lane == 0) red[wave] = largest;
-        __syncthreads();
-        largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        float largest;
+        if (!table_entries(a, b, kv, bs_log, c0, c1, tid, ent_row, ent_k, ent_v, red, largest)) continue;
         if (largest > 0.0f) {
             if (unit_v > 0.0f && unit_v != largest) {
                 const float change = unit_v / largest;
@@ -695,26 +699,23 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         // weights that vanish as 16-bit floats)
         for (uint32_t i = tid; i <= ((c1 - 1) >> bs_log) - e0; i += 256) {          // (the entries that this thread wrote)
             const float w = largest > 0.0f ? fmaxf(ent_v[i] * (kPScale / largest), 0x1p-60f) : 1.0f;
-            ent[i] = make_float4(ent_k[i], __builtin_amdgcn_logf(w), 1.0f / w, __uint_as_float(ent_row[i] == ~0u ? ~0u : 0u));
+            ent[i] = make_float4(ent_k[i], __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
         }
         __syncthreads();
 
         u32x4 kr[KL];
         uint32_t vr[VL][8];
-        bool v_gone[2];
         const uint32_t k_row = lane >> 2, oct = 2 * wave + (lane >> 5), v_row = 4 * (oct & 3), v_word = lane & 31;
         // the codes from token `start` on (16 of them, in one block; those behind the last token are the last one): their first row's
         // offset, and how many there are
-        auto place = [&](uint32_t start, uint32_t& limit, bool& gone) {
+        auto place = [&](uint32_t start, uint32_t& limit) {
             const uint32_t pos = min(start, c1 - 1), base = __builtin_amdgcn_readfirstlane(ent_row[(pos >> bs_log) - e0]);
             limit = min(c1 - 1 - pos, 15u);
-            gone = base == ~0u;
-            return (uint64_t)((gone ? 0u : base) + (pos & (bs - 1))) * dim;
+            return (uint64_t)(base + (pos & (bs - 1))) * dim;
         };
         auto fetch = [&](uint32_t t0) {
             uint32_t limit;
-            bool gone;
-            const uint8_t* kb = a.k_codes + place(t0 + 16 * wave, limit, gone);     // (scores of tokens of no block are masked)
+            const uint8_t* kb = a.k_codes + place(t0 + 16 * wave, limit);
             const uint32_t kr0 = (limit == 15 ? k_row : min(k_row, limit)) * dim;
 #pragma unroll
             for (int i = 0; i < KL; i++) {
@@ -723,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
             }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const uint8_t* vb = a.v_codes + place(t0 + 32 * (wave >> 1) + 16 * h, limit, v_gone[h]);
+                const uint8_t* vb = a.v_codes + place(t0 + 32 * (wave >> 1) + 16 * h, limit);
 #pragma unroll
                 for (int i = 0; i < VL; i++) {
                     const uint32_t c = 4 * (v_word + 32 * i), at = c < dim ? c : 0;
@@ -738,31 +739,29 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                 }
             }
         };
-        auto store = [&](int buf) {
-#pragma unroll
-            for (int i = 0; i < KL; i++) {
-                _Float16* to = &keys[buf][(16 * wave + k_row) * kKeyLd + 64 * i + 16 * (lane & 3)];
-                *reinterpret_cast<f16x8*>(to) = decode8<CODES>(kr[i][0], kr[i][1]);
-                *reinterpret_cast<f16x8*>(to + 8) = decode8<CODES>(kr[i][2], kr[i][3]);
-            }
-            if (v_gone[0] || v_gone[1]) {
-#pragma unroll
-                for (int i = 0; i < VL; i++)
-#pragma unroll
-                    for (int r = 0; r < 8; r++) vr[i][r] = v_gone[r / 4] ? 0u : vr[i][r];
-            }
-#pragma unroll
-            for (int i = 0; i < VL; i++) {
+        // the codes in registers become 16-bit floats in LDS, piece by piece: eight of a row of keys, or eight of a column of values
+        constexpr int kPieces = 2 * KL + 4 * VL;
+        auto store_piece = [&](int buf, int j) {
+            if (j < 2 * KL) {
+                const int i = j / 2, half = j % 2;
+                *reinterpret_cast<f16x8*>(&keys[buf][(16 * wave + k_row) * kKeyLd + 64 * i + 16 * (lane & 3) + 8 * half]) = decode8<CODES>(kr[i][2 * half], kr[i][2 * half + 1]);
+            } else {
+                const int i = (j - 2 * KL) / 4, col = (j - 2 * KL) % 4;
                 const uint32_t c = 4 * (v_word + 32 * i);
-                if (DP % 128 && c >= DP) break;
                 f16x8 v[4];
                 decode_columns<CODES>(vr[i], v);
-#pragma unroll
-                for (int j = 0; j < 4; j++) *reinterpret_cast<f16x8*>(&vals[buf][val_at(c + j, oct)]) = v[j];
+                if (DP % 128 == 0 || c < DP) *reinterpret_cast<f16x8*>(&vals[buf][val_at(c + col, oct)]) = v[col];
             }
         };
+        auto store = [&](int buf) {
+#pragma unroll
+            for (int j = 0; j < kPieces; j++) store_piece(buf, j);
+        };
         auto compute = [&](uint32_t t0, int buf) {
-            if (t0 >= most) return;                             // none of this wavefront's rows sees the tile
+            if (t0 >= most) {                                   // none of this wavefront's rows sees the tile
+                if constexpr (NBUF == 2) store(buf ^ 1);
+                return;
+            }
             f32x4 s[MT][4];
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
@@ -780,14 +779,14 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 x[t] = ent[(min(t0 + 16 * t, c1 - 1) >> bs_log) - e0];
-                gone[t] = __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].w)) != 0;
+                gone[t] = __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].x)) >> 31;
                 any_gone |= gone[t];
             }
             const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || any_gone;
-            f16x8 p[MT][2][PT];
+            float f[MT][4], ref[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
-                float local = -__builtin_inff(), f[4];
+                float local = -__builtin_inff();
                 if (ragged) {
                     const int left = (int)(min(seen[mt], c1) - t0 - 4 * g);         // (both are below 2^31)
 #pragma unroll
@@ -797,8 +796,8 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                 }
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    f[t] = fmaxf(x[t].x * factor[mt], 0x1p-126f);                   // (not 0, which masked scores would make NaN)
-                    local = fmaxf(local, f[t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
+                    f[mt][t] = fmaxf(x[t].x * factor[mt], 0x1p-126f);               // (not 0, which masked scores would make NaN)
+                    local = fmaxf(local, f[mt][t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
                 }
                 if (__ballot(local > top[mt] + kLead)) {
                     const float now = fmaxf(top[mt], max_over_groups(local));
@@ -808,32 +807,47 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
 #pragma unroll
                     for (int i = 0; i < DT; i++) o[mt][i] *= shrink;
                 }
-                const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+                ref[mt] = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+            }
+            // the two halves of the tile: weights of one while the other's meet the values, and the next tile's codes become
+            // 16-bit floats meanwhile (their loads were issued before the scores)
+            f16x8 p[2][MT][PT];
+            auto weigh = [&](int mt, int t) {
+                const float by = x[t].y - ref[mt];
+                float part_sum = 0.0f;
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const float by = x[t].y - ref;
-                    float part_sum = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][t][r], f[t], by));
-                        part_sum += w;
-                        const _Float16 hi = (_Float16)w;
-                        p[mt][t / 2][0][4 * (t % 2) + r] = hi;
-                        if constexpr (PT == 2) p[mt][t / 2][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
-                    }
-                    sum[mt] = __builtin_fmaf(part_sum, x[t].z, sum[mt]);
+                for (int r = 0; r < 4; r++) {
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][t][r], f[mt][t], by));
+                    part_sum += w;
+                    const _Float16 hi = (_Float16)w;
+                    p[t / 2][mt][0][4 * (t % 2) + r] = hi;
+                    if constexpr (PT == 2) p[t / 2][mt][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
                 }
+                sum[mt] = __builtin_fmaf(part_sum, x[t].z, sum[mt]);
+            };
+            auto meet = [&](int h, int i) {
+                const f16x8 v = *reinterpret_cast<const f16x8*>(&vals[buf][val_at(16 * i + m, 4 * h + g)]);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int pt = 0; pt < PT; pt++) o[mt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[h][mt][pt], o[mt][i], 0, 0, 0);
+            };
+#pragma unroll
+            for (int j = 0; j < 2 * MT; j++) weigh(j / 2, j % 2);
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                meet(0, i);
+#pragma unroll
+                for (int j = i * 2 * MT / DT; j < (i + 1) * 2 * MT / DT; j++) weigh(j / 2, 2 + j % 2);
             }
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int i = 0; i < DT; i++) {
+                meet(1, i);
+                if constexpr (NBUF == 2) {
 #pragma unroll
-                for (int i = 0; i < DT; i++) {
-                    const f16x8 v = *reinterpret_cast<const f16x8*>(&vals[buf][val_at(16 * i + m, 4 * h + g)]);
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                        for (int pt = 0; pt < PT; pt++) o[mt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[mt][h][pt], o[mt][i], 0, 0, 0);
+                    for (int j = i * kPieces / DT; j < (i + 1) * kPieces / DT; j++) store_piece(buf ^ 1, j);
                 }
+            }
         };
 
         fetch(c0);
@@ -841,12 +855,14 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         __syncthreads();
         int buf = 0;
         for (uint32_t t0 = c0; t0 < c1; t0 += kTokens) {
-            const bool more = t0 + kTokens < c1;
-            if (more) fetch(t0 + kTokens);
+            if (t0 + kTokens < c1) fetch(t0 + kTokens);
             compute(t0, buf);
-            if constexpr (NBUF == 1) __syncthreads();           // (the only buffer is about to be overwritten)
-            if (NBUF == 2) buf ^= 1;
-            if (more) store(buf);
+            if constexpr (NBUF == 1) {                          // the only buffer is about to be overwritten
+                __syncthreads();
+                store(0);
+            } else {
+                buf ^= 1;
+            }
             __syncthreads();
         }
     }
