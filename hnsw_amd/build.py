@@ -11,7 +11,7 @@ LIB = os.path.join(HERE, "libhnsw_amd.so")
 def build(verbose: bool = False) -> str:
     out = None if verbose else subprocess.DEVNULL
     # `checks`: the same library with the visited sets' invariants re-read and counted, for one GPU test (never loaded otherwise)
-    subprocess.check_call(["make", "-C", os.path.join(HERE, "csrc"), "-j2", "all", "checks"], stdout=out)
+    subprocess.check_call(["make", "-C", os.path.join(HERE, "csrc"), f"-j{min(8, os.cpu_count() or 1)}", "all", "checks"], stdout=out)
     if not os.path.exists(LIB):
         raise RuntimeError("libhnsw_amd.so was not produced")
     return LIB

@@ -15,20 +15,32 @@ from typing import NamedTuple
 
 from . import capi
 
-_TYPES: dict = {}       # torch dtype -> TYPE_*  (torch is only imported when a cache is used)
+_TYPES: dict = {}       # torch dtype -> TYPE_*
 _CODES: dict = {}       # torch dtype -> CODES_*
+_T = None               # torch, which is only imported when a cache is used
 
 
 def _torch():
-    import torch
-    if not _TYPES:
+    global _T
+    if _T is None:
+        import torch
         _CODES.update({torch.int8: capi.CODES_I8, torch.float8_e4m3fn: capi.CODES_E4M3})
         _TYPES.update({torch.float32: capi.TYPE_F32, torch.float16: capi.TYPE_F16, torch.bfloat16: capi.TYPE_BF16})
-    return torch
+        _T = torch
+    return _T
+
+
+def _stream(device) -> int:
+    """The hipStream_t of the device's current torch stream (torch.cuda.current_stream builds an object first, which costs as much
+    as a launch)."""
+    raw = getattr(_T._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw is not None else _T.cuda.current_stream(device).cuda_stream
 
 
 def _need(t, name, dtype, shape, device):
     """`t` is a contiguous tensor of this type and shape (None: any extent) on `device`."""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == device:
+        return
     if t.dtype is not dtype or t.device != device or t.dim() != len(shape) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {len(shape)}-dimensional {dtype} tensor on {device}")
     for have, want in zip(t.shape, shape):
@@ -54,22 +66,23 @@ def cache_plan(lens, grow, table, ring, state, *, block_tokens: int, n_slots: in
     dev = lens.device
     if dev.type != "cuda":
         raise ValueError("cache_plan: the tensors must be on a GPU")
-    _need(lens, "lens", torch.int32, (None,), dev)
+    i32 = torch.int32
+    _need(lens, "lens", i32, (None,), dev)
     n = lens.shape[0]
-    _need(grow, "grow", torch.int32, (n,), dev)
-    _need(table, "table", torch.int32, (n, None), dev)
-    _need(ring, "ring", torch.int32, (None,), dev)
+    _need(grow, "grow", i32, (n,), dev)
+    _need(table, "table", i32, (n, None), dev)
+    _need(ring, "ring", i32, (None,), dev)
     _need(state, "state", torch.int64, (2,), dev)
     if not 0 <= n_slots < 1 << 31:
         raise ValueError("cache_plan: n_slots must be 0..2^31 - 1")
-    longs = torch.empty(n_slots + 2, dtype=torch.int64, device=dev)
-    words = torch.empty(2 * n + 2, dtype=torch.int32, device=dev)
-    plan = Plan(longs[:n_slots], words[:n + 1], words[n + 1:2 * n + 1], longs[n_slots:], words[2 * n + 1:])
+    longs, words = state.new_empty(n_slots + 2), lens.new_empty(2 * n + 2)
+    slots, state_out = longs.split_with_sizes((n_slots, 2))
+    cu_new, lens_out, status = words.split_with_sizes((n + 1, n, 1))
     at, word = longs.data_ptr(), words.data_ptr()
     capi.check(capi.lib().hnsw_amd_cache_plan_device(lens.data_ptr(), grow.data_ptr(), n, table.data_ptr(), table.shape[1], ring.data_ptr(), ring.shape[0],
                                                      state.data_ptr(), block_tokens, n_slots, at, word, word + 4 * (n + 1), at + 8 * n_slots,
-                                                     word + 4 * (2 * n + 1), dev.index, torch.cuda.current_stream(dev).cuda_stream))
-    return plan
+                                                     word + 4 * (2 * n + 1), dev.index, _stream(dev)))
+    return Plan(slots, cu_new, lens_out, state_out, status)
 
 
 class TokenCache:
@@ -84,8 +97,8 @@ class TokenCache:
             raise ValueError("TokenCache: the buffers must be on a GPU")
         if k_codes.dtype not in _CODES:
             raise ValueError("TokenCache: codes must be int8 or float8_e4m3fn")
-        _need(k_codes, "k_codes", k_codes.dtype, (None,) * 4, dev)
         shape = k_codes.shape
+        _need(k_codes, "k_codes", k_codes.dtype, (None,) * 4, dev)
         _need(v_codes, "v_codes", k_codes.dtype, shape, dev)
         _need(k_scale, "k_scale", torch.float32, shape[:2], dev)
         _need(v_scale, "v_scale", torch.float32, shape[:2], dev)
@@ -100,9 +113,6 @@ class TokenCache:
         shape = (n_blocks, n_heads, block_tokens, dim)
         make = lambda: torch.zeros(shape, dtype=torch.int8, device=device).view(codes or torch.int8)  # noqa: E731
         return cls(make(), make(), torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
-
-    def _stream(self):
-        return _torch().cuda.current_stream(self.device).cuda_stream
 
     def _rows(self, t, name, heads):
         if t.dtype not in _TYPES or t.device != self.device or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.dim:
@@ -122,7 +132,7 @@ class TokenCache:
             raise ValueError("append: k and v must have the same shape and type")
         _need(slots, "slots", torch.int64, (k.shape[0],), self.device)
         capi.check(capi.lib().hnsw_amd_cache_append_device(self._at, k.data_ptr(), v.data_ptr(), k.shape[0], _TYPES[k.dtype], ks[0], ks[1], vs[0], vs[1],
-                                                           slots.data_ptr(), self.device.index, self._stream()))
+                                                           slots.data_ptr(), self.device.index, _stream(self.device)))
 
     def read(self, slots, dtype=None):
         """(keys, values) of the slots [rows] int64: two [rows, n_heads, dim] tensors (float32 unless `dtype` says otherwise)."""
@@ -135,7 +145,7 @@ class TokenCache:
         k = torch.empty((n, self.n_heads, self.dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         capi.check(capi.lib().hnsw_amd_cache_read_device(self._at, slots.data_ptr(), n, _TYPES[dtype], k.data_ptr(), v.data_ptr(), self.device.index,
-                                                         self._stream()))
+                                                         _stream(self.device)))
         return k, v
 
     def _asked(self, q, table, lens, cu_q):
@@ -149,8 +159,7 @@ class TokenCache:
         _need(table, "table", torch.int32, (n, None), dev)
         if cu_q is not None:
             _need(cu_q, "cu_q", torch.int32, (n + 1,), dev)
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        return s, n, out, torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+        return s, n, q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
 
     def attend(self, q, table, lens, *, cu_q=None, causal: bool = True, scale: float | None = None, max_len: int = 0):
         """(out, lse) of the queries q [rows, heads, dim] over all tokens of their requests; table [n, width], lens [n] int32.  Without
@@ -160,11 +169,11 @@ class TokenCache:
         s, n, out, lse = self._asked(q, table, lens, cu_q)
         L, rows, heads, width = capi.lib(), q.shape[0], q.shape[1], table.shape[1]
         nbytes = L.hnsw_amd_cache_attend_workspace(self._at, rows, heads, n, width, max_len)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         capi.check(L.hnsw_amd_cache_attend_device(self._at, q.data_ptr(), rows, heads, s[0], s[1], _TYPES[q.dtype], table.data_ptr(), width, lens.data_ptr(), n,
                                                   cu_q.data_ptr() if cu_q is not None else None, 1 if causal else 0,
                                                   self.dim ** -0.5 if scale is None else scale, max_len, out.data_ptr(), lse.data_ptr(),
-                                                  work.data_ptr() if nbytes else None, nbytes, self.device.index, self._stream()))
+                                                  work.data_ptr() if nbytes else None, nbytes, self.device.index, _stream(self.device)))
         return out, lse
 
     def attend_found(self, q, table, lens, ids, *, cu_q=None, causal: bool = True, scale: float | None = None):
@@ -177,10 +186,10 @@ class TokenCache:
         _need(ids, "ids", torch.int32, (rows, None, None), self.device)
         lists, n_ids = ids.shape[1], ids.shape[2]
         nbytes = L.hnsw_amd_cache_attend_found_workspace(self._at, rows, heads, lists, n_ids)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         capi.check(L.hnsw_amd_cache_attend_found_device(self._at, q.data_ptr(), rows, heads, s[0], s[1], _TYPES[q.dtype], table.data_ptr(), table.shape[1],
                                                         lens.data_ptr(), n, cu_q.data_ptr() if cu_q is not None else None, 1 if causal else 0,
                                                         ids.data_ptr(), lists, n_ids, self.dim ** -0.5 if scale is None else scale,
                                                         out.data_ptr(), lse.data_ptr(), work.data_ptr() if nbytes else None, nbytes,
-                                                        self.device.index, self._stream()))
+                                                        self.device.index, _stream(self.device)))
         return out, lse

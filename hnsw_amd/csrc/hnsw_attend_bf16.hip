@@ -1,0 +1,6 @@
+// The attention for bf16 queries and outputs.
+#include "hnsw_attend_kernels.h"
+
+namespace hnsw_amd {
+template void launch_attend<bf16>(const AttendArgs&, const Cut&, uint32_t, float*, hipStream_t);
+}

@@ -1,0 +1,1052 @@
+// The attention's kernels (what they compute: hnsw_attend.hip), for one row type in each file that includes this.
+#pragma once
+#include "hnsw_attend.h"
+
+namespace hnsw_amd {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWaves = 4;                 // wavefronts of a workgroup of attend_tile_kernel and attend_join_kernel
+constexpr uint32_t kScanTokens = 4096;    // of one table of block entries in LDS (all tokens), and
+constexpr uint32_t kListTokens = 1024;    // of one table of token entries (listed tokens)
+// A softmax's reference is only moved when a score is more than this above it, in base 2: moving it costs as much as a third of a tile
+// (the outputs are multiplied by the change), and over random scores some row of 16 sees a new maximum in every second tile.
+// Probabilities relative to the reference are then up to 2^4, and what they are multiplied by before they become 16-bit floats
+// (largest 2^16) leaves room for that.
+constexpr float kLead = 4.0f;
+constexpr float kPScale = 2048.0f;
+
+template <class T> constexpr int kQTerms = sizeof(T) == 4 ? 2 : 1;                  // 16-bit floats that a query element is split into
+template <class T> constexpr int kPTerms = std::is_same_v<T, bf16> ? 1 : 2;         // and a probability
+
+__device__ __forceinline__ float max_over_groups(float x)       // over the four lanes that share lane & 15
+{
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float x)
+{
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ f16x2 as_f16x2(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+
+// Two signed bytes, each in the low half of a 16-bit lane of w (the high halves are 0), as 16-bit floats: with its sign bit turned a
+// byte is code + 128, and 0x6400 | b is the 16-bit float 1024 + b, so 1152 less is the code, exactly.
+__device__ __forceinline__ f16x2 bytes_to_f16(uint32_t w)
+{
+    return as_f16x2(w ^ 0x64806480u) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
+}
+
+// Eight consecutive codes of a row as 16-bit floats (exact for both kinds of codes).  Signed bytes come out in the order
+// 0 2 1 3 4 6 5 7, which the queries are laid out to match.
+template <int CODES> __device__ __forceinline__ f16x8 decode8(uint32_t w0, uint32_t w1)
+{
+    union { f16x8 v; f16x2 h[4]; } u;
+    if constexpr (CODES == HNSW_AMD_CODES_I8) {
+        u.h[0] = bytes_to_f16(w0 & 0x00ff00ffu);
+        u.h[1] = bytes_to_f16((w0 >> 8) & 0x00ff00ffu);
+        u.h[2] = bytes_to_f16(w1 & 0x00ff00ffu);
+        u.h[3] = bytes_to_f16((w1 >> 8) & 0x00ff00ffu);
+    } else {
+        u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
+        u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
+        u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
+        u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
+    }
+    return u.v;
+}
+constexpr int kOrderI8[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+
+// Byte b of eight rows' words (one word of each of two times four rows), as 16-bit floats: a column of the values.
+template <int CODES> __device__ __forceinline__ void decode_columns(const uint32_t (&w)[8], f16x8 (&out)[4])
+{
+    union U { f16x8 v; f16x2 h[4]; };
+    U u[4];
+    if constexpr (CODES == HNSW_AMD_CODES_I8) {
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                u[b].h[j] = bytes_to_f16(__builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x0c000c00u | ((4u + b) << 16) | (uint32_t)b));
+    } else {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t* x = &w[4 * half];
+            const uint32_t a0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), a1 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+            const uint32_t c0 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u), c1 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+            const uint32_t t[4] = {__builtin_amdgcn_perm(c0, a0, 0x05040100u), __builtin_amdgcn_perm(c0, a0, 0x07060302u),
+                                   __builtin_amdgcn_perm(c1, a1, 0x05040100u), __builtin_amdgcn_perm(c1, a1, 0x07060302u)};
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                u[b].h[2 * half] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(t[b], 1.0f, false);
+                u[b].h[2 * half + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(t[b], 1.0f, true);
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++) out[b] = u[b].v;
+}
+
+// Where a request's rows lie among the query rows, kept within n_rows whatever cu_q holds.
+struct Span { uint32_t first, count; };
+__device__ __forceinline__ Span rows_of(const AttendArgs& a, uint32_t b)
+{
+    if (!a.cu_q) return {b, 1};
+    const int64_t lo = min(max((int64_t)a.cu_q[b], (int64_t)0), (int64_t)a.n_rows), hi = min(max((int64_t)a.cu_q[b + 1], lo), (int64_t)a.n_rows);
+    return {(uint32_t)lo, (uint32_t)(hi - lo)};
+}
+__device__ __forceinline__ Span uniform(Span s)                 // the same in all lanes: say so
+{
+    return {(uint32_t)__builtin_amdgcn_readfirstlane(s.first), (uint32_t)__builtin_amdgcn_readfirstlane(s.count)};
+}
+__device__ __forceinline__ uint32_t length_of(const AttendArgs& a, uint32_t b)
+{
+    const int64_t cap = (int64_t)a.width * a.block_tokens;
+    return (uint32_t)min(max((int64_t)a.lens[b], (int64_t)0), cap);
+}
+// tokens that row i of a request's n rows sees
+__device__ __forceinline__ uint32_t seen_by(const AttendArgs& a, uint32_t len, uint32_t n, uint32_t i)
+{
+    if (!a.causal) return len;
+    const int64_t s = (int64_t)len - n + i + 1;
+    return (uint32_t)min(max(s, (int64_t)0), (int64_t)len);
+}
+
+// Unit u of the rows cut into tiles of `tile` (row, head) pairs, request after request: its request and the tile within it; false
+// when there are fewer units.
+__device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_t group, uint32_t tile, uint32_t lane, uint32_t& request, uint32_t& part)
+{
+    if (!a.cu_q) {
+        const uint32_t per = (group + tile - 1) / tile;
+        request = u / per;
+        part = u - request * per;
+        return request < a.n_requests;
+    }
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.n_requests; b0 += 64) {
+        uint32_t n = 0;
+        if (b0 + lane < a.n_requests) n = (uint32_t)(((uint64_t)rows_of(a, b0 + lane).count * group + tile - 1) / tile);
+        uint32_t upto = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(upto, off);
+            if (lane >= (uint32_t)off) upto += y;
+        }
+        const unsigned long long m = __ballot(before + upto > u);
+        if (m) {
+            const int at = __builtin_ctzll(m);
+            request = b0 + at;
+            part = __builtin_amdgcn_readfirstlane(u - before - (__shfl(upto, at) - __shfl(n, at)));
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+// A query row as it lies in memory, eight elements from column col(s) on for step s (zeros behind dim, or where there is no row): the
+// loads.
+template <class T, int KS> struct RawQuery { T x[KS][8]; };
+template <class T, int KS, class Col>
+__device__ __forceinline__ void load_query(const AttendArgs& a, bool there, uint32_t row, uint32_t head, uint32_t vec, Col&& col, RawQuery<T, KS>& raw)
+{
+    const T* x = (const T*)a.q + (int64_t)row * a.q_row_stride + (int64_t)head * a.q_head_stride;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const uint32_t c = col(s);
+#pragma unroll
+        for (int j = 0; j < 8; j++) raw.x[s][j] = T{};
+        if (there && c < a.dim) {
+            if (vec) {
+                struct alignas(16) Piece { T x[16 / sizeof(T)]; };
+#pragma unroll
+                for (int h = 0; h < (int)sizeof(T) / 2; h++) {
+                    const Piece p = *reinterpret_cast<const Piece*>(x + c + h * (16 / sizeof(T)));
+#pragma unroll
+                    for (int j = 0; j < (int)(16 / sizeof(T)); j++) raw.x[s][h * (16 / sizeof(T)) + j] = p.x[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) raw.x[s][j] = x[c + j];
+            }
+        }
+    }
+}
+// Its operands, and what the products with codes are multiplied by to be scores in base 2.  The row is scaled by the power of two that
+// puts its largest element into [2^14, 2^15).  The four lanes that share a row call this together.
+template <class T, int CODES, int KS, int QT>
+__device__ __forceinline__ float query_operands(const AttendArgs& a, const RawQuery<T, KS>& raw, f16x8 (&q)[KS][QT])
+{
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;           // (goes into the queries, so that factors are not negative)
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(to_float(raw.x[s][j])));
+    top = max_over_groups(top);
+    const int e = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float y = ldexpf(to_float(raw.x[s][CODES == HNSW_AMD_CODES_I8 ? kOrderI8[j] : j]) * sign, e);
+            const _Float16 hi = (_Float16)y;
+            q[s][0][j] = hi;
+            if constexpr (QT == 2) q[s][1][j] = (_Float16)(y - (float)hi);
+        }
+    return ldexpf(fabsf(a.scale) * kLog2e, -e);
+}
+
+// Block entries of the tokens c0 .. c1 of request b into LDS, by a workgroup of 256 threads: first row of a block's codes (in rows of dim
+// bytes) and its scales.  An entry of no block has the key scale -1 and the row of one that is, so that loads stay among codes of
+// live tokens: weights of 0 do not meet the NaN that stale codes can be.  Returns the largest value scale; false where no entry is of a block.
+struct Reduced { float largest[kWaves]; uint32_t some[kWaves]; };
+__device__ __forceinline__ bool table_entries(const AttendArgs& a, uint32_t b, uint32_t kv, uint32_t bs_log, uint32_t c0, uint32_t c1, uint32_t tid,
+                                              uint32_t* ent_row, float* ent_k, float* ent_v, Reduced& red, float& largest)
+{
+    const uint32_t e0 = c0 >> bs_log, n_e = ((c1 - 1) >> bs_log) - e0 + 1, lane = tid & 63, wave = tid >> 6;
+    uint32_t some = 0;                                          // a row + 1
+    largest = 0.0f;
+    for (uint32_t i = tid; i < n_e; i += 256) {
+        const uint32_t blk = (uint32_t)a.table[(size_t)b * a.width + e0 + i];
+        uint32_t row = 0;
+        float sk = -1.0f, sv = 0.0f;
+        if (blk < a.n_blocks) {
+            const uint32_t bh = blk * a.n_heads + kv;
+            row = bh << bs_log;
+            sk = a.k_scale[bh];
+            sv = a.v_scale[bh];
+            some = row + 1;
+            largest = fmaxf(largest, sv);
+        }
+        ent_row[i] = row; ent_k[i] = sk; ent_v[i] = sv;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        largest = fmaxf(largest, __shfl_xor(largest, off));
+        some = max(some, (uint32_t)__shfl_xor((int)some, off));
+    }
+    if (lane == 0) { red.largest[wave] = largest; red.some[wave] = some; }
+    __syncthreads();
+    largest = fmaxf(fmaxf(red.largest[0], red.largest[1]), fmaxf(red.largest[2], red.largest[3]));
+    some = __builtin_amdgcn_readfirstlane(max(max(red.some[0], red.some[1]), max(red.some[2], red.some[3])));
+    for (uint32_t i = tid; i < n_e; i += 256)                   // (the entries that this thread wrote)
+        if (ent_k[i] < 0.0f) ent_row[i] = some - 1;
+    return some != 0;
+}
+
+// Attention of few query rows over many tokens: for single tokens the codes are read once and that is the time.
+//
+// The workgroup takes one key head of one request (or one list), up to 16 * MT rows of queries and one chunk of the tokens; its
+// NW wavefronts take tiles of 32 tokens in turn, each with a softmax of its own, and join at the end.  Scores are computed
+// transposed, S^T = K Q^T, with v_mfma_f32_16x16x32_f16: the lane that then holds scores of query (lane & 15) is the one that needs
+// their probabilities as the operand of O^T = V^T P^T, so that nothing is exchanged between lanes, and the softmax's maximum and
+// sum are scalars of a lane.  Codes go from memory to registers as the matrix instructions want them, without LDS:
+//   keys    lane (m, g): row m of 16, 16-byte pieces g, g + 4, ... (the order of the dims is free as long as the queries have it too)
+//   values  lane (m, g): the same DP / 16 bytes of rows 4g .. 4g + 3 of both halves of the tile; a byte of eight rows is an operand
+// and the next tile is under way while one is computed.  Codes become 16-bit floats, which hold both kinds exactly.
+// Queries are scaled by a power of two to just under 2^15 and rounded to 16-bit floats (nothing is lost of bf16 and f16 but what
+// lies 2^-29 under the row's largest element); 32-bit queries are split into two terms.  A block's key scale multiplies the
+// scores; its value scale, over the largest of the table's, multiplies the probabilities, which as 16-bit floats in units of 2^-11
+// reach down to 2^-35 of the reference: 2^-11 of each is rounded away for bf16 rows (whose outputs keep 2^-8), and a second term
+// takes that up for the others.  Sums, maxima and outputs are in 32 bits.
+// A workgroup's start is a chain of loads that wait for one another (length, table, codes; for lists: ids, table, codes): the first
+// tile's codes are asked for as soon as the table is there, and queries and scales are made ready meanwhile.
+template <class T, int CODES, int DP, int MT, int NW, bool FOUND>
+__global__ __launch_bounds__(64 * NW) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
+{
+    constexpr int KS = DP / 32, KW = DP / 64, VW = DP / 64, VB = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
+    constexpr uint32_t kThreads = 64 * NW, kTable = FOUND ? (NW == 1 ? 256 : kListTokens) : (NW == 1 ? 1024 : kScanTokens);      // items of a table
+    constexpr uint32_t kEntries = FOUND ? kTable + kTile : kTable / 16 + 1, kMine = FOUND ? kTable / kThreads : 1;   // (one a thread of all tokens: 16 to a block at least)
+    static_assert(FOUND || kTable / 16 <= kThreads);
+    constexpr int kOutLd = DP + 4, kJoin = NW == 1 ? 1 : NW / 2;
+    __shared__ uint32_t ent_row[kEntries];                      // first row of a block's (a token's) codes, in rows of dim bytes; ~0: of no block
+    __shared__ __align__(16) float ent_k[kEntries], ent_v[kEntries];         // its scales; key scale -1: of no block
+    __shared__ __align__(16) float join[kJoin][16 * MT][kOutLd];
+    __shared__ float join_m[NW][16 * MT], join_l[NW][16 * MT], red[NW];
+    __shared__ uint32_t red_n[NW];
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t head = blockIdx.x % heads, unit = blockIdx.x / heads, split = blockIdx.y;
+    const uint32_t dim = a.dim, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs);
+    const uint32_t group = a.q_heads / heads;                   // rows of a token: query heads that share this key head, or list
+    const uint32_t kv = FOUND ? head / (heads / a.n_heads) : head;
+
+    // which rows: `first` + r / group is the query row of row r, head * group + r % group its head
+    uint32_t b, first, count, r0;
+    if constexpr (FOUND) {
+        const uint32_t per = (group + 16 * MT - 1) / (16 * MT);
+        first = unit / per;
+        r0 = (unit - first * per) * 16 * MT;
+        if (first >= a.n_rows) return;
+        b = __builtin_amdgcn_readfirstlane(a.cu_q ? request_of(a.cu_q, a.n_requests, first) : first);
+        if (b >= a.n_requests) return;
+        count = 1;
+    } else {
+        uint32_t part;
+        if (!unit_of(a, unit, group, 16 * MT, lane, b, part)) return;
+        const Span s = uniform(rows_of(a, b));
+        first = s.first;
+        count = s.count;
+        r0 = part * 16 * MT;
+    }
+    const uint32_t n_r = count * group;                         // (fits: n_rows * q_heads < 2^24)
+    if (r0 >= n_r) return;
+
+    // the rows of this lane's columns: their queries, and what they see
+    RawQuery<T, KS> raw[MT];
+    uint32_t seen[MT], least = 0xffffffffu, most = 0;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const uint32_t r = r0 + 16 * mt + m;
+        const bool there = r < n_r;
+        const uint32_t i = there ? r / group : 0, h = head * group + (there ? r - i * group : 0);
+        load_query<T, KS>(a, there, first + i, h, q_vec, [&](int s) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); }, raw[mt]);
+    }
+    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const uint32_t r = r0 + 16 * mt + m;
+        if constexpr (FOUND) {
+            const Span s = rows_of(a, b);
+            seen[mt] = seen_by(a, len, s.count, first - s.first);
+        } else {
+            seen[mt] = r < n_r ? seen_by(a, len, count, r / group) : 0;
+        }
+    }
+    // (rows follow one another in what they see)
+    if constexpr (FOUND) {
+        least = most = seen[0];
+    } else {
+        least = seen_by(a, len, count, r0 / group);
+        most = seen_by(a, len, count, (min(r0 + 16 * MT, n_r) - 1) / group);
+    }
+
+    const uint32_t all = FOUND ? a.n_ids : most;                // items: tokens, or list entries
+    const uint32_t begin = split * parts.chunk;
+    if (!FOUND && split > 0 && begin >= all) return;            // (a row that sees no token of a chunk does not ask for its part)
+    const uint32_t end = split + 1 < parts.n_splits ? min(begin + parts.chunk, all) : all;
+
+    f16x8 q[MT][KS][QT];
+    float factor[MT];                                           // of the products: scores in base 2
+    f32x4 o[MT][VB];
+    float top[MT], sum[MT], unit_v = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        top[mt] = -__builtin_inff();
+        sum[mt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VB; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    bool ready = false;                                         // the queries are
+    auto make_ready = [&]() {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
+        ready = true;
+    };
+
+    for (uint32_t c0 = begin; c0 < end; c0 += kTable) {
+        const uint32_t c1 = min(end - c0, kTable) + c0;
+        uint32_t n = c1 - c0, e0 = 0, safe = 0;                 // items in the table; a row of codes of a live token
+        uint32_t bh[kMine], at[kMine];                          // (block, head) of this thread's entries, ~0: of none, and their places
+        if (c0 != begin) __syncthreads();                       // the table's last readers are done
+        if constexpr (FOUND) {
+            // listed tokens that the row sees and that exist, moved together (in order): entries, then 32 or less that weigh nothing
+            const int32_t* ids = a.ids + ((size_t)first * heads + head) * a.n_ids;
+            uint32_t id[kMine], kept = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < kMine; e++) id[e] = e * kThreads + tid < n ? (uint32_t)ids[c0 + e * kThreads + tid] : ~0u;
+#pragma unroll
+            for (uint32_t e = 0; e < kMine; e++) {
+                const uint32_t blk = id[e] < seen[0] ? (uint32_t)a.table[(size_t)b * a.width + (id[e] >> bs_log)] : ~0u;
+                bh[e] = blk < a.n_blocks ? blk * a.n_heads + kv : ~0u;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < kMine; e++) {
+                if (e * kThreads >= n) break;
+                const unsigned long long mine = __ballot(bh[e] != ~0u);
+                if (e) __syncthreads();
+                if (lane == 0) red_n[wave] = (uint32_t)__popcll(mine);
+                __syncthreads();
+                at[e] = kept + (uint32_t)__popcll(mine & ((1ull << lane) - 1));
+                for (uint32_t w = 0; w < NW; w++) {
+                    if (w < wave) at[e] += red_n[w];
+                    kept += red_n[w];
+                }
+                if (bh[e] != ~0u) ent_row[at[e]] = (bh[e] << bs_log) + (id[e] & (bs - 1));
+            }
+            n = kept;
+            if (n == 0) continue;                               // (the same in all threads)
+            __syncthreads();
+            if (tid < kTile) { ent_row[n + tid] = ent_row[n - 1]; ent_k[n + tid] = 0.0f; ent_v[n + tid] = 0.0f; }
+            __syncthreads();
+        } else {
+            e0 = c0 >> bs_log;
+            const bool mine = tid <= ((c1 - 1) >> bs_log) - e0;
+            const uint32_t blk = mine ? (uint32_t)a.table[(size_t)b * a.width + e0 + tid] : ~0u;
+            bh[0] = blk < a.n_blocks ? blk * a.n_heads + kv : ~0u;
+            if (mine) ent_row[tid] = bh[0] == ~0u ? ~0u : bh[0] << bs_log;
+            const unsigned long long fine = __ballot(bh[0] != ~0u);
+            if (lane == 0) red_n[wave] = fine ? (__builtin_amdgcn_readlane(bh[0], __builtin_ctzll(fine)) << bs_log) + 1 : 0;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; w++) safe = safe ? safe : red_n[w];
+            safe = __builtin_amdgcn_readfirstlane(safe);
+            if (!safe--) continue;                              // none of these blocks exists
+        }
+
+        // a tile's codes: where they are, and the loads
+        struct Tile { u32x4 k[2][KW]; uint32_t v[8][VW]; };
+        const uint32_t k_col = min(16 * g, dim - 16), v_col = VB * m;
+        auto fetch = [&](uint32_t j, Tile& t) {
+            const uint32_t i0 = 32 * j;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t row_k, row_v[4];
+                const uint8_t *kb = a.k_codes, *vb = a.v_codes;
+                if constexpr (FOUND) {
+                    row_k = ent_row[i0 + 16 * h + m];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) row_v[r] = ent_row[i0 + 16 * h + 4 * g + r];
+                } else {
+                    const uint32_t last = c1 - 1, start = min(c0 + i0 + 16 * h, last);
+                    uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
+                    if (base == ~0u) base = safe;               // (stale codes can be NaN, which a weight of 0 would not remove)
+                    const uint64_t at = (uint64_t)(base + (start & (bs - 1))) * dim;
+                    kb += at;
+                    vb += at;
+                    row_k = min(m, last - start);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) row_v[r] = min(4 * g + r, last - start);
+                }
+                auto offset = [&](uint32_t row) { if constexpr (FOUND) return (uint64_t)row * dim; else return row * dim; };
+#pragma unroll
+                for (int i = 0; i < KW; i++)
+                    t.k[h][i] = *reinterpret_cast<const u32x4*>(kb + offset(row_k) + (64 * i + 16 * g < dim ? 64 * i + 16 * g : k_col));
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint8_t* p = vb + offset(row_v[r]);
+                    if constexpr (VW == 2) {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(p + (v_col + 8 <= dim ? v_col : 0));
+                        t.v[4 * h + r][0] = w[0]; t.v[4 * h + r][1] = w[1];
+                    } else if constexpr (VW == 4) {
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(p + (v_col + 16 <= dim ? v_col : 0));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) t.v[4 * h + r][i] = w[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VW; i++) t.v[4 * h + r][i] = *reinterpret_cast<const uint32_t*>(p + (v_col + 4 * i + 4 <= dim ? v_col + 4 * i : 0));
+                    }
+                }
+            }
+        };
+        const uint32_t tiles = (n + kTile - 1) / kTile;
+        Tile t[2];
+        if (wave < tiles) fetch(wave, t[0]);
+        if (!ready) make_ready();
+        // the entries' scales, and the largest value scale
+        float largest = 0.0f;
+#pragma unroll
+        for (uint32_t e = 0; e < kMine; e++) {
+            if constexpr (FOUND) {
+                if (bh[e] != ~0u) {
+                    const float sv = a.v_scale[bh[e]];
+                    ent_k[at[e]] = a.k_scale[bh[e]];
+                    ent_v[at[e]] = sv;
+                    largest = fmaxf(largest, sv);
+                }
+            } else if (tid <= ((c1 - 1) >> bs_log) - e0) {
+                const float sv = bh[0] != ~0u ? a.v_scale[bh[0]] : 0.0f;
+                ent_k[tid] = bh[0] != ~0u ? a.k_scale[bh[0]] : -1.0f;
+                ent_v[tid] = sv;
+                largest = sv;
+            }
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
+        if (lane == 0) red[wave] = largest;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; w++) largest = fmaxf(largest, red[w]);
+        const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
+        if (largest > 0.0f) {
+            if (unit_v > 0.0f && unit_v != largest) {           // outputs so far are in units of the last table's largest scale
+                const float change = unit_v / largest;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < VB; i++) o[mt][i] *= change;
+            }
+            unit_v = largest;
+        }
+
+        auto take = [&](uint32_t j, Tile& t) {
+            const uint32_t i0 = 32 * j;
+            f32x4 s[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const f16x8 k = decode8<CODES>(t.k[h][ks / 2][2 * (ks % 2)], t.k[h][ks / 2][2 * (ks % 2) + 1]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int qt = 0; qt < QT; qt++) s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], s[mt][h], 0, 0, 0);
+                }
+            float fk[2][4], pw[2][4];                           // the scales of this lane's tokens 4g + r of both halves
+            bool gone[2] = {false, false}, ragged;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if constexpr (FOUND) {
+                    const float4 x = *reinterpret_cast<const float4*>(&ent_k[i0 + 16 * h + 4 * g]), y = *reinterpret_cast<const float4*>(&ent_v[i0 + 16 * h + 4 * g]);
+                    fk[h][0] = x.x; fk[h][1] = x.y; fk[h][2] = x.z; fk[h][3] = x.w;
+                    pw[h][0] = y.x * per_v; pw[h][1] = y.y * per_v; pw[h][2] = y.z * per_v; pw[h][3] = y.w * per_v;
+                } else {
+                    const uint32_t e = (min(c0 + i0 + 16 * h, c1 - 1) >> bs_log) - e0;
+                    const float x = ent_k[e], y = ent_v[e] * per_v;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) { fk[h][r] = x; pw[h][r] = y; }
+                    gone[h] = __builtin_amdgcn_readfirstlane(__float_as_uint(x)) >> 31;
+                }
+            }
+            if constexpr (FOUND) ragged = i0 + 32 > n;
+            else ragged = c0 + i0 + 32 > least || c0 + i0 + 32 > c1 || gone[0] || gone[1];
+            f16x8 p[MT][PT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                float x[2][4], local = -__builtin_inff();
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[h][r] = s[mt][h][r] * (fk[h][r] * factor[mt]);
+                if (ragged) {
+                    const int left = (int)((FOUND ? n : min(seen[mt], c1) - c0) - i0 - 4 * g);
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) x[h][r] = 16 * h + r < left && !gone[h] ? x[h][r] : -__builtin_inff();
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) local = fmaxf(local, x[h][r]);
+                if (__ballot(local > top[mt] + kLead)) {        // rare after the first tile
+                    const float now = fmaxf(top[mt], max_over_groups(local));
+                    const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
+                    top[mt] = now;
+                    sum[mt] *= shrink;
+#pragma unroll
+                    for (int i = 0; i < VB; i++) o[mt][i] *= shrink;
+                }
+                const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float y = __builtin_amdgcn_exp2f(x[h][r] - ref);
+                        sum[mt] += y;
+                        const float w = y * pw[h][r];
+                        const _Float16 hi = (_Float16)w;
+                        p[mt][0][4 * h + r] = hi;
+                        if constexpr (PT == 2) p[mt][1][4 * h + r] = (_Float16)(w - (float)hi);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < VW; i++) {
+                uint32_t w[8];
+                f16x8 v[4];
+#pragma unroll
+                for (int r = 0; r < 8; r++) w[r] = t.v[r][i];
+                decode_columns<CODES>(w, v);
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int pt = 0; pt < PT; pt++) o[mt][4 * i + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p[mt][pt], o[mt][4 * i + c], 0, 0, 0);
+            }
+        };
+        for (uint32_t j = wave; j < tiles; j += 2 * NW) {
+            if (j + NW < tiles) fetch(j + NW, t[1]);
+            take(j, t[0]);
+            if (j + NW >= tiles) break;
+            if (j + 2 * NW < tiles) fetch(j + 2 * NW, t[0]);
+            take(j + NW, t[1]);
+        }
+    }
+
+    // the wavefronts' softmaxes become one
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        sum[mt] = sum_over_groups(sum[mt]);
+        if (g == 0) { join_m[wave][16 * mt + m] = top[mt]; join_l[wave][16 * mt + m] = sum[mt]; }
+    }
+    __syncthreads();
+    auto ref_of = [&](uint32_t r) {
+        float x = join_m[0][r];
+#pragma unroll
+        for (int w = 1; w < NW; w++) x = fmaxf(x, join_m[w][r]);
+        return x == -__builtin_inff() ? 0.0f : x;
+    };
+    auto put = [&](bool add) {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            const float f = __builtin_amdgcn_exp2f(top[mt] - ref_of(16 * mt + m));
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int i = 0; i < VB; i += 4) {
+                    float4* to = reinterpret_cast<float4*>(&join[wave % kJoin][16 * mt + m][(4 * g + r) * VB + i]);
+                    float4 x = make_float4(o[mt][i][r] * f, o[mt][i + 1][r] * f, o[mt][i + 2][r] * f, o[mt][i + 3][r] * f);
+                    if (add) { const float4 y = *to; x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); }
+                    *to = x;
+                }
+        }
+    };
+    if (wave >= kJoin || NW == 1) put(false);
+    __syncthreads();
+    if constexpr (NW > 1) {
+        if (wave < kJoin) put(true);
+        __syncthreads();
+    }
+    auto joined = [&](uint32_t r, uint32_t d) {
+        float x = join[0][r][d];
+#pragma unroll
+        for (int w = 1; w < kJoin; w++) x += join[w][r][d];
+        return x;
+    };
+    const float unit_o = unit_v / kPScale;
+    for (uint32_t r = wave; r < 16 * MT && r0 + r < n_r; r += NW) {
+        const uint32_t i = (r0 + r) / group;
+        const size_t to = (size_t)(first + i) * a.q_heads + head * group + (r0 + r - i * group);
+        const float ref = ref_of(r);
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) l += join_l[w][r] * __builtin_amdgcn_exp2f(join_m[w][r] - ref);
+        const float inv = l == 0.0f ? 0.0f : unit_o / l;
+        if (parts.n_splits == 1) {
+            for (uint32_t d = lane; d < dim; d += 64) ((T*)a.out)[to * dim + d] = from_float<T>(joined(r, d) * inv);
+            if (lane == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        } else {
+            const size_t at = to * parts.n_splits + split;
+            for (uint32_t d = lane; d < dim; d += 64) parts.out[at * dim + d] = joined(r, d) * inv;
+            if (lane == 0) parts.lse[at] = l == 0.0f ? -__builtin_inff() : ref + __builtin_amdgcn_logf(l);
+        }
+    }
+}
+
+// Attention of many query rows: prompts.  The codes of 64 tokens become 16-bit floats once for all 64 * MT rows of the workgroup: in
+// LDS, keys [token][dim] (rows of an odd number of 16-byte pieces, so that operands are read without bank conflicts), values
+// [dim][token] (the eight tokens of a matrix operand next to each other, the pieces of a row in an order that differs by row to
+// the same end), while the next tile's codes are on their way to registers: each wavefront moves the keys of 16 tokens and a quarter
+// of the values' octets, so that the blocks they lie in are scalars.
+// Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel, but that a block's value scale goes
+// into the exponent instead of being multiplied in: weights are 2^(score - maximum + log2 of the scale over the table's largest), their
+// sum is put right by the inverse per 16 tokens.
+template <class T, int CODES, int DP, int MT, int NBUF>
+__global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
+{
+    constexpr int KS = DP / 32, DT = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
+    constexpr int kTokens = 64, kKeyLd = DP + 8;                 // 16-bit elements
+    constexpr int KL = DP / 64, VL = (DP + 127) / 128;          // 16-byte pieces of keys, and words x 8 tokens of values, that a thread moves
+    constexpr uint32_t kEntries = kScanTokens / 16 + 2;
+    __shared__ uint32_t ent_row[kEntries];
+    __shared__ float ent_k[kEntries], ent_v[kEntries];
+    __shared__ Reduced red;
+    __shared__ __align__(16) float4 ent[kEntries];              // key scale, log2 of the weights' factor, its inverse; key scale -1: there is no block
+    __shared__ __align__(16) _Float16 keys[NBUF][kTokens * kKeyLd];
+    __shared__ __align__(16) _Float16 vals[NBUF][DP * kTokens];
+    auto val_at = [](uint32_t d, uint32_t oct) { return d * kTokens + 8 * (oct ^ ((d >> 1) & 7)); };
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t kv = blockIdx.x % a.n_heads, split = blockIdx.y;
+    const uint32_t unit = gridDim.x / a.n_heads - 1 - blockIdx.x / a.n_heads;   // the last rows of a prompt see the most: first
+    const uint32_t dim = a.dim, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs);
+    const uint32_t group = a.q_heads / a.n_heads;
+    constexpr uint32_t kRows = kWaves * 16 * MT;
+    uint32_t b, part;
+    if (!unit_of(a, unit, group, kRows, lane, b, part)) return;
+    const Span rows = uniform(rows_of(a, b));
+    const uint32_t n_r = rows.count * group, r0 = part * kRows + wave * 16 * MT;
+    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
+
+    uint32_t seen[MT], least = 0xffffffffu, most = 0;
+    f16x8 q[MT][KS][QT];
+    float factor[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const uint32_t r = r0 + 16 * mt + m;
+        const bool there = r < n_r;
+        const uint32_t i = there ? r / group : 0, h = kv * group + (there ? r - i * group : 0);
+        seen[mt] = there ? seen_by(a, len, rows.count, i) : 0;
+        if (there) { least = min(least, seen[mt]); most = max(most, seen[mt]); }
+        RawQuery<T, KS> raw;
+        load_query<T, KS>(a, there, rows.first + i, h, q_vec, [&](int s) { return 32 * s + 8 * g; }, raw);
+        factor[mt] = query_operands<T, CODES, KS, QT>(a, raw, q[mt]);
+    }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+        least = min(least, (uint32_t)__shfl_xor((int)least, off));
+        most = max(most, (uint32_t)__shfl_xor((int)most, off));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    // what the workgroup's last row sees
+    const uint32_t last_r = min((part + 1) * kRows, n_r) - 1;
+    const uint32_t all = seen_by(a, len, rows.count, last_r / group);
+    const uint32_t begin = split * parts.chunk;
+    if (split > 0 && begin >= all) return;
+    const uint32_t end = split + 1 < parts.n_splits ? min(begin + parts.chunk, all) : all;
+
+    f32x4 o[MT][DT];
+    float top[MT], sum[MT], unit_v = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        top[mt] = -__builtin_inff();
+        sum[mt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (uint32_t c0 = begin; c0 < end; c0 += kScanTokens) {
+        const uint32_t c1 = min(end - c0, kScanTokens) + c0, e0 = c0 >> bs_log;
+        __syncthreads();                                        // the last table's readers are done
+        float largest;
+        if (!table_entries(a, b, kv, bs_log, c0, c1, tid, ent_row, ent_k, ent_v, red, largest)) continue;
+        if (largest > 0.0f) {
+            if (unit_v > 0.0f && unit_v != largest) {
+                const float change = unit_v / largest;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < DT; i++) o[mt][i] *= change;
+            }
+            unit_v = largest;
+        }
+        // weights get a block's value scale over the largest by way of the exponent (a scale of 0 next to others counts as 2^-60 of it:
+        // weights that vanish as 16-bit floats)
+        for (uint32_t i = tid; i <= ((c1 - 1) >> bs_log) - e0; i += 256) {          // (the entries that this thread wrote)
+            const float w = largest > 0.0f ? fmaxf(ent_v[i] * (kPScale / largest), 0x1p-60f) : 1.0f;
+            ent[i] = make_float4(ent_k[i], __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
+        }
+        __syncthreads();
+
+        u32x4 kr[KL];
+        uint32_t vr[VL][8];
+        const uint32_t k_row = lane >> 2, oct = 2 * wave + (lane >> 5), v_row = 4 * (oct & 3), v_word = lane & 31;
+        // the codes from token `start` on (16 of them, in one block; those behind the last token are the last one): their first row's
+        // offset, and how many there are
+        auto place = [&](uint32_t start, uint32_t& limit) {
+            const uint32_t pos = min(start, c1 - 1), base = __builtin_amdgcn_readfirstlane(ent_row[(pos >> bs_log) - e0]);
+            limit = min(c1 - 1 - pos, 15u);
+            return (uint64_t)(base + (pos & (bs - 1))) * dim;
+        };
+        auto fetch = [&](uint32_t t0) {
+            uint32_t limit;
+            const uint8_t* kb = a.k_codes + place(t0 + 16 * wave, limit);
+            const uint32_t kr0 = (limit == 15 ? k_row : min(k_row, limit)) * dim;
+#pragma unroll
+            for (int i = 0; i < KL; i++) {
+                const uint32_t c = 64 * i + 16 * (lane & 3);
+                kr[i] = *reinterpret_cast<const u32x4*>(kb + kr0 + (c < dim ? c : 0));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint8_t* vb = a.v_codes + place(t0 + 32 * (wave >> 1) + 16 * h, limit);
+#pragma unroll
+                for (int i = 0; i < VL; i++) {
+                    const uint32_t c = 4 * (v_word + 32 * i), at = c < dim ? c : 0;
+                    if (limit == 15) {
+                        const uint32_t v0 = v_row * dim + at;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(vb + (size_t)r * dim + v0);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(vb + min(v_row + r, limit) * dim + at);
+                    }
+                }
+            }
+        };
+        // the codes in registers become 16-bit floats in LDS, piece by piece: eight of a row of keys, or eight of a column of values
+        constexpr int kPieces = 2 * KL + 4 * VL;
+        auto store_piece = [&](int buf, int j) {
+            if (j < 2 * KL) {
+                const int i = j / 2, half = j % 2;
+                *reinterpret_cast<f16x8*>(&keys[buf][(16 * wave + k_row) * kKeyLd + 64 * i + 16 * (lane & 3) + 8 * half]) = decode8<CODES>(kr[i][2 * half], kr[i][2 * half + 1]);
+            } else {
+                const int i = (j - 2 * KL) / 4, col = (j - 2 * KL) % 4;
+                const uint32_t c = 4 * (v_word + 32 * i);
+                f16x8 v[4];
+                decode_columns<CODES>(vr[i], v);
+                if (DP % 128 == 0 || c < DP) *reinterpret_cast<f16x8*>(&vals[buf][val_at(c + col, oct)]) = v[col];
+            }
+        };
+        auto store = [&](int buf) {
+#pragma unroll
+            for (int j = 0; j < kPieces; j++) store_piece(buf, j);
+        };
+        auto compute = [&](uint32_t t0, int buf) {
+            if (t0 >= most) {                                   // none of this wavefront's rows sees the tile
+                if constexpr (NBUF == 2) store(buf ^ 1);
+                return;
+            }
+            f32x4 s[MT][4];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const f16x8 k = *reinterpret_cast<const f16x8*>(&keys[buf][(16 * t + m) * kKeyLd + 32 * ks + 8 * g]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int qt = 0; qt < QT; qt++)
+                            s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][t] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                }
+            float4 x[4];
+            bool gone[4], any_gone = false;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                x[t] = ent[(min(t0 + 16 * t, c1 - 1) >> bs_log) - e0];
+                gone[t] = __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].x)) >> 31;
+                any_gone |= gone[t];
+            }
+            const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || any_gone;
+            float f[MT][4], ref[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                float local = -__builtin_inff();
+                if (ragged) {
+                    const int left = (int)(min(seen[mt], c1) - t0 - 4 * g);         // (both are below 2^31)
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) s[mt][t][r] = 16 * t + r < left && !gone[t] ? s[mt][t][r] : -__builtin_inff();
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    f[mt][t] = fmaxf(x[t].x * factor[mt], 0x1p-126f);               // (not 0, which masked scores would make NaN)
+                    local = fmaxf(local, f[mt][t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
+                }
+                if (__ballot(local > top[mt] + kLead)) {
+                    const float now = fmaxf(top[mt], max_over_groups(local));
+                    const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
+                    top[mt] = now;
+                    sum[mt] *= shrink;
+#pragma unroll
+                    for (int i = 0; i < DT; i++) o[mt][i] *= shrink;
+                }
+                ref[mt] = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+            }
+            // the two halves of the tile: weights of one while the other's meet the values, and the next tile's codes become
+            // 16-bit floats meanwhile (their loads were issued before the scores)
+            f16x8 p[2][MT][PT];
+            auto weigh = [&](int mt, int t) {
+                const float by = x[t].y - ref[mt];
+                float part_sum = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][t][r], f[mt][t], by));
+                    part_sum += w;
+                    const _Float16 hi = (_Float16)w;
+                    p[t / 2][mt][0][4 * (t % 2) + r] = hi;
+                    if constexpr (PT == 2) p[t / 2][mt][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
+                }
+                sum[mt] = __builtin_fmaf(part_sum, x[t].z, sum[mt]);
+            };
+            auto meet = [&](int h, int i) {
+                const f16x8 v = *reinterpret_cast<const f16x8*>(&vals[buf][val_at(16 * i + m, 4 * h + g)]);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int pt = 0; pt < PT; pt++) o[mt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[h][mt][pt], o[mt][i], 0, 0, 0);
+            };
+#pragma unroll
+            for (int j = 0; j < 2 * MT; j++) weigh(j / 2, j % 2);
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                meet(0, i);
+#pragma unroll
+                for (int j = i * 2 * MT / DT; j < (i + 1) * 2 * MT / DT; j++) weigh(j / 2, 2 + j % 2);
+            }
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                meet(1, i);
+                if constexpr (NBUF == 2) {
+#pragma unroll
+                    for (int j = i * kPieces / DT; j < (i + 1) * kPieces / DT; j++) store_piece(buf ^ 1, j);
+                }
+            }
+        };
+
+        fetch(c0);
+        store(0);
+        __syncthreads();
+        int buf = 0;
+        for (uint32_t t0 = c0; t0 < c1; t0 += kTokens) {
+            if (t0 + kTokens < c1) fetch(t0 + kTokens);
+            compute(t0, buf);
+            if constexpr (NBUF == 1) {                          // the only buffer is about to be overwritten
+                __syncthreads();
+                store(0);
+            } else {
+                buf ^= 1;
+            }
+            __syncthreads();
+        }
+    }
+
+    const float unit_o = unit_v / kPScale;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const float l = sum_over_groups(sum[mt]);
+        const uint32_t r = r0 + 16 * mt + m;
+        if (r >= n_r) continue;
+        const uint32_t i = r / group;
+        const size_t to = (size_t)(rows.first + i) * a.q_heads + kv * group + (r - i * group);
+        const float inv = l == 0.0f ? 0.0f : unit_o / l, lse = l == 0.0f ? -__builtin_inff() : top[mt] + __builtin_amdgcn_logf(l);
+        if (parts.n_splits == 1) {
+            T* out = (T*)a.out + to * dim;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+                if (16 * t < (int)dim) {
+                    const uint32_t d = 16 * t + 4 * g;
+                    if constexpr (sizeof(T) == 4) {
+                        *reinterpret_cast<float4*>(out + d) = make_float4(o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
+                    } else {
+                        u32x2 w;
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            w[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(o[mt][t][2 * j] * inv)) | ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(o[mt][t][2 * j + 1] * inv)) << 16);
+                        *reinterpret_cast<u32x2*>(out + d) = w;
+                    }
+                }
+            if (g == 0 && a.lse) a.lse[to] = lse * 0.6931471805599453f;
+        } else {
+            const size_t at = to * parts.n_splits + split;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+                if (16 * t < (int)dim)
+                    *reinterpret_cast<float4*>(parts.out + at * dim + 16 * t + 4 * g) = make_float4(o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
+            if (g == 0) parts.lse[at] = lse;
+        }
+    }
+}
+
+// The chunks' outputs of a row and head become one: weights 2^(lse - largest).  One workgroup each: dim / 4 lanes take a chunk, so that
+// 256 / (dim / 4) chunks are read at a time.
+template <class T>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials parts)
+{
+    __shared__ float red[kWaves], weight[256];
+    __shared__ __align__(16) float4 out_s[256];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, to = blockIdx.x, row = to / a.q_heads;
+    const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
+    if (b >= a.n_requests) return;
+    uint32_t n = parts.n_splits;
+    if (!a.found) {
+        const Span s = rows_of(a, b);
+        const uint32_t sees = seen_by(a, length_of(a, b), s.count, row - s.first);
+        n = min(n, (uint32_t)(((uint64_t)sees + parts.chunk - 1) / parts.chunk));
+    }
+    const float* lse = parts.lse + (size_t)to * parts.n_splits;
+    const float* x = parts.out + (size_t)to * parts.n_splits * a.dim;
+    const uint32_t lanes = a.dim / 4, per = 256 / lanes, mine = tid / lanes, d = (tid - mine * lanes) * 4;
+    float top = -__builtin_inff();
+    for (uint32_t i = tid; i < n; i += 256) top = fmaxf(top, lse[i]);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    if (lane == 0) red[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+    for (uint32_t i0 = 0; i0 < n; i0 += 256) {
+        const float w = i0 + tid < n ? __builtin_amdgcn_exp2f(lse[i0 + tid] - ref) : 0.0f;
+        l += w;
+        __syncthreads();
+        weight[tid] = w;
+        __syncthreads();
+        const uint32_t here = min(n - i0, 256u);
+        if (mine < per)
+#pragma unroll 4
+            for (uint32_t i = mine; i < here; i += per) {
+                const float4 y = *reinterpret_cast<const float4*>(x + (size_t)(i0 + i) * a.dim + d);
+                const float f = weight[i];
+                o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
+            }
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
+    __syncthreads();
+    if (lane == 0) red[tid >> 6] = l;
+    out_s[tid] = o;
+    __syncthreads();
+    l = red[0] + red[1] + red[2] + red[3];
+    if (mine == 0) {
+        for (uint32_t i = 1; i < per; i++) {
+            const float4 y = out_s[tid + i * lanes];
+            o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        T* out = (T*)a.out + (size_t)to * a.dim + d;
+        out[0] = from_float<T>(o.x * inv); out[1] = from_float<T>(o.y * inv); out[2] = from_float<T>(o.z * inv); out[3] = from_float<T>(o.w * inv);
+    }
+    if (tid == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+}  // namespace
+
+template <class T> void launch_attend(const AttendArgs& a, const Cut& cut, uint32_t codes_, float* workspace, hipStream_t stream)
+{
+    const char* who = a.found ? "cache_attend_found" : "cache_attend";
+    const Partials parts{workspace, workspace + (uint64_t)a.n_rows * a.q_heads * cut.n_splits * a.dim, cut.n_splits, cut.chunk};
+    const int64_t step = 16 / (int64_t)sizeof(T);
+    const uint32_t q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && a.q_row_stride % step == 0 && a.q_head_stride % step == 0;
+    const dim3 grid(cut.units * cut.heads, cut.n_splits);
+    auto rows = [&](auto codes, auto dp, auto mt, auto nw) {
+        if (a.found) hipLaunchKernelGGL((attend_rows_kernel<T, codes.value, dp.value, mt.value, nw.value, true>), grid, dim3(64 * nw.value), 0, stream, a, parts, cut.heads, q_vec);
+        else hipLaunchKernelGGL((attend_rows_kernel<T, codes.value, dp.value, mt.value, nw.value, false>), grid, dim3(64 * nw.value), 0, stream, a, parts, cut.heads, q_vec);
+    };
+    auto by_size = [&](auto codes, auto dp) {
+        constexpr int kTileMt = dp.value <= 128 ? 2 : 1;
+        if (cut.tiles) {
+            hipLaunchKernelGGL((attend_tile_kernel<T, codes.value, dp.value, kTileMt, dp.value <= 128 ? 2 : 1>), grid, dim3(256), 0, stream, a, parts, q_vec);
+        } else if (dp.value <= 128 && cut.mt == 2) {
+            if constexpr (dp.value <= 128) rows(codes, dp, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+        } else if (cut.waves == 1) {
+            rows(codes, dp, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+        } else if (cut.waves == 8) {
+            rows(codes, dp, std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+        } else {
+            rows(codes, dp, std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+        }
+    };
+    auto by_dim = [&](auto codes) {
+        if (a.dim <= 64) by_size(codes, std::integral_constant<int, 64>{});
+        else if (a.dim <= 128) by_size(codes, std::integral_constant<int, 128>{});
+        else if (a.dim <= 192) by_size(codes, std::integral_constant<int, 192>{});
+        else by_size(codes, std::integral_constant<int, 256>{});
+    };
+    if (codes_ == HNSW_AMD_CODES_I8) by_dim(std::integral_constant<int, HNSW_AMD_CODES_I8>{});
+    else by_dim(std::integral_constant<int, HNSW_AMD_CODES_E4M3>{});
+    check_launch(who);
+    if (cut.n_splits > 1) {
+        hipLaunchKernelGGL((attend_join_kernel<T>), dim3(a.n_rows * a.q_heads), dim3(256), 0, stream, a, parts);
+        check_launch(who);
+    }
+}
+
+}  // namespace hnsw_amd

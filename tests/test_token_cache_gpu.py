@@ -251,13 +251,18 @@ ONE = [
     ([90, 5000], 1, 2, 16, 32, I8, BF16), ([2300], 1, 1, 128, 48, E4, F16)]
 
 
+# requests in such numbers, and so short or long, that a call is cut in other ways: one wavefront each, eight, chunks of tokens
+ONE += [([(7 * i) % 251 for i in range(300)], 4, 1, 16, 64, E4, BF16), ([1000 - i for i in range(3)], 2, 1, 32, 192, I8, F16), ([1024, 1025], 1, 2, 256, 256, E4, F32),
+        ([256 - (i % 3) for i in range(520)], 2, 2, 256, 128, I8, F32), ([9000, 10, 4000], 1, 1, 32, 96, E4, BF16)]
+
+
 @pytest.mark.parametrize("lens,heads,group,block,dim,codes,dtype", ONE)
 def test_attend_one_token(lens, heads, group, block, dim, codes, dtype):
     s = Setup(lens, heads, block, dim, codes)
     q = _queries(len(lens), heads * group, dim, dtype)
     for max_len in (0, max(lens), 1, 10 ** 6):
         out, lse = s.cache.attend(q, s.d_table, s.d_lens, max_len=max_len)
-        _compare(s, q, out, lse, lambda r, h: (r, np.arange(lens[r])), dim ** -0.5)
+        _compare(s, q, out, lse, lambda r, h: (r, np.arange(lens[r])), dim ** -0.5, pick=None if len(lens) < 100 else [0, 1, 36, 40, 255, 299])
 
 
 MANY = [
@@ -300,7 +305,8 @@ FOUND = [
     # lens, kv heads, lists per kv head, group, block, dim, codes, type, ids
     ([1], 1, 1, 1, 16, 64, I8, F32, 5), ([100, 0, 9], 2, 1, 4, 16, 128, I8, BF16, 10), ([3000, 700], 2, 4, 4, 32, 128, E4, BF16, 100), ([900], 1, 2, 8, 64, 96, I8, F16, 257),
     ([5000, 1], 1, 1, 16, 128, 80, E4, F32, 1100), ([400], 1, 3, 3, 16, 256, I8, F16, 33), ([800, 60], 1, 1, 40, 32, 192, E4, BF16, 64), ([4000], 2, 1, 8, 16, 128, E4, F16, 4000),
-    ([70], 3, 1, 1, 16, 48, I8, BF16, 1)]
+    ([70], 3, 1, 1, 16, 48, I8, BF16, 1), ([i for i in range(600)], 2, 2, 4, 16, 128, E4, F16, 200), ([3 * i for i in range(300)], 4, 1, 1, 32, 256, I8, F32, 257),
+    ([2000] * 3, 1, 2, 2, 64, 192, E4, BF16, 1000)]
 
 
 @pytest.mark.parametrize("lens,heads,share,group,block,dim,codes,dtype,k", FOUND)
@@ -319,7 +325,7 @@ def test_attend_found(lens, heads, share, group, block, dim, codes, dtype, k):
     q = _queries(len(lens), heads * group, dim, dtype)
     out, lse = s.cache.attend_found(q, s.d_table, s.d_lens, _gpu(ids))
     each = heads * group // (heads * share)
-    _compare(s, q, out, lse, lambda r, h: (r, ref.visible(ids[r, h // each], lens[r])), dim ** -0.5)
+    _compare(s, q, out, lse, lambda r, h: (r, ref.visible(ids[r, h // each], lens[r])), dim ** -0.5, pick=None if len(lens) < 100 else [0, 1, 2, 150, 256, len(lens) - 1])
 
 
 def test_work_that_needs_no_splitting_and_more_than_one_table():
