@@ -54,10 +54,9 @@ static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_
         c.waves = 8;
         chunk = 1024;
     } else {
-        // one round of two workgroups a compute unit, or where that leaves more than 1024 items to each, several rounds, which even out
-        // requests of different lengths
-        chunk = total / 512;
-        if (chunk > 1024) chunk = std::max<uint64_t>(1024, total / 4096);
+        // one round of three workgroups a compute unit, but no chunk of more than 4096: a long request among short ones is not left to
+        // a few workgroups
+        chunk = std::min<uint64_t>(total / 768, 4096);
         chunk = std::max<uint64_t>((chunk + 127) / 128 * 128, 128);
     }
     c.chunk = (uint32_t)std::min<uint64_t>(chunk, 0x80000000ull);

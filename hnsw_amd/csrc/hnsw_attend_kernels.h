@@ -242,6 +242,9 @@ __device__ __forceinline__ bool table_entries(const AttendArgs& a, uint32_t b, u
     return some != 0;
 }
 
+// Wavefronts of a SIMD that the registers must leave room for: what hides the latency of the loads.
+constexpr int rows_waves(int dp, int mt) { return mt == 1 ? (dp == 64 ? 4 : dp == 128 ? 3 : 2) : (dp == 64 ? 3 : 2); }
+
 // Attention of few query rows over many tokens: for single tokens the codes are read once and that is the time.
 //
 // The workgroup takes one key head of one request (or one list), up to 16 * MT rows of queries and one chunk of the tokens; its
@@ -260,7 +263,7 @@ __device__ __forceinline__ bool table_entries(const AttendArgs& a, uint32_t b, u
 // A workgroup's start is a chain of loads that wait for one another (length, table, codes; for lists: ids, table, codes): the first
 // tile's codes are asked for as soon as the table is there, and queries and scales are made ready meanwhile.
 template <class T, int CODES, int DP, int MT, int NW, bool FOUND>
-__global__ __launch_bounds__(64 * NW) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
+__global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
 {
     constexpr int KS = DP / 32, KW = DP / 64, VW = DP / 64, VB = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
     constexpr uint32_t kThreads = 64 * NW, kTable = FOUND ? (NW == 1 ? 256 : kListTokens) : (NW == 1 ? 1024 : kScanTokens);      // items of a table
@@ -346,18 +349,15 @@ __global__ __launch_bounds__(64 * NW) void attend_rows_kernel(AttendArgs a, Part
 #pragma unroll
         for (int i = 0; i < VB; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    bool ready = false;                                         // the queries are
-    auto make_ready = [&]() {
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
-        ready = true;
-    };
+    u32x4 tk[2][KW];                                            // a tile's codes, keys and values
+    uint32_t tv[8][VW];
+    uint32_t c0 = begin, c1 = 0, n = 0, e0 = 0, safe = 0;       // the table: items c0 .. c1, n of them; its first block; a row of codes of a live token
+    uint32_t bh[kMine], at[kMine];                              // (block, head) of this thread's entries, ~0: of none, and their places
 
-    for (uint32_t c0 = begin; c0 < end; c0 += kTable) {
-        const uint32_t c1 = min(end - c0, kTable) + c0;
-        uint32_t n = c1 - c0, e0 = 0, safe = 0;                 // items in the table; a row of codes of a live token
-        uint32_t bh[kMine], at[kMine];                          // (block, head) of this thread's entries, ~0: of none, and their places
-        if (c0 != begin) __syncthreads();                       // the table's last readers are done
+    // Entries c0 .. c1 but for the scales; false where there is nothing in them.
+    auto open_table = [&]() {
+        c1 = min(end - c0, kTable) + c0;
+        n = c1 - c0;
         if constexpr (FOUND) {
             // listed tokens that the row sees and that exist, moved together (in order): entries, then 32 or less that weigh nothing
             const int32_t* ids = a.ids + ((size_t)first * heads + head) * a.n_ids;
@@ -383,11 +383,12 @@ __global__ __launch_bounds__(64 * NW) void attend_rows_kernel(AttendArgs a, Part
                 }
                 if (bh[e] != ~0u) ent_row[at[e]] = (bh[e] << bs_log) + (id[e] & (bs - 1));
             }
-            n = kept;
-            if (n == 0) continue;                               // (the same in all threads)
+            n = __builtin_amdgcn_readfirstlane(kept);
+            if (n == 0) return false;
             __syncthreads();
             if (tid < kTile) { ent_row[n + tid] = ent_row[n - 1]; ent_k[n + tid] = 0.0f; ent_v[n + tid] = 0.0f; }
             __syncthreads();
+            return true;
         } else {
             e0 = c0 >> bs_log;
             const bool mine = tid <= ((c1 - 1) >> bs_log) - e0;
@@ -397,191 +398,228 @@ __global__ __launch_bounds__(64 * NW) void attend_rows_kernel(AttendArgs a, Part
             const unsigned long long fine = __ballot(bh[0] != ~0u);
             if (lane == 0) red_n[wave] = fine ? (__builtin_amdgcn_readlane(bh[0], __builtin_ctzll(fine)) << bs_log) + 1 : 0;
             __syncthreads();
+            safe = 0;
 #pragma unroll
             for (int w = 0; w < NW; w++) safe = safe ? safe : red_n[w];
             safe = __builtin_amdgcn_readfirstlane(safe);
-            if (!safe--) continue;                              // none of these blocks exists
+            return safe-- != 0;
         }
-
-        // a tile's codes: where they are, and the loads
-        struct Tile { u32x4 k[2][KW]; uint32_t v[8][VW]; };
-        const uint32_t k_col = min(16 * g, dim - 16), v_col = VB * m;
-        auto fetch = [&](uint32_t j, Tile& t) {
-            const uint32_t i0 = 32 * j;
+    };
+    // Where tile j's codes are: of all tokens, the two runs of 16 lie in a block each (tokens behind the last one are the last one).
+    struct Where { uint64_t at[2]; uint32_t limit[2]; };
+    auto locate = [&](uint32_t j) {
+        Where w{};
+        if constexpr (!FOUND) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                uint32_t row_k, row_v[4];
-                const uint8_t *kb = a.k_codes, *vb = a.v_codes;
-                if constexpr (FOUND) {
-                    row_k = ent_row[i0 + 16 * h + m];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) row_v[r] = ent_row[i0 + 16 * h + 4 * g + r];
-                } else {
-                    const uint32_t last = c1 - 1, start = min(c0 + i0 + 16 * h, last);
-                    uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
-                    if (base == ~0u) base = safe;               // (stale codes can be NaN, which a weight of 0 would not remove)
-                    const uint64_t at = (uint64_t)(base + (start & (bs - 1))) * dim;
-                    kb += at;
-                    vb += at;
-                    row_k = min(m, last - start);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) row_v[r] = min(4 * g + r, last - start);
-                }
-                auto offset = [&](uint32_t row) { if constexpr (FOUND) return (uint64_t)row * dim; else return row * dim; };
-#pragma unroll
-                for (int i = 0; i < KW; i++)
-                    t.k[h][i] = *reinterpret_cast<const u32x4*>(kb + offset(row_k) + (64 * i + 16 * g < dim ? 64 * i + 16 * g : k_col));
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint8_t* p = vb + offset(row_v[r]);
-                    if constexpr (VW == 2) {
-                        const u32x2 w = *reinterpret_cast<const u32x2*>(p + (v_col + 8 <= dim ? v_col : 0));
-                        t.v[4 * h + r][0] = w[0]; t.v[4 * h + r][1] = w[1];
-                    } else if constexpr (VW == 4) {
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(p + (v_col + 16 <= dim ? v_col : 0));
-#pragma unroll
-                        for (int i = 0; i < 4; i++) t.v[4 * h + r][i] = w[i];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < VW; i++) t.v[4 * h + r][i] = *reinterpret_cast<const uint32_t*>(p + (v_col + 4 * i + 4 <= dim ? v_col + 4 * i : 0));
-                    }
-                }
+                const uint32_t start = min(c0 + 32 * j + 16 * h, c1 - 1);
+                uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
+                if (base == ~0u) base = safe;                   // (stale codes can be NaN, which a weight of 0 would not remove)
+                w.at[h] = (uint64_t)(base + (start & (bs - 1))) * dim;
+                w.limit[h] = min(c1 - 1 - start, 15u);
             }
-        };
-        const uint32_t tiles = (n + kTile - 1) / kTile;
-        Tile t[2];
-        if (wave < tiles) fetch(wave, t[0]);
-        if (!ready) make_ready();
-        // the entries' scales, and the largest value scale
-        float largest = 0.0f;
+        }
+        return w;
+    };
+    auto fetch_keys = [&](uint32_t j, const Where& w) {
 #pragma unroll
-        for (uint32_t e = 0; e < kMine; e++) {
+        for (int h = 0; h < 2; h++) {
+            const uint8_t* p = a.k_codes;
+            uint32_t off = 0;
             if constexpr (FOUND) {
-                if (bh[e] != ~0u) {
-                    const float sv = a.v_scale[bh[e]];
-                    ent_k[at[e]] = a.k_scale[bh[e]];
-                    ent_v[at[e]] = sv;
-                    largest = fmaxf(largest, sv);
+                p += (uint64_t)ent_row[32 * j + 16 * h + m] * dim;
+            } else {
+                p += w.at[h];
+                off = (w.limit[h] == 15 ? m : min(m, w.limit[h])) * dim;
+            }
+#pragma unroll
+            for (int i = 0; i < KW; i++) {
+                const uint32_t c = 64 * i + 16 * g;
+                tk[h][i] = *reinterpret_cast<const u32x4*>(p + off + (c < dim ? c : 0));
+            }
+        }
+    };
+    auto fetch_values = [&](uint32_t j, const Where& w) {
+        const uint32_t c = VB * m;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint8_t* p = a.v_codes;
+                uint32_t off = 0;
+                if constexpr (FOUND) {
+                    p += (uint64_t)ent_row[32 * j + 16 * h + 4 * g + r] * dim;
+                } else if (w.limit[h] == 15) {
+                    p += w.at[h] + (uint64_t)r * dim;
+                    off = 4 * g * dim;
+                } else {
+                    p += w.at[h];
+                    off = min(4 * g + r, w.limit[h]) * dim;
                 }
-            } else if (tid <= ((c1 - 1) >> bs_log) - e0) {
-                const float sv = bh[0] != ~0u ? a.v_scale[bh[0]] : 0.0f;
-                ent_k[tid] = bh[0] != ~0u ? a.k_scale[bh[0]] : -1.0f;
-                ent_v[tid] = sv;
-                largest = sv;
+                if constexpr (VW == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(p + off + (c < dim ? c : 0));
+                    tv[4 * h + r][0] = x[0]; tv[4 * h + r][1] = x[1];
+                } else if constexpr (VW == 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(p + off + (c < dim ? c : 0));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) tv[4 * h + r][i] = x[i];
+                } else {                                        // (a lane's bytes can end with the row in their middle)
+#pragma unroll
+                    for (int i = 0; i < VW; i++) tv[4 * h + r][i] = *reinterpret_cast<const uint32_t*>(p + off + (c + 4 * i < dim ? c + 4 * i : 0));
+                }
             }
-        }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
-        if (lane == 0) red[wave] = largest;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; w++) largest = fmaxf(largest, red[w]);
-        const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
-        if (largest > 0.0f) {
-            if (unit_v > 0.0f && unit_v != largest) {           // outputs so far are in units of the last table's largest scale
-                const float change = unit_v / largest;
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int i = 0; i < VB; i++) o[mt][i] *= change;
-            }
-            unit_v = largest;
-        }
+    };
 
-        auto take = [&](uint32_t j, Tile& t) {
-            const uint32_t i0 = 32 * j;
-            f32x4 s[MT][2];
+    bool some = begin < end && open_table();                    // (the same in all threads)
+    if (some && 32 * wave < n) {
+        const Where w = locate(wave);
+        fetch_keys(wave, w);
+        fetch_values(wave, w);
+    }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
+    while (c0 < end) {
+        if (some) {
+            // the entries' scales, and the largest value scale
+            float largest = 0.0f;
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (uint32_t e = 0; e < kMine; e++) {
+                if constexpr (FOUND) {
+                    if (bh[e] != ~0u) {
+                        const float sv = a.v_scale[bh[e]];
+                        ent_k[at[e]] = a.k_scale[bh[e]];
+                        ent_v[at[e]] = sv;
+                        largest = fmaxf(largest, sv);
+                    }
+                } else if (tid <= ((c1 - 1) >> bs_log) - e0) {
+                    const float sv = bh[0] != ~0u ? a.v_scale[bh[0]] : 0.0f;
+                    ent_k[tid] = bh[0] != ~0u ? a.k_scale[bh[0]] : -1.0f;
+                    ent_v[tid] = sv;
+                    largest = sv;
+                }
+            }
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const f16x8 k = decode8<CODES>(t.k[h][ks / 2][2 * (ks % 2)], t.k[h][ks / 2][2 * (ks % 2) + 1]);
+            for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
+            if (lane == 0) red[wave] = largest;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; w++) largest = fmaxf(largest, red[w]);
+            const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
+            if (largest > 0.0f) {
+                if (unit_v > 0.0f && unit_v != largest) {       // outputs so far are in units of the last table's largest scale
+                    const float change = unit_v / largest;
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                        for (int qt = 0; qt < QT; qt++) s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], s[mt][h], 0, 0, 0);
+                        for (int i = 0; i < VB; i++) o[mt][i] *= change;
                 }
-            float fk[2][4], pw[2][4];                           // the scales of this lane's tokens 4g + r of both halves
-            bool gone[2] = {false, false}, ragged;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (FOUND) {
-                    const float4 x = *reinterpret_cast<const float4*>(&ent_k[i0 + 16 * h + 4 * g]), y = *reinterpret_cast<const float4*>(&ent_v[i0 + 16 * h + 4 * g]);
-                    fk[h][0] = x.x; fk[h][1] = x.y; fk[h][2] = x.z; fk[h][3] = x.w;
-                    pw[h][0] = y.x * per_v; pw[h][1] = y.y * per_v; pw[h][2] = y.z * per_v; pw[h][3] = y.w * per_v;
-                } else {
-                    const uint32_t e = (min(c0 + i0 + 16 * h, c1 - 1) >> bs_log) - e0;
-                    const float x = ent_k[e], y = ent_v[e] * per_v;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) { fk[h][r] = x; pw[h][r] = y; }
-                    gone[h] = __builtin_amdgcn_readfirstlane(__float_as_uint(x)) >> 31;
-                }
+                unit_v = largest;
             }
-            if constexpr (FOUND) ragged = i0 + 32 > n;
-            else ragged = c0 + i0 + 32 > least || c0 + i0 + 32 > c1 || gone[0] || gone[1];
-            f16x8 p[MT][PT];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float x[2][4], local = -__builtin_inff();
+
+            for (uint32_t j = wave; 32 * j < n; j += NW) {
+                const uint32_t i0 = 32 * j;
+                const bool more = i0 + 32 * NW < n;
+                f32x4 s[MT][2];
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) x[h][r] = s[mt][h][r] * (fk[h][r] * factor[mt]);
-                if (ragged) {
-                    const int left = (int)((FOUND ? n : min(seen[mt], c1) - c0) - i0 - 4 * g);
+                    for (int ks = 0; ks < KS; ks++) {
+                        const f16x8 k = decode8<CODES>(tk[h][ks / 2][2 * (ks % 2)], tk[h][ks / 2][2 * (ks % 2) + 1]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                            for (int qt = 0; qt < QT; qt++)
+                                s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][h] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    }
+                // the keys' registers are free: the next tile's keys are under way while this one's weights meet its values
+                Where next{};
+                if (more) {
+                    next = locate(j + NW);
+                    fetch_keys(j + NW, next);
+                }
+                float fk[2][4], pw[2][4];                       // the scales of this lane's tokens 4g + r of both halves
+                bool gone[2] = {false, false}, ragged;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (FOUND) {
+                        const float4 x = *reinterpret_cast<const float4*>(&ent_k[i0 + 16 * h + 4 * g]), y = *reinterpret_cast<const float4*>(&ent_v[i0 + 16 * h + 4 * g]);
+                        fk[h][0] = x.x; fk[h][1] = x.y; fk[h][2] = x.z; fk[h][3] = x.w;
+                        pw[h][0] = y.x * per_v; pw[h][1] = y.y * per_v; pw[h][2] = y.z * per_v; pw[h][3] = y.w * per_v;
+                    } else {
+                        const uint32_t e = (min(c0 + i0 + 16 * h, c1 - 1) >> bs_log) - e0;
+                        const float x = ent_k[e], y = ent_v[e] * per_v;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) { fk[h][r] = x; pw[h][r] = y; }
+                        gone[h] = __builtin_amdgcn_readfirstlane(__float_as_uint(x)) >> 31;
+                    }
+                }
+                if constexpr (FOUND) ragged = i0 + 32 > n;
+                else ragged = c0 + i0 + 32 > least || c0 + i0 + 32 > c1 || gone[0] || gone[1];
+                f16x8 p[MT][PT];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    float x[2][4], local = -__builtin_inff();
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) x[h][r] = 16 * h + r < left && !gone[h] ? x[h][r] : -__builtin_inff();
-                }
+                        for (int r = 0; r < 4; r++) x[h][r] = s[mt][h][r] * (fk[h][r] * factor[mt]);
+                    if (ragged) {
+                        const int left = (int)((FOUND ? n : min(seen[mt], c1) - c0) - i0 - 4 * g);
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                        for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) local = fmaxf(local, x[h][r]);
-                if (__ballot(local > top[mt] + kLead)) {        // rare after the first tile
-                    const float now = fmaxf(top[mt], max_over_groups(local));
-                    const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
-                    top[mt] = now;
-                    sum[mt] *= shrink;
-#pragma unroll
-                    for (int i = 0; i < VB; i++) o[mt][i] *= shrink;
-                }
-                const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float y = __builtin_amdgcn_exp2f(x[h][r] - ref);
-                        sum[mt] += y;
-                        const float w = y * pw[h][r];
-                        const _Float16 hi = (_Float16)w;
-                        p[mt][0][4 * h + r] = hi;
-                        if constexpr (PT == 2) p[mt][1][4 * h + r] = (_Float16)(w - (float)hi);
+                            for (int r = 0; r < 4; r++) x[h][r] = 16 * h + r < left && !gone[h] ? x[h][r] : -__builtin_inff();
                     }
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) local = fmaxf(local, x[h][r]);
+                    if (__ballot(local > top[mt] + kLead)) {    // rare after the first tile
+                        const float now = fmaxf(top[mt], max_over_groups(local));
+                        const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
+                        top[mt] = now;
+                        sum[mt] *= shrink;
+#pragma unroll
+                        for (int i = 0; i < VB; i++) o[mt][i] *= shrink;
+                    }
+                    const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const float y = __builtin_amdgcn_exp2f(x[h][r] - ref);
+                            sum[mt] += y;
+                            const float w = y * pw[h][r];
+                            const _Float16 hi = (_Float16)w;
+                            p[mt][0][4 * h + r] = hi;
+                            if constexpr (PT == 2) p[mt][1][4 * h + r] = (_Float16)(w - (float)hi);
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < VW; i++) {
+                    uint32_t w[8];
+                    f16x8 v[4];
+#pragma unroll
+                    for (int r = 0; r < 8; r++) w[r] = tv[r][i];
+                    decode_columns<CODES>(w, v);
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                            for (int pt = 0; pt < PT; pt++) o[mt][4 * i + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p[mt][pt], o[mt][4 * i + c], 0, 0, 0);
+                }
+                if (more) fetch_values(j + NW, next);
             }
-#pragma unroll
-            for (int i = 0; i < VW; i++) {
-                uint32_t w[8];
-                f16x8 v[4];
-#pragma unroll
-                for (int r = 0; r < 8; r++) w[r] = t.v[r][i];
-                decode_columns<CODES>(w, v);
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                        for (int pt = 0; pt < PT; pt++) o[mt][4 * i + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p[mt][pt], o[mt][4 * i + c], 0, 0, 0);
-            }
-        };
-        for (uint32_t j = wave; j < tiles; j += 2 * NW) {
-            if (j + NW < tiles) fetch(j + NW, t[1]);
-            take(j, t[0]);
-            if (j + NW >= tiles) break;
-            if (j + 2 * NW < tiles) fetch(j + 2 * NW, t[0]);
-            take(j + NW, t[1]);
+        }
+        c0 += kTable;
+        if (c0 >= end) break;
+        __syncthreads();                                        // the table's last readers are done
+        some = open_table();
+        if (some && 32 * wave < n) {
+            const Where w = locate(wave);
+            fetch_keys(wave, w);
+            fetch_values(wave, w);
         }
     }
 

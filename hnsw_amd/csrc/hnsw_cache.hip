@@ -54,7 +54,7 @@ __device__ __forceinline__ uint32_t last_not_after(const uint32_t* pre, uint32_t
 __global__ void plan_kernel(PlanArgs a)
 {
     extern __shared__ uint32_t lds[];
-    const uint32_t n = a.n_requests, bs = a.block_tokens, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const uint32_t n = a.n_requests, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
     uint32_t* len_s = lds;            // tokens held
     uint32_t* cu_s = len_s + n;       // new tokens before this request
     uint32_t* need_s = cu_s + n;      // blocks taken before this request
@@ -63,6 +63,7 @@ __global__ void plan_kernel(PlanArgs a)
     __shared__ unsigned long long total_grow, total_back;
     __shared__ uint32_t trouble;
     if (tid == 0) { total_grow = 0; total_back = 0; trouble = 0; }
+    const int64_t head = a.state[0], tail = a.state[1], avail = tail - head;
     __syncthreads();
 
     const uint32_t per = (n + blockDim.x - 1) / blockDim.x, lo = min(tid * per, n), hi = min(lo + per, n);
@@ -73,8 +74,8 @@ __global__ void plan_kernel(PlanArgs a)
         if (l < 0 || r < -1) bad |= HNSW_AMD_PLAN_BAD_LENGTH;
         len = (uint32_t)max(l, 0);
         g = (uint32_t)max(r, 0);
-        const uint32_t have = (len + bs - 1) / bs;                                  // (lengths are below 2^31)
-        const uint32_t want = (uint32_t)(((unsigned long long)len + g + bs - 1) / bs);
+        const uint32_t have = (len + bs - 1) >> bs_log;                                  // (lengths are below 2^31)
+        const uint32_t want = (uint32_t)(((unsigned long long)len + g + bs - 1) >> bs_log);
         if (want > a.width) bad |= HNSW_AMD_PLAN_TABLE_FULL;
         need = want - have;
         back = r == -1 ? have : 0;
@@ -97,7 +98,6 @@ __global__ void plan_kernel(PlanArgs a)
         grown += wsum[0][w]; taken += wsum[1][w]; given += wsum[2][w];
     }
     for (uint32_t b = lo; b < hi; b++) { cu_s[b] += g0; need_s[b] += n0; back_s[b] += b0; }
-    const int64_t head = a.state[0], tail = a.state[1], avail = tail - head;
     uint32_t status = trouble;
     if (head < 0 || avail < 0 || avail > (int64_t)a.n_blocks) status |= HNSW_AMD_PLAN_BAD_LENGTH;
     if (total_grow > a.n_slots) status |= HNSW_AMD_PLAN_SLOTS_FULL;
@@ -105,22 +105,33 @@ __global__ void plan_kernel(PlanArgs a)
     if (!status && (int64_t)taken > avail) status |= HNSW_AMD_PLAN_NO_BLOCKS;
     if (!status && (int64_t)total_back > (int64_t)a.n_blocks - avail) status |= HNSW_AMD_PLAN_BAD_LENGTH;
     if (status) { grown = 0; taken = 0; given = 0; }                                // all or nothing
-    const uint32_t head_at = status ? 0u : (uint32_t)(head % a.n_blocks), tail_at = status ? 0u : (uint32_t)(tail % a.n_blocks);
+    auto wrap = [&](int64_t x) { return x >> 32 ? (uint32_t)((uint64_t)x % a.n_blocks) : (uint32_t)x % a.n_blocks; };      // (64-bit division is long)
+    const uint32_t head_at = status ? 0u : wrap(head), tail_at = status ? 0u : wrap(tail);
     __syncthreads();
 
     auto ring_at = [&](uint32_t from, uint32_t i) { const unsigned long long p = (unsigned long long)from + i; return (uint32_t)(p >= a.n_blocks ? p - a.n_blocks : p); };
     const uint32_t stride = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + tid;
-    for (uint32_t t = me; t < a.n_slots; t += stride) {
-        int64_t slot = -1;
-        if (t < grown) {
-            const uint32_t b = last_not_after(cu_s, n, t), pos = len_s[b] + (t - cu_s[b]), j = pos / bs, have = (len_s[b] + bs - 1) / bs;
-            const int32_t blk = j < have ? a.table[(size_t)b * a.width + j] : a.ring[ring_at(head_at, need_s[b] + j - have)];
-            if ((uint32_t)blk < a.n_blocks) slot = (int64_t)blk * bs + pos % bs;
+    // four slots in a row: one search for the request, one block looked up for most of them
+    for (uint32_t t0 = 4 * me; t0 < a.n_slots; t0 += 4 * stride) {
+        uint32_t b = t0 < grown ? last_not_after(cu_s, n, t0) : n, block = ~0u, of = ~0u;        // (block `block` of request `of` is number blk)
+        int32_t blk = -1;
+        for (uint32_t t = t0; t < t0 + 4 && t < a.n_slots; t++) {
+            int64_t slot = -1;
+            if (t < grown) {
+                while (b + 1 < n && cu_s[b + 1] <= t) b++;
+                const uint32_t pos = len_s[b] + (t - cu_s[b]), j = pos >> bs_log, have = (len_s[b] + bs - 1) >> bs_log;
+                if (j != block || b != of) {
+                    blk = j < have ? a.table[(size_t)b * a.width + j] : a.ring[ring_at(head_at, need_s[b] + j - have)];
+                    block = j;
+                    of = b;
+                }
+                if ((uint32_t)blk < a.n_blocks) slot = ((int64_t)blk << bs_log) + (pos & (bs - 1));
+            }
+            a.slots[t] = slot;
         }
-        a.slots[t] = slot;
     }
     for (uint32_t i = me; i < taken; i += stride) {
-        const uint32_t b = last_not_after(need_s, n, i), have = (len_s[b] + bs - 1) / bs;
+        const uint32_t b = last_not_after(need_s, n, i), have = (len_s[b] + bs - 1) >> bs_log;
         a.table[(size_t)b * a.width + have + (i - need_s[b])] = a.ring[ring_at(head_at, i)];
     }
     for (uint32_t i = me; i < given; i += stride) {
@@ -158,102 +169,133 @@ __device__ __forceinline__ int scale_exponent(float peak, float most)
     return e;
 }
 
-// One wavefront per (run of rows that lie next to each other in one block, head, keys or values).  First the rows' largest
-// value, which gives the block's scale; where that raises the scale of a block that held earlier tokens, their codes move to
-// it; then the rows' codes.  Latency bound for single tokens, memory bound for prompts (rows are read from memory once and
-// a second time from the L2).
+// WPR wavefronts per (run of rows that lie next to each other in one block, head, keys or values).  First the rows' largest value, which
+// gives the block's scale; where that raises the scale of a block that held earlier tokens, their codes move to it; then the rows'
+// codes.  The first rows stay in registers between the two.  Single tokens (WPR = 1, one row a wavefront) are latency: the row is
+// asked for together with the slots, then the block's scale.  Prompts (WPR = 4, a block's worth of rows a workgroup) are memory.
 // A power of two as scale makes x / scale exact, so a code is ONE rounding of x, and moving codes to a larger scale one more.
-template <class T, int CODES, bool VEC>
+template <class T, int CODES, bool VEC, int WPR>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
 {
-    const uint32_t lane = threadIdx.x & 63;
-    const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int kKeep = WPR == 1 ? 1 : 4;                     // passes over the rows whose values are kept
+    const uint32_t lane = threadIdx.x & 63, sub = WPR == 1 ? 0 : threadIdx.x >> 6;
+    const uint64_t unit = WPR == 1 ? (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     const uint32_t part = (uint32_t)(unit % 2), head = (uint32_t)(unit / 2 % a.n_heads);
     const uint64_t t0 = unit / 2 / a.n_heads * a.span;
     if (t0 >= a.n_rows) return;
-    const uint32_t bs = a.block_tokens, dim = a.dim, lanes_per_row = dim / 8, rows_per_pass = 64 / lanes_per_row;
-    const uint32_t my_row = lane / lanes_per_row, my_col = (lane - my_row * lanes_per_row) * 8;
-    const bool active = my_row < rows_per_pass;
-    const int64_t n_slots = (int64_t)a.n_blocks * bs;
+    __shared__ float peaks[4];
+    const uint32_t bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs), dim = a.dim, lanes_per_row = dim / 8, rows_per_wave = 64 / lanes_per_row;
+    const uint32_t wave_row = lane / lanes_per_row, my_row = sub * rows_per_wave + wave_row, my_col = (lane - wave_row * lanes_per_row) * 8;
+    const uint32_t step = rows_per_wave * WPR;
+    const bool active = wave_row < rows_per_wave;
+    const int64_t n_slots = (int64_t)a.n_blocks << bs_log;
     const T* rows = (const T*)a.rows[part];
     const int64_t row_stride = a.row_stride[part], col = a.head_stride[part] * head + my_col;
 
+    float kept[kKeep][8];
+    auto load = [&](uint32_t row0, uint32_t r, float (&x)[8]) { load8<T, VEC>(rows + (int64_t)(row0 + r) * row_stride + col, x); };
+    if (WPR == 1 && active && t0 + my_row < a.n_rows) load((uint32_t)t0, my_row, kept[0]);
+
     const uint32_t end = (uint32_t)(t0 + a.span < a.n_rows ? t0 + a.span : a.n_rows);
-    unsigned long long firsts = 0;                 // of the 64 rows from `base` on: those that begin a run
-    for (uint32_t t = (uint32_t)t0, base = t; ; ) {
-        if (!firsts) {
-            if (t >= end) break;
-            base = t;
-            t += 64;
-            bool first = false;
-            if (base + lane < end) {
-                const int64_t s = a.slots[base + lane];
-                first = s >= 0 && s < n_slots && (base + lane == 0 || s % bs == 0 || a.slots[base + lane - 1] != s - 1);
-            }
-            firsts = __ballot(first);
-            continue;
-        }
-        const uint32_t row0 = base + (uint32_t)__builtin_ctzll(firsts);
-        firsts &= firsts - 1;
-        const int64_t slot = a.slots[row0];
-        const uint32_t block = (uint32_t)(slot / bs), off = (uint32_t)(slot % bs);
-        uint32_t n = 1;
-        for (;;) {                                                                 // the run's length
-            const uint32_t i = n + lane;
-            const bool more = off + i < bs && (uint64_t)row0 + i < a.n_rows && a.slots[row0 + i] == slot + i;
-            const unsigned long long m = __ballot(more);
-            if (m != ~0ull) { n += (uint32_t)__builtin_ctzll(~m); break; }
-            n += 64;
-        }
-        float peak = 0.0f;
-        if (active)
-            for (uint32_t r = my_row; r < n; r += rows_per_pass) {
-                float x[8];
-                load8<T, VEC>(rows + (int64_t)(row0 + r) * row_stride + col, x);
+    for (uint32_t base = (uint32_t)t0; base < end; base += 62) {
+        // lanes 1 .. 62 have the slots of rows base .. base + 61, the others those before and behind
+        const int64_t at = (int64_t)base - 1 + lane;
+        const int64_t slot_l = at >= 0 && at < (int64_t)a.n_rows ? a.slots[at] : -1;
+        const bool valid = slot_l >= 0 && slot_l < n_slots;
+        const int64_t prev_l = __shfl_up(slot_l, 1);
+        const bool follows = valid && (slot_l & (bs - 1)) != 0 && prev_l == slot_l - 1 && lane > 0;      // the row before is of the same run
+        const unsigned long long follow = __ballot(follows);
+        unsigned long long firsts = __ballot(valid && !follows) & ~(1ull << 63) & ~1ull;
+        if (end - base < 62) firsts &= (2ull << (end - base)) - 1;
+        while (firsts) {
+            const int l = __builtin_ctzll(firsts);
+            firsts &= firsts - 1;
+            const uint32_t row0 = base + l - 1;
+            const int64_t slot = ((int64_t)__builtin_amdgcn_readlane((int)(slot_l >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)slot_l, l);
+            const uint32_t block = (uint32_t)(slot >> bs_log), off = (uint32_t)(slot & (bs - 1));
+            float* scale = a.scale[part] + (size_t)block * a.n_heads + head;
+            uint8_t* codes = a.codes[part] + ((size_t)block * a.n_heads + head) * bs * dim;
+            const float before = *scale;
+            uint32_t n = 1 + (l < 63 ? (uint32_t)__builtin_ctzll(~(follow >> (l + 1))) : 0);
+            if (l + n == 64)                                    // the run goes on behind what the wavefront has in view
+                for (;;) {
+                    const uint32_t i = n + lane;
+                    const bool more = off + i < bs && (uint64_t)row0 + i < a.n_rows && a.slots[row0 + i] == slot + i;
+                    const unsigned long long more_l = __ballot(more);
+                    if (more_l != ~0ull) { n += (uint32_t)__builtin_ctzll(~more_l); break; }
+                    n += 64;
+                }
+            float peak = 0.0f;
+            auto look = [&](const float (&x)[8]) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float y = fabsf(x[j]);
                     peak = y < __builtin_inff() ? fmaxf(peak, y) : peak;            // (NaN and infinities do not set the scale)
                 }
+            };
+            if (active) {
+                if (WPR > 1)
+#pragma unroll
+                    for (int i = 0; i < kKeep; i++)
+                        if (my_row + i * step < n) load(row0, my_row + i * step, kept[i]);
+#pragma unroll
+                for (int i = 0; i < kKeep; i++)
+                    if (my_row + i * step < n) look(kept[i]);
+                for (uint32_t r = my_row + kKeep * step; r < n; r += step) {
+                    float x[8];
+                    load(row0, r, x);
+                    look(x);
+                }
             }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
-        int e = scale_exponent(peak, kCodeMax<CODES>);
-        float* scale = a.scale[part] + (size_t)block * a.n_heads + head;
-        uint8_t* codes = a.codes[part] + ((size_t)block * a.n_heads + head) * bs * dim;
-        const float before = *scale;
-        const bool held = off > 0 && before > 0.0f && before < __builtin_inff();    // the block holds earlier tokens
-        if (held) {
-            int eb = (int)((__float_as_uint(before) >> 23) & 255u) - 127;
-            if (eb < -100) eb = -100;
-            else if (__float_as_uint(before) & 0x7fffffu) eb++;                     // (a scale from elsewhere: the next power of two)
-            e = max(e, min(eb, 121));
-        }
-        const float now = ldexpf(1.0f, e);
-        if (held && now != before) {
-            const float ratio = before / now;
-            for (uint32_t i = lane; i < bs * dim / 4; i += 64) {
-                const uint32_t o = i * 4 / dim;
-                if (o >= off && o < off + n) continue;                              // about to be written
-                float x[4];
-                uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
-                decode4<CODES>(*w, x);
-#pragma unroll
-                for (int j = 0; j < 4; j++) x[j] *= ratio;
-                *w = encode4<CODES>(x);
+            for (int o = 32; o >= 1; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
+            if constexpr (WPR > 1) {
+                if (lane == 0) peaks[sub] = peak;
+                __syncthreads();
+                peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
             }
-        }
-        const float inv = ldexpf(1.0f, -e);
-        if (active)
-            for (uint32_t r = my_row; r < n; r += rows_per_pass) {
-                float x[8];
-                load8<T, VEC>(rows + (int64_t)(row0 + r) * row_stride + col, x);
+            int e = scale_exponent(peak, kCodeMax<CODES>);
+            const bool held = off > 0 && before > 0.0f && before < __builtin_inff();        // the block holds earlier tokens
+            if (held) {
+                int eb = (int)((__float_as_uint(before) >> 23) & 255u) - 127;
+                if (eb < -100) eb = -100;
+                else if (__float_as_uint(before) & 0x7fffffu) eb++;                 // (a scale from elsewhere: the next power of two)
+                e = max(e, min(eb, 121));
+            }
+            const float now = ldexpf(1.0f, e);
+            if (held && now != before) {
+                const float ratio = before / now;
+                for (uint32_t i = sub * 64 + lane; i < bs * dim / 4; i += 64 * WPR) {
+                    const uint32_t o = i * 4 / dim;
+                    if (o >= off && o < off + n) continue;                          // about to be written
+                    float x[4];
+                    uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
+                    decode4<CODES>(*w, x);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[j] *= ratio;
+                    *w = encode4<CODES>(x);
+                }
+            }
+            const float inv = ldexpf(1.0f, -e);
+            auto write = [&](uint32_t r, const float (&x)[8]) {
                 float lo[4], hi[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) { lo[j] = x[j] * inv; hi[j] = x[j + 4] * inv; }
                 *reinterpret_cast<u32x2*>(codes + (size_t)(off + r) * dim + my_col) = u32x2{encode4<CODES>(lo), encode4<CODES>(hi)};
+            };
+            if (active) {
+#pragma unroll
+                for (int i = 0; i < kKeep; i++)
+                    if (my_row + i * step < n) write(my_row + i * step, kept[i]);
+                for (uint32_t r = my_row + kKeep * step; r < n; r += step) {
+                    float x[8];
+                    load(row0, r, x);
+                    write(r, x);
+                }
             }
-        if (lane == 0) *scale = now;
+            if constexpr (WPR > 1) __syncthreads();             // (all have read the old scale and the peaks)
+            if (lane == 0 && sub == 0) *scale = now;
+        }
     }
 }
 
@@ -331,10 +373,11 @@ void cache_plan(const int32_t* lens, const int32_t* grow, uint32_t n_requests, i
     if (lens == lens_out || state == state_out) throw std::invalid_argument("cache_plan: the new lengths and ring state need buffers of their own");
     const OnDevice on(device);
     const PlanArgs a{lens, grow, table, ring, state, slots, cu_new, lens_out, status, state_out, n_requests, width, n_blocks, block_tokens, n_slots};
-    const uint32_t items = n_slots > n_requests ? n_slots : n_requests;
+    // Few requests and slots: one small workgroup.  Else enough workgroups for a pass of four slots (one request) a thread, 512 at most.
+    const uint32_t items = (n_slots + 3) / 4 > n_requests ? (n_slots + 3) / 4 : n_requests;
     const uint32_t threads = items <= 256 ? 256 : 1024;
-    uint32_t groups = (items + 4095) / 4096;
-    if (groups > 256) groups = 256;
+    uint32_t groups = (items + threads - 1) / threads;
+    if (groups > 512) groups = 512;
     const size_t lds = (size_t)n_requests * 16;
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -354,17 +397,25 @@ void cache_append(const hnsw_amd_token_cache* c, const void* k, const void* v, u
     const OnDevice on(device);
     AppendArgs a{{(uint8_t*)c->k_codes, (uint8_t*)c->v_codes}, {c->k_scale, c->v_scale}, {k, v}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride},
                  slots, n_rows, c->n_blocks, c->n_heads, c->block_tokens, c->dim, 1};
-    // Few rows: a wavefront looks at one row each, so that single tokens of many requests run side by side.  Many rows (a
-    // prompt): it looks at a block's worth, most of which are one run.
-    a.span = (uint64_t)n_rows * c->n_heads <= 16384 ? 1 : c->block_tokens;
-    const uint64_t units = (uint64_t)((n_rows + a.span - 1) / a.span) * c->n_heads * 2, groups = (units + 3) / 4;
+    // Few rows: a wavefront looks at one row each, so that single tokens of many requests run side by side.  Many rows (a prompt): a
+    // workgroup looks at a block's worth, most of which are one run.
+    const bool many = (uint64_t)n_rows * c->n_heads > 16384;
+    if (many) a.span = c->block_tokens;
+    const uint64_t units = (uint64_t)((n_rows + a.span - 1) / a.span) * c->n_heads * 2, groups = many ? units : (units + 3) / 4;
     if (groups >= 1ull << 24) throw std::invalid_argument("cache_append: too many rows and heads for one call");
     by_types(row_type, c->codes, [&](auto t, auto codes) {
         using T = decltype(t);
         const int64_t step = 16 / (int64_t)sizeof(T);
         const bool vec = aligned16(k) && aligned16(v) && k_row_stride % step == 0 && k_head_stride % step == 0 && v_row_stride % step == 0 && v_head_stride % step == 0;
-        if (vec) hipLaunchKernelGGL((append_kernel<T, codes.value, true>), dim3((uint32_t)groups), dim3(256), 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL((append_kernel<T, codes.value, false>), dim3((uint32_t)groups), dim3(256), 0, (hipStream_t)stream, a);
+        auto go = [&](auto v, auto wpr) {
+            hipLaunchKernelGGL((append_kernel<T, codes.value, v.value, wpr.value>), dim3((uint32_t)groups), dim3(256), 0, (hipStream_t)stream, a);
+        };
+        auto by_rows = [&](auto v) {
+            if (many) go(v, std::integral_constant<int, 4>{});
+            else go(v, std::integral_constant<int, 1>{});
+        };
+        if (vec) by_rows(std::true_type{});
+        else by_rows(std::false_type{});
     });
     check_launch("cache_append");
 }
