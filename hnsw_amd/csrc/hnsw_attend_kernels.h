@@ -133,17 +133,12 @@ __device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_
     for (uint32_t b0 = 0; b0 < a.n_requests; b0 += 64) {
         uint32_t n = 0;
         if (b0 + lane < a.n_requests) n = (uint32_t)(((uint64_t)rows_of(a, b0 + lane).count * group + tile - 1) / tile);
-        uint32_t upto = n;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t y = __shfl_up(upto, off);
-            if (lane >= (uint32_t)off) upto += y;
-        }
+        const uint32_t upto = wave_inclusive_sum(n);
         const unsigned long long m = __ballot(before + upto > u);
         if (m) {
             const int at = __builtin_ctzll(m);
             request = b0 + at;
-            part = __builtin_amdgcn_readfirstlane(u - before - (__shfl(upto, at) - __shfl(n, at)));
+            part = u - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
@@ -243,7 +238,8 @@ __device__ __forceinline__ bool table_entries(const AttendArgs& a, uint32_t b, u
 }
 
 // Wavefronts of a SIMD that the registers must leave room for: what hides the latency of the loads.
-constexpr int rows_waves(int dp, int mt) { return mt == 1 ? (dp == 64 ? 4 : dp == 128 ? 3 : 2) : (dp == 64 ? 3 : 2); }
+constexpr int rows_depth(int dp, int mt, int nw) { return dp <= 128 && mt == 1 && (dp == 64 || nw != 4) ? 2 : 1; }
+constexpr int rows_waves(int dp, int mt, int nw) { return dp == 64 ? (mt == 1 ? 4 : 3) : dp == 128 && mt == 1 && rows_depth(dp, mt, nw) == 1 ? 3 : 2; }
 
 // Attention of few query rows over many tokens: for single tokens the codes are read once and that is the time.
 //
@@ -263,9 +259,9 @@ constexpr int rows_waves(int dp, int mt) { return mt == 1 ? (dp == 64 ? 4 : dp =
 // A workgroup's start is a chain of loads that wait for one another (length, table, codes; for lists: ids, table, codes): the first
 // tile's codes are asked for as soon as the table is there, and queries and scales are made ready meanwhile.
 template <class T, int CODES, int DP, int MT, int NW, bool FOUND>
-__global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
+__global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
 {
-    constexpr int KS = DP / 32, KW = DP / 64, VW = DP / 64, VB = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
+    constexpr int KS = DP / 32, KW = DP / 64, VW = DP / 64, VB = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>, DEPTH = rows_depth(DP, MT, NW);
     constexpr uint32_t kThreads = 64 * NW, kTable = FOUND ? (NW == 1 ? 256 : kListTokens) : (NW == 1 ? 1024 : kScanTokens);      // items of a table
     constexpr uint32_t kEntries = FOUND ? kTable + kTile : kTable / 16 + 1, kMine = FOUND ? kTable / kThreads : 1;   // (one a thread of all tokens: 16 to a block at least)
     static_assert(FOUND || kTable / 16 <= kThreads);
@@ -349,8 +345,8 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
 #pragma unroll
         for (int i = 0; i < VB; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    u32x4 tk[2][KW];                                            // a tile's codes, keys and values
-    uint32_t tv[8][VW];
+    u32x4 tk[DEPTH][2][KW];                                     // tiles' codes, keys and values
+    uint32_t tv[DEPTH][8][VW];
     uint32_t c0 = begin, c1 = 0, n = 0, e0 = 0, safe = 0;       // the table: items c0 .. c1, n of them; its first block; a row of codes of a live token
     uint32_t bh[kMine], at[kMine];                              // (block, head) of this thread's entries, ~0: of none, and their places
 
@@ -421,7 +417,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
         }
         return w;
     };
-    auto fetch_keys = [&](uint32_t j, const Where& w) {
+    auto fetch_keys = [&](auto buf, uint32_t j, const Where& w) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint8_t* p = a.k_codes;
@@ -435,11 +431,11 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
 #pragma unroll
             for (int i = 0; i < KW; i++) {
                 const uint32_t c = 64 * i + 16 * g;
-                tk[h][i] = *reinterpret_cast<const u32x4*>(p + off + (c < dim ? c : 0));
+                tk[buf.value][h][i] = *reinterpret_cast<const u32x4*>(p + off + (c < dim ? c : 0));
             }
         }
     };
-    auto fetch_values = [&](uint32_t j, const Where& w) {
+    auto fetch_values = [&](auto buf, uint32_t j, const Where& w) {
         const uint32_t c = VB * m;
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -458,24 +454,32 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
                 }
                 if constexpr (VW == 2) {
                     const u32x2 x = *reinterpret_cast<const u32x2*>(p + off + (c < dim ? c : 0));
-                    tv[4 * h + r][0] = x[0]; tv[4 * h + r][1] = x[1];
+                    tv[buf.value][4 * h + r][0] = x[0]; tv[buf.value][4 * h + r][1] = x[1];
                 } else if constexpr (VW == 4) {
                     const u32x4 x = *reinterpret_cast<const u32x4*>(p + off + (c < dim ? c : 0));
 #pragma unroll
-                    for (int i = 0; i < 4; i++) tv[4 * h + r][i] = x[i];
+                    for (int i = 0; i < 4; i++) tv[buf.value][4 * h + r][i] = x[i];
                 } else {                                        // (a lane's bytes can end with the row in their middle)
 #pragma unroll
-                    for (int i = 0; i < VW; i++) tv[4 * h + r][i] = *reinterpret_cast<const uint32_t*>(p + off + (c + 4 * i < dim ? c + 4 * i : 0));
+                    for (int i = 0; i < VW; i++) tv[buf.value][4 * h + r][i] = *reinterpret_cast<const uint32_t*>(p + off + (c + 4 * i < dim ? c + 4 * i : 0));
                 }
             }
     };
 
+    auto first_tiles = [&]() {
+        auto one = [&](auto buf) {
+            const uint32_t j = wave + buf.value * NW;
+            if (32 * j < n) {
+                const Where w = locate(j);
+                fetch_keys(buf, j, w);
+                fetch_values(buf, j, w);
+            }
+        };
+        one(std::integral_constant<int, 0>{});
+        if constexpr (DEPTH == 2) one(std::integral_constant<int, 1>{});
+    };
     bool some = begin < end && open_table();                    // (the same in all threads)
-    if (some && 32 * wave < n) {
-        const Where w = locate(wave);
-        fetch_keys(wave, w);
-        fetch_values(wave, w);
-    }
+    if (some) first_tiles();
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
     while (c0 < end) {
@@ -498,8 +502,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
                     largest = sv;
                 }
             }
-#pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off));
+            largest = wave_max_not_negative(largest);
             if (lane == 0) red[wave] = largest;
             __syncthreads();
 #pragma unroll
@@ -516,26 +519,26 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
                 unit_v = largest;
             }
 
-            for (uint32_t j = wave; 32 * j < n; j += NW) {
-                const uint32_t i0 = 32 * j;
-                const bool more = i0 + 32 * NW < n;
+            auto take = [&](auto buf, uint32_t j) {
+                const uint32_t i0 = 32 * j, ahead = j + DEPTH * NW;
+                const bool more = 32 * ahead < n;
                 f32x4 s[MT][2];
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++) {
-                        const f16x8 k = decode8<CODES>(tk[h][ks / 2][2 * (ks % 2)], tk[h][ks / 2][2 * (ks % 2) + 1]);
+                        const f16x8 k = decode8<CODES>(tk[buf.value][h][ks / 2][2 * (ks % 2)], tk[buf.value][h][ks / 2][2 * (ks % 2) + 1]);
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                             for (int qt = 0; qt < QT; qt++)
                                 s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][h] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
                     }
-                // the keys' registers are free: the next tile's keys are under way while this one's weights meet its values
+                // the keys' registers are free: a later tile's keys are under way while this one's weights meet its values
                 Where next{};
                 if (more) {
-                    next = locate(j + NW);
-                    fetch_keys(j + NW, next);
+                    next = locate(ahead);
+                    fetch_keys(buf, ahead, next);
                 }
                 float fk[2][4], pw[2][4];                       // the scales of this lane's tokens 4g + r of both halves
                 bool gone[2] = {false, false}, ragged;
@@ -600,7 +603,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
                     uint32_t w[8];
                     f16x8 v[4];
 #pragma unroll
-                    for (int r = 0; r < 8; r++) w[r] = tv[r][i];
+                    for (int r = 0; r < 8; r++) w[r] = tv[buf.value][r][i];
                     decode_columns<CODES>(w, v);
 #pragma unroll
                     for (int c = 0; c < 4; c++)
@@ -609,18 +612,21 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT)) void attend_rows_kerne
 #pragma unroll
                             for (int pt = 0; pt < PT; pt++) o[mt][4 * i + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p[mt][pt], o[mt][4 * i + c], 0, 0, 0);
                 }
-                if (more) fetch_values(j + NW, next);
+                if (more) fetch_values(buf, ahead, next);
+            };
+            for (uint32_t j = wave; 32 * j < n; j += DEPTH * NW) {
+                take(std::integral_constant<int, 0>{}, j);
+                if constexpr (DEPTH == 2) {
+                    if (32 * (j + NW) >= n) break;
+                    take(std::integral_constant<int, 1>{}, j + NW);
+                }
             }
         }
         c0 += kTable;
         if (c0 >= end) break;
         __syncthreads();                                        // the table's last readers are done
         some = open_table();
-        if (some && 32 * wave < n) {
-            const Where w = locate(wave);
-            fetch_keys(wave, w);
-            fetch_values(wave, w);
-        }
+        if (some) first_tiles();
     }
 
     // the wavefronts' softmaxes become one
@@ -720,7 +726,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     const uint32_t n_r = rows.count * group, r0 = part * kRows + wave * 16 * MT;
     const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
 
-    uint32_t seen[MT], least = 0xffffffffu, most = 0;
+    uint32_t seen[MT];
     f16x8 q[MT][KS][QT];
     float factor[MT];
 #pragma unroll
@@ -729,18 +735,13 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         const bool there = r < n_r;
         const uint32_t i = there ? r / group : 0, h = kv * group + (there ? r - i * group : 0);
         seen[mt] = there ? seen_by(a, len, rows.count, i) : 0;
-        if (there) { least = min(least, seen[mt]); most = max(most, seen[mt]); }
         RawQuery<T, KS> raw;
         load_query<T, KS>(a, there, rows.first + i, h, q_vec, [&](int s) { return 32 * s + 8 * g; }, raw);
         factor[mt] = query_operands<T, CODES, KS, QT>(a, raw, q[mt]);
     }
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
-        least = min(least, (uint32_t)__shfl_xor((int)least, off));
-        most = max(most, (uint32_t)__shfl_xor((int)most, off));
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
+    // (rows follow one another in what they see; a wavefront without rows sees nothing)
+    const uint32_t least = r0 < n_r ? seen_by(a, len, rows.count, r0 / group) : 0;
+    const uint32_t most = r0 < n_r ? seen_by(a, len, rows.count, (min(r0 + 16 * MT, n_r) - 1) / group) : 0;
     // what the workgroup's last row sees
     const uint32_t last_r = min((part + 1) * kRows, n_r) - 1;
     const uint32_t all = seen_by(a, len, rows.count, last_r / group);

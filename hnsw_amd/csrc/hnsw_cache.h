@@ -111,6 +111,29 @@ template <int CODES> __device__ __forceinline__ uint32_t encode4(const float (&x
     }
 }
 
+// Across the 64 lanes with the data-parallel moves of the vector unit, which take a few cycles where a shuffle through LDS takes a hundred.
+__device__ __forceinline__ uint32_t wave_inclusive_sum(uint32_t x)
+{
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);      // 1, 2, 4, 8 lanes up within 16
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);      // the last lane of 16 to the next 16
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);      // the last lane of 32 to the other 32
+    return x;
+}
+__device__ __forceinline__ float wave_max_not_negative(float y)
+{
+    int x = __float_as_int(y);                                  // (floats that are not negative are ordered as integers)
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return __int_as_float(__builtin_amdgcn_readlane(x, 63));
+}
+
 // The request that row t belongs to: largest b with cu[b] <= t (cu ascending, cu[0] = 0); n when t is behind the last one.
 __device__ __forceinline__ uint32_t request_of(const int32_t* cu, uint32_t n, uint32_t t)
 {

@@ -7,6 +7,8 @@
 // A token's row of one head is contiguous, so that a token found by a search is one 128-byte line (at 128 dims), and the rows
 // of a block and head are contiguous, so that a scan streams.
 // The reference indexes vectors and has no counterpart of this.
+#include <algorithm>
+
 #include "hnsw_cache.h"
 
 namespace hnsw_amd {
@@ -23,18 +25,8 @@ struct PlanArgs {
     int64_t* slots;
     int32_t *cu_new, *lens_out, *status;
     int64_t* state_out;
-    uint32_t n_requests, width, n_blocks, block_tokens, n_slots;
+    uint32_t n_requests, width, n_blocks, block_tokens, n_slots, per;      // per: slots in a row that a thread maps
 };
-
-template <class T> __device__ __forceinline__ T wave_inclusive_sum(T x, uint32_t lane)
-{
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T y = __shfl_up(x, off);
-        if (lane >= (uint32_t)off) x += y;
-    }
-    return x;
-}
 
 // last b in [0, n) with pre[b] <= i (pre ascending, pre[0] = 0)
 __device__ __forceinline__ uint32_t last_not_after(const uint32_t* pre, uint32_t n, uint32_t i)
@@ -86,7 +78,7 @@ __global__ void plan_kernel(PlanArgs a)
         len_s[b] = len; cu_s[b] = g_sum; need_s[b] = need_sum; back_s[b] = back_sum;
         g_sum += g; need_sum += need; back_sum += back; g_all += g; back_all += back;
     }
-    const uint32_t gi = wave_inclusive_sum(g_sum, lane), ni = wave_inclusive_sum(need_sum, lane), bi = wave_inclusive_sum(back_sum, lane);
+    const uint32_t gi = wave_inclusive_sum(g_sum), ni = wave_inclusive_sum(need_sum), bi = wave_inclusive_sum(back_sum);
     if (lane == 63) { wsum[0][wave] = gi; wsum[1][wave] = ni; wsum[2][wave] = bi; }
     if (bad) atomicOr(&trouble, bad);
     if (g_all) atomicAdd(&total_grow, g_all);
@@ -111,11 +103,11 @@ __global__ void plan_kernel(PlanArgs a)
 
     auto ring_at = [&](uint32_t from, uint32_t i) { const unsigned long long p = (unsigned long long)from + i; return (uint32_t)(p >= a.n_blocks ? p - a.n_blocks : p); };
     const uint32_t stride = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + tid;
-    // four slots in a row: one search for the request, one block looked up for most of them
-    for (uint32_t t0 = 4 * me; t0 < a.n_slots; t0 += 4 * stride) {
+    // slots in a row: one search for the request, one block looked up for most of them
+    for (uint32_t t0 = a.per * me; t0 < a.n_slots; t0 += a.per * stride) {
         uint32_t b = t0 < grown ? last_not_after(cu_s, n, t0) : n, block = ~0u, of = ~0u;        // (block `block` of request `of` is number blk)
         int32_t blk = -1;
-        for (uint32_t t = t0; t < t0 + 4 && t < a.n_slots; t++) {
+        for (uint32_t t = t0; t < t0 + a.per && t < a.n_slots; t++) {
             int64_t slot = -1;
             if (t < grown) {
                 while (b + 1 < n && cu_s[b + 1] <= t) b++;
@@ -247,8 +239,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
                     look(x);
                 }
             }
-#pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
+            peak = wave_max_not_negative(peak);
             if constexpr (WPR > 1) {
                 if (lane == 0) peaks[sub] = peak;
                 __syncthreads();
@@ -372,12 +363,11 @@ void cache_plan(const int32_t* lens, const int32_t* grow, uint32_t n_requests, i
     if (n_slots > 0x7fffffffu) throw std::invalid_argument("cache_plan: n_slots must be below 2^31");
     if (lens == lens_out || state == state_out) throw std::invalid_argument("cache_plan: the new lengths and ring state need buffers of their own");
     const OnDevice on(device);
-    const PlanArgs a{lens, grow, table, ring, state, slots, cu_new, lens_out, status, state_out, n_requests, width, n_blocks, block_tokens, n_slots};
-    // Few requests and slots: one small workgroup.  Else enough workgroups for a pass of four slots (one request) a thread, 512 at most.
-    const uint32_t items = (n_slots + 3) / 4 > n_requests ? (n_slots + 3) / 4 : n_requests;
-    const uint32_t threads = items <= 256 ? 256 : 1024;
+    // A slot a thread, or four in a row where there are more than a few workgroups of them; 512 workgroups at most.
+    const uint32_t per = n_slots > 4096 ? 4 : 1, items = std::max((n_slots + per - 1) / per, n_requests), threads = items <= 256 ? 256 : 1024;
     uint32_t groups = (items + threads - 1) / threads;
     if (groups > 512) groups = 512;
+    const PlanArgs a{lens, grow, table, ring, state, slots, cu_new, lens_out, status, state_out, n_requests, width, n_blocks, block_tokens, n_slots, per};
     const size_t lds = (size_t)n_requests * 16;
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
