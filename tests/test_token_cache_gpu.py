@@ -1,4 +1,5 @@
 """The token cache's kernels against plain statements of the same operators in 64 bits (tests/cache_reference.py)."""
+import ctypes
 import random
 
 import numpy as np
@@ -288,11 +289,13 @@ def test_attend_many_tokens(lens, new, heads, group, block, dim, codes, dtype, c
         return b, np.arange(max(0, lens[b] - new[b] + (r - cu[b]) + 1) if causal else lens[b])
 
     L, cache = capi.lib(), s.cache
-    nbytes = L.hnsw_amd_cache_attend_workspace(cache._at, rows + behind, heads * group, len(lens), s.table.shape[1], max(lens))
+    c = capi.TokenCacheC(cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), *cache.k_codes.shape, int(codes is E4))
+    c_at = ctypes.addressof(c)
+    nbytes = L.hnsw_amd_cache_attend_workspace(c_at, rows + behind, heads * group, len(lens), s.table.shape[1], max(lens))
     work = torch.full((max(nbytes, 1),), 0xff, dtype=torch.uint8, device="cuda")
     out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
     d_cu = _gpu(cu)
-    capi.check(L.hnsw_amd_cache_attend_device(cache._at, q.data_ptr(), rows + behind, heads * group, q.stride(0), q.stride(1), {F32: 0, F16: 1, BF16: 2}[dtype],
+    capi.check(L.hnsw_amd_cache_attend_device(c_at, q.data_ptr(), rows + behind, heads * group, q.stride(0), q.stride(1), {F32: 0, F16: 1, BF16: 2}[dtype],
                                               s.d_table.data_ptr(), s.table.shape[1], s.d_lens.data_ptr(), len(lens), d_cu.data_ptr(), int(causal), dim ** -0.5, max(lens),
                                               out.data_ptr(), lse.data_ptr(), work.data_ptr(), nbytes, 0, torch.cuda.current_stream().cuda_stream))
     assert bool((out[rows:] == 7.0).all()) and bool((lse[rows:] == 7.0).all())
