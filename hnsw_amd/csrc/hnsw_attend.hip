@@ -42,9 +42,9 @@ static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_
     const uint64_t have = (uint64_t)c.units * heads, total = have * items;
     uint64_t chunk;
     if (c.tiles) {
-        // enough workgroups for every compute unit; a chunk of 512 tokens at least
-        const uint64_t splits = have ? (256 + have - 1) / have : 1;
-        chunk = std::max<uint64_t>((((uint64_t)items + splits - 1) / splits + 511) / 512 * 512, 512);
+        // two workgroups for every compute unit; a chunk of 512 tokens at least
+        const uint64_t splits = have ? (512 + have - 1) / have : 1;
+        chunk = std::max<uint64_t>((((uint64_t)items + splits - 1) / splits + 63) / 64 * 64, 512);
     } else if (c.mt == 1 && have >= 1024 && items <= 256) {
         // short requests (lists) in number: a wavefront for each, nothing to join
         c.waves = 1;

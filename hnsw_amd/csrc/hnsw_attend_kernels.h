@@ -310,6 +310,20 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
         const uint32_t i = there ? r / group : 0, h = head * group + (there ? r - i * group : 0);
         load_query<T, KS>(a, there, first + i, h, q_vec, [&](int s) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); }, raw[mt]);
     }
+    // the first table's block numbers, or ids: asked for before the length is there to say how many count
+    const uint32_t begin = split * parts.chunk;
+    uint32_t early[kMine];
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; e++) {
+        early[e] = ~0u;
+        if constexpr (FOUND) {
+            const uint32_t i = begin + e * kThreads + tid;
+            if (i < a.n_ids) early[e] = (uint32_t)a.ids[((size_t)first * heads + head) * a.n_ids + i];
+        } else {
+            const uint32_t i = (begin >> bs_log) + tid;
+            if (tid < kEntries && i < a.width) early[e] = (uint32_t)a.table[(size_t)b * a.width + i];
+        }
+    }
     const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
@@ -330,7 +344,6 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     }
 
     const uint32_t all = FOUND ? a.n_ids : most;                // items: tokens, or list entries
-    const uint32_t begin = split * parts.chunk;
     if (!FOUND && split > 0 && begin >= all) return;            // (a row that sees no token of a chunk does not ask for its part)
     const uint32_t end = split + 1 < parts.n_splits ? min(begin + parts.chunk, all) : all;
 
@@ -359,7 +372,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
             const int32_t* ids = a.ids + ((size_t)first * heads + head) * a.n_ids;
             uint32_t id[kMine], kept = 0;
 #pragma unroll
-            for (uint32_t e = 0; e < kMine; e++) id[e] = e * kThreads + tid < n ? (uint32_t)ids[c0 + e * kThreads + tid] : ~0u;
+            for (uint32_t e = 0; e < kMine; e++) id[e] = e * kThreads + tid >= n ? ~0u : c0 == begin ? early[e] : (uint32_t)ids[c0 + e * kThreads + tid];
 #pragma unroll
             for (uint32_t e = 0; e < kMine; e++) {
                 const uint32_t blk = id[e] < seen[0] ? (uint32_t)a.table[(size_t)b * a.width + (id[e] >> bs_log)] : ~0u;
@@ -388,7 +401,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
         } else {
             e0 = c0 >> bs_log;
             const bool mine = tid <= ((c1 - 1) >> bs_log) - e0;
-            const uint32_t blk = mine ? (uint32_t)a.table[(size_t)b * a.width + e0 + tid] : ~0u;
+            const uint32_t blk = !mine ? ~0u : c0 == begin ? early[0] : (uint32_t)a.table[(size_t)b * a.width + e0 + tid];
             bh[0] = blk < a.n_blocks ? blk * a.n_heads + kv : ~0u;
             if (mine) ent_row[tid] = bh[0] == ~0u ? ~0u : bh[0] << bs_log;
             const unsigned long long fine = __ballot(bh[0] != ~0u);
@@ -983,6 +996,15 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     }
 }
 
+// Chunks that a row's softmax has parts of.
+__device__ __forceinline__ uint32_t chunks_of(const AttendArgs& a, const Partials& parts, uint32_t b, uint32_t row)
+{
+    if (a.found) return parts.n_splits;
+    const Span s = rows_of(a, b);
+    const uint32_t sees = seen_by(a, length_of(a, b), s.count, row - s.first);
+    return min(parts.n_splits, (uint32_t)(((uint64_t)sees + parts.chunk - 1) / parts.chunk));
+}
+
 // The chunks' outputs of a row and head become one: weights 2^(lse - largest).  One workgroup each: dim / 4 lanes take a chunk, so that
 // 256 / (dim / 4) chunks are read at a time.
 template <class T>
@@ -993,12 +1015,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials
     const uint32_t tid = threadIdx.x, lane = tid & 63, to = blockIdx.x, row = to / a.q_heads;
     const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
     if (b >= a.n_requests) return;
-    uint32_t n = parts.n_splits;
-    if (!a.found) {
-        const Span s = rows_of(a, b);
-        const uint32_t sees = seen_by(a, length_of(a, b), s.count, row - s.first);
-        n = min(n, (uint32_t)(((uint64_t)sees + parts.chunk - 1) / parts.chunk));
-    }
+    const uint32_t n = chunks_of(a, parts, b, row);
     const float* lse = parts.lse + (size_t)to * parts.n_splits;
     const float* x = parts.out + (size_t)to * parts.n_splits * a.dim;
     const uint32_t lanes = a.dim / 4, per = 256 / lanes, mine = tid / lanes, d = (tid - mine * lanes) * 4;
@@ -1046,6 +1063,36 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials
     if (tid == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
+// The same for few chunks: dim / 4 lanes take a row and head, and all of its chunks one after the other.
+template <class T>
+__global__ __launch_bounds__(256) void attend_join_few_kernel(AttendArgs a, Partials parts)
+{
+    const uint32_t lanes = a.dim / 4, per = 256 / lanes, mine = threadIdx.x / lanes, d = (threadIdx.x - mine * lanes) * 4;
+    const uint64_t to = (uint64_t)blockIdx.x * per + mine;
+    if (mine >= per || to >= (uint64_t)a.n_rows * a.q_heads) return;
+    const uint32_t row = (uint32_t)(to / a.q_heads);
+    const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
+    if (b >= a.n_requests) return;
+    const uint32_t n = chunks_of(a, parts, b, row);
+    const float* lse = parts.lse + to * parts.n_splits;
+    const float* x = parts.out + to * parts.n_splits * a.dim + d;
+    float top = -__builtin_inff(), l = 0.0f;
+    for (uint32_t i = 0; i < n; i++) top = fmaxf(top, lse[i]);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (uint32_t i = 0; i < n; i++) {
+        const float4 y = *reinterpret_cast<const float4*>(x + (size_t)i * a.dim);
+        const float f = __builtin_amdgcn_exp2f(lse[i] - ref);
+        l += f;
+        o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = (T*)a.out + to * a.dim + d;
+    out[0] = from_float<T>(o.x * inv); out[1] = from_float<T>(o.y * inv); out[2] = from_float<T>(o.z * inv); out[3] = from_float<T>(o.w * inv);
+    if (d == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
 }  // namespace
 
 template <class T> void launch_attend(const AttendArgs& a, const Cut& cut, uint32_t codes_, float* workspace, hipStream_t stream)
@@ -1083,7 +1130,13 @@ template <class T> void launch_attend(const AttendArgs& a, const Cut& cut, uint3
     else by_dim(std::integral_constant<int, HNSW_AMD_CODES_E4M3>{});
     check_launch(who);
     if (cut.n_splits > 1) {
-        hipLaunchKernelGGL((attend_join_kernel<T>), dim3(a.n_rows * a.q_heads), dim3(256), 0, stream, a, parts);
+        // few chunks: many rows to a workgroup (20480 rows of 64 dims in 2 chunks: 4 us, 38 with a workgroup each)
+        if (cut.n_splits <= 8) {
+            const uint32_t per = 256 / (a.dim / 4);
+            hipLaunchKernelGGL((attend_join_few_kernel<T>), dim3((a.n_rows * a.q_heads + per - 1) / per), dim3(256), 0, stream, a, parts);
+        } else {
+            hipLaunchKernelGGL((attend_join_kernel<T>), dim3(a.n_rows * a.q_heads), dim3(256), 0, stream, a, parts);
+        }
         check_launch(who);
     }
 }
