@@ -199,44 +199,6 @@ __device__ __forceinline__ float query_operands(const AttendArgs& a, const RawQu
     return ldexpf(fabsf(a.scale) * kLog2e, -e);
 }
 
-// Block entries of the tokens c0 .. c1 of request b into LDS, by a workgroup of 256 threads: first row of a block's codes (in rows of dim
-// bytes) and its scales.  An entry of no block has the key scale -1 and the row of one that is, so that loads stay among codes of
-// live tokens: weights of 0 do not meet the NaN that stale codes can be.  Returns the largest value scale; false where no entry is of a block.
-struct Reduced { float largest[kWaves]; uint32_t some[kWaves]; };
-__device__ __forceinline__ bool table_entries(const AttendArgs& a, uint32_t b, uint32_t kv, uint32_t bs_log, uint32_t c0, uint32_t c1, uint32_t tid,
-                                              uint32_t* ent_row, float* ent_k, float* ent_v, Reduced& red, float& largest)
-{
-    const uint32_t e0 = c0 >> bs_log, n_e = ((c1 - 1) >> bs_log) - e0 + 1, lane = tid & 63, wave = tid >> 6;
-    uint32_t some = 0;                                          // a row + 1
-    largest = 0.0f;
-    for (uint32_t i = tid; i < n_e; i += 256) {
-        const uint32_t blk = (uint32_t)a.table[(size_t)b * a.width + e0 + i];
-        uint32_t row = 0;
-        float sk = -1.0f, sv = 0.0f;
-        if (blk < a.n_blocks) {
-            const uint32_t bh = blk * a.n_heads + kv;
-            row = bh << bs_log;
-            sk = a.k_scale[bh];
-            sv = a.v_scale[bh];
-            some = row + 1;
-            largest = fmaxf(largest, sv);
-        }
-        ent_row[i] = row; ent_k[i] = sk; ent_v[i] = sv;
-    }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        largest = fmaxf(largest, __shfl_xor(largest, off));
-        some = max(some, (uint32_t)__shfl_xor((int)some, off));
-    }
-    if (lane == 0) { red.largest[wave] = largest; red.some[wave] = some; }
-    __syncthreads();
-    largest = fmaxf(fmaxf(red.largest[0], red.largest[1]), fmaxf(red.largest[2], red.largest[3]));
-    some = __builtin_amdgcn_readfirstlane(max(max(red.some[0], red.some[1]), max(red.some[2], red.some[3])));
-    for (uint32_t i = tid; i < n_e; i += 256)                   // (the entries that this thread wrote)
-        if (ent_k[i] < 0.0f) ent_row[i] = some - 1;
-    return some != 0;
-}
-
 // Wavefronts of a SIMD that the registers must leave room for: what hides the latency of the loads.
 constexpr int rows_depth(int dp, int mt, int nw) { return dp <= 128 && mt == 1 && (dp == 64 || nw != 4) ? 2 : 1; }
 constexpr int rows_waves(int dp, int mt, int nw) { return dp == 64 ? (mt == 1 ? 4 : 3) : dp == 128 && mt == 1 && rows_depth(dp, mt, nw) == 1 ? 3 : 2; }
@@ -717,10 +679,10 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     constexpr int KS = DP / 32, DT = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
     constexpr int kTokens = 64, kKeyLd = DP + 8;                 // 16-bit elements
     constexpr int KL = DP / 64, VL = (DP + 127) / 128;          // 16-byte pieces of keys, and words x 8 tokens of values, that a thread moves
-    constexpr uint32_t kEntries = kScanTokens / 16 + 2;
-    __shared__ uint32_t ent_row[kEntries];
-    __shared__ float ent_k[kEntries], ent_v[kEntries];
-    __shared__ Reduced red;
+    constexpr uint32_t kEntries = kScanTokens / 16 + 1;
+    static_assert(kScanTokens / 16 <= 256);
+    __shared__ uint32_t ent_row[kEntries], some[kWaves];        // first row of a block's codes, in rows of dim bytes; ~0: of no block
+    __shared__ float red[kWaves];
     __shared__ __align__(16) float4 ent[kEntries];              // key scale, log2 of the weights' factor, its inverse; key scale -1: there is no block
     __shared__ __align__(16) _Float16 keys[NBUF][kTokens * kKeyLd];
     __shared__ __align__(16) _Float16 vals[NBUF][DP * kTokens];
@@ -737,31 +699,33 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     if (!unit_of(a, unit, group, kRows, lane, b, part)) return;
     const Span rows = uniform(rows_of(a, b));
     const uint32_t n_r = rows.count * group, r0 = part * kRows + wave * 16 * MT;
-    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
-
+    // queries and the first table's block numbers: asked for before the length is there
+    RawQuery<T, KS> raw[MT];
     uint32_t seen[MT];
-    f16x8 q[MT][KS][QT];
-    float factor[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
         const uint32_t r = r0 + 16 * mt + m;
         const bool there = r < n_r;
         const uint32_t i = there ? r / group : 0, h = kv * group + (there ? r - i * group : 0);
-        seen[mt] = there ? seen_by(a, len, rows.count, i) : 0;
-        RawQuery<T, KS> raw;
-        load_query<T, KS>(a, there, rows.first + i, h, q_vec, [&](int s) { return 32 * s + 8 * g; }, raw);
-        factor[mt] = query_operands<T, CODES, KS, QT>(a, raw, q[mt]);
+        seen[mt] = i;
+        load_query<T, KS>(a, there, rows.first + i, h, q_vec, [&](int s) { return 32 * s + 8 * g; }, raw[mt]);
     }
+    const uint32_t begin = split * parts.chunk, e_begin = begin >> bs_log;
+    const uint32_t early = e_begin + tid < a.width ? (uint32_t)a.table[(size_t)b * a.width + e_begin + tid] : ~0u;
+    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) seen[mt] = r0 + 16 * mt + m < n_r ? seen_by(a, len, rows.count, seen[mt]) : 0;
     // (rows follow one another in what they see; a wavefront without rows sees nothing)
     const uint32_t least = r0 < n_r ? seen_by(a, len, rows.count, r0 / group) : 0;
     const uint32_t most = r0 < n_r ? seen_by(a, len, rows.count, (min(r0 + 16 * MT, n_r) - 1) / group) : 0;
     // what the workgroup's last row sees
     const uint32_t last_r = min((part + 1) * kRows, n_r) - 1;
     const uint32_t all = seen_by(a, len, rows.count, last_r / group);
-    const uint32_t begin = split * parts.chunk;
     if (split > 0 && begin >= all) return;
     const uint32_t end = split + 1 < parts.n_splits ? min(begin + parts.chunk, all) : all;
 
+    f16x8 q[MT][KS][QT];
+    float factor[MT];
     f32x4 o[MT][DT];
     float top[MT], sum[MT], unit_v = 0.0f;
 #pragma unroll
@@ -772,191 +736,233 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         for (int i = 0; i < DT; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    for (uint32_t c0 = begin; c0 < end; c0 += kScanTokens) {
-        const uint32_t c1 = min(end - c0, kScanTokens) + c0, e0 = c0 >> bs_log;
-        __syncthreads();                                        // the last table's readers are done
-        float largest;
-        if (!table_entries(a, b, kv, bs_log, c0, c1, tid, ent_row, ent_k, ent_v, red, largest)) continue;
-        if (largest > 0.0f) {
-            if (unit_v > 0.0f && unit_v != largest) {
-                const float change = unit_v / largest;
+    // the table: tokens c0 .. c1, its first block, a row of codes of a live token, (block, head) of this thread's entry (~0: of none)
+    uint32_t c0 = begin, c1 = 0, e0 = 0, safe = 0, bh = ~0u;
+    u32x4 kr[KL];
+    uint32_t vr[VL][8];
+    const uint32_t k_row = lane >> 2, oct = 2 * wave + (lane >> 5), v_row = 4 * (oct & 3), v_word = lane & 31;
+    uint32_t k_off[KL], v_off[VL];                              // of a whole tile's codes
+#pragma unroll
+    for (int i = 0; i < KL; i++) k_off[i] = k_row * dim + (64 * i + 16 * (lane & 3) < dim ? 64 * i + 16 * (lane & 3) : 0);
+#pragma unroll
+    for (int i = 0; i < VL; i++) v_off[i] = v_row * dim + (4 * (v_word + 32 * i) < dim ? 4 * (v_word + 32 * i) : 0);
+    // The next tile's codes: this wavefront's keys are 16 tokens of one block, its values the octets of two runs of 16 tokens.  (Tokens
+    // behind the last one are the last one; those of no block are some live token: stale codes can be NaN, which a weight of 0 would
+    // not remove.)
+    auto fetch = [&](uint32_t t0) {
+        const uint32_t last = c1 - 1, kt = min(t0 + 16 * wave, last), vt0 = min(t0 + 32 * (wave >> 1), last), vt1 = min(t0 + 32 * (wave >> 1) + 16, last);
+        const uint32_t ek = ent_row[(kt >> bs_log) - e0], ev0 = ent_row[(vt0 >> bs_log) - e0], ev1 = ent_row[(vt1 >> bs_log) - e0];
+        auto codes_at = [&](const uint8_t* codes, uint32_t entry, uint32_t pos) {
+            const uint32_t base = __builtin_amdgcn_readfirstlane(entry);
+            return codes + (uint64_t)((base == ~0u ? safe : base) + (pos & (bs - 1))) * dim;
+        };
+        const uint8_t *kb = codes_at(a.k_codes, ek, kt), *vb0 = codes_at(a.v_codes, ev0, vt0), *vb1 = codes_at(a.v_codes, ev1, vt1);
+        if (t0 + kTokens <= c1) {
+#pragma unroll
+            for (int i = 0; i < KL; i++) kr[i] = *reinterpret_cast<const u32x4*>(kb + k_off[i]);
+#pragma unroll
+            for (int i = 0; i < VL; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    vr[i][r] = *reinterpret_cast<const uint32_t*>(vb0 + (size_t)r * dim + v_off[i]);
+                    vr[i][4 + r] = *reinterpret_cast<const uint32_t*>(vb1 + (size_t)r * dim + v_off[i]);
+                }
+        } else {
+            const uint32_t k_back = k_row - min(k_row, last - kt);                  // rows that are not there
+#pragma unroll
+            for (int i = 0; i < KL; i++) kr[i] = *reinterpret_cast<const u32x4*>(kb + (k_off[i] - k_back * dim));
+#pragma unroll
+            for (int i = 0; i < VL; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t row = v_row + r;
+                    vr[i][r] = *reinterpret_cast<const uint32_t*>(vb0 + (v_off[i] - v_row * dim + min(row, last - vt0) * dim));
+                    vr[i][4 + r] = *reinterpret_cast<const uint32_t*>(vb1 + (v_off[i] - v_row * dim + min(row, last - vt1) * dim));
+                }
+        }
+    };
+    // the codes in registers become 16-bit floats in LDS, piece by piece: eight of a row of keys, or eight of a column of values
+    constexpr int kPieces = 2 * KL + 4 * VL;
+    auto store_piece = [&](int buf, int j) {
+        if (j < 2 * KL) {
+            const int i = j / 2, half = j % 2;
+            *reinterpret_cast<f16x8*>(&keys[buf][(16 * wave + k_row) * kKeyLd + 64 * i + 16 * (lane & 3) + 8 * half]) = decode8<CODES>(kr[i][2 * half], kr[i][2 * half + 1]);
+        } else {
+            const int i = (j - 2 * KL) / 4, col = (j - 2 * KL) % 4;
+            const uint32_t c = 4 * (v_word + 32 * i);
+            f16x8 v[4];
+            decode_columns<CODES>(vr[i], v);
+            if (DP % 128 == 0 || c < DP) *reinterpret_cast<f16x8*>(&vals[buf][val_at(c + col, oct)]) = v[col];
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < kPieces; j++) store_piece(buf, j);
+    };
+    auto compute = [&](uint32_t t0, int buf) {
+        if (t0 >= most) {                                   // none of this wavefront's rows sees the tile
+            if constexpr (NBUF == 2) store(buf ^ 1);
+            return;
+        }
+        float4 x[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) x[t] = ent[(min(t0 + 16 * t, c1 - 1) >> bs_log) - e0];
+        f32x4 s[MT][4];
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const f16x8 k = *reinterpret_cast<const f16x8*>(&keys[buf][(16 * t + m) * kKeyLd + 32 * ks + 8 * g]);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int i = 0; i < DT; i++) o[mt][i] *= change;
+                    for (int qt = 0; qt < QT; qt++)
+                        s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][t] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             }
-            unit_v = largest;
+        bool gone[4], any_gone = false;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            gone[t] = __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].x)) >> 31;
+            any_gone |= gone[t];
         }
-        // weights get a block's value scale over the largest by way of the exponent (a scale of 0 next to others counts as 2^-60 of it:
-        // weights that vanish as 16-bit floats)
-        for (uint32_t i = tid; i <= ((c1 - 1) >> bs_log) - e0; i += 256) {          // (the entries that this thread wrote)
-            const float w = largest > 0.0f ? fmaxf(ent_v[i] * (kPScale / largest), 0x1p-60f) : 1.0f;
-            ent[i] = make_float4(ent_k[i], __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
+        const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || any_gone;
+        float f[MT][4], ref[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            float local = -__builtin_inff();
+            if (ragged) {
+                const int left = (int)(min(seen[mt], c1) - t0 - 4 * g);         // (both are below 2^31)
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[mt][t][r] = 16 * t + r < left && !gone[t] ? s[mt][t][r] : -__builtin_inff();
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                f[mt][t] = fmaxf(x[t].x * factor[mt], 0x1p-126f);               // (not 0, which masked scores would make NaN)
+                local = fmaxf(local, f[mt][t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
+            }
+            if (__ballot(local > top[mt] + kLead)) {
+                const float now = fmaxf(top[mt], max_over_groups(local));
+                const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
+                top[mt] = now;
+                sum[mt] *= shrink;
+#pragma unroll
+                for (int i = 0; i < DT; i++) o[mt][i] *= shrink;
+            }
+            ref[mt] = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
         }
-        __syncthreads();
+        // the two halves of the tile: weights of one while the other's meet the values, and the next tile's codes become
+        // 16-bit floats meanwhile (their loads were issued before the scores)
+        f16x8 p[2][MT][PT];
+        auto weigh = [&](int mt, int t) {
+            const float by = x[t].y - ref[mt];
+            float part_sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][t][r], f[mt][t], by));
+                part_sum += w;
+                const _Float16 hi = (_Float16)w;
+                p[t / 2][mt][0][4 * (t % 2) + r] = hi;
+                if constexpr (PT == 2) p[t / 2][mt][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
+            }
+            sum[mt] = __builtin_fmaf(part_sum, x[t].z, sum[mt]);
+        };
+        // the values' operands are read from LDS kAhead products ahead
+        constexpr int kAhead = 2;
+        f16x8 v[kAhead];
+        auto read_values = [&](int j) { v[j % kAhead] = *reinterpret_cast<const f16x8*>(&vals[buf][val_at(16 * (j % DT) + m, 4 * (j / DT) + g)]); };
+        auto meet = [&](int j) {
+            const f16x8 now = v[j % kAhead];
+            if (j + kAhead < 2 * DT) read_values(j + kAhead);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int pt = 0; pt < PT; pt++) o[mt][j % DT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(now, p[j / DT][mt][pt], o[mt][j % DT], 0, 0, 0);
+        };
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) read_values(j);
+#pragma unroll
+        for (int j = 0; j < 2 * MT; j++) weigh(j / 2, j % 2);
+#pragma unroll
+        for (int i = 0; i < DT; i++) {
+            meet(i);
+#pragma unroll
+            for (int j = i * 2 * MT / DT; j < (i + 1) * 2 * MT / DT; j++) weigh(j / 2, 2 + j % 2);
+        }
+#pragma unroll
+        for (int i = 0; i < DT; i++) {
+            meet(DT + i);
+            if constexpr (NBUF == 2) {
+#pragma unroll
+                for (int j = i * kPieces / DT; j < (i + 1) * kPieces / DT; j++) store_piece(buf ^ 1, j);
+            }
+        }
+    };
 
-        u32x4 kr[KL];
-        uint32_t vr[VL][8];
-        const uint32_t k_row = lane >> 2, oct = 2 * wave + (lane >> 5), v_row = 4 * (oct & 3), v_word = lane & 31;
-        // the codes from token `start` on (16 of them, in one block; those behind the last token are the last one): their first row's
-        // offset, and how many there are
-        auto place = [&](uint32_t start, uint32_t& limit) {
-            const uint32_t pos = min(start, c1 - 1), base = __builtin_amdgcn_readfirstlane(ent_row[(pos >> bs_log) - e0]);
-            limit = min(c1 - 1 - pos, 15u);
-            return (uint64_t)(base + (pos & (bs - 1))) * dim;
-        };
-        auto fetch = [&](uint32_t t0) {
-            uint32_t limit;
-            const uint8_t* kb = a.k_codes + place(t0 + 16 * wave, limit);
-            const uint32_t kr0 = (limit == 15 ? k_row : min(k_row, limit)) * dim;
+    auto open_table = [&]() {                                   // false where no block of it exists
+        c1 = min(end - c0, kScanTokens) + c0;
+        e0 = c0 >> bs_log;
+        const bool mine = tid <= ((c1 - 1) >> bs_log) - e0;
+        const uint32_t blk = !mine ? ~0u : c0 == begin ? early : (uint32_t)a.table[(size_t)b * a.width + e0 + tid];
+        bh = blk < a.n_blocks ? blk * a.n_heads + kv : ~0u;
+        if (mine) ent_row[tid] = bh == ~0u ? ~0u : bh << bs_log;
+        const unsigned long long fine = __ballot(bh != ~0u);
+        if (lane == 0) some[wave] = fine ? (__builtin_amdgcn_readlane(bh, __builtin_ctzll(fine)) << bs_log) + 1 : 0;
+        __syncthreads();
+        safe = 0;
 #pragma unroll
-            for (int i = 0; i < KL; i++) {
-                const uint32_t c = 64 * i + 16 * (lane & 3);
-                kr[i] = *reinterpret_cast<const u32x4*>(kb + kr0 + (c < dim ? c : 0));
+        for (int w = 0; w < kWaves; w++) safe = safe ? safe : some[w];
+        safe = __builtin_amdgcn_readfirstlane(safe);
+        return safe-- != 0;
+    };
+    bool has = begin < end && open_table();                     // (the same in all threads)
+    if (has) fetch(c0);
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
+    while (c0 < end) {
+        if (has) {
+            // the entries' scales; weights get a block's value scale over the largest by way of the exponent (a scale of 0 next to others
+            // counts as 2^-60 of it: weights that vanish as 16-bit floats)
+            const float sk = bh != ~0u ? a.k_scale[bh] : -1.0f, sv = bh != ~0u ? a.v_scale[bh] : 0.0f;
+            float largest = wave_max_not_negative(sv);
+            if (lane == 0) red[wave] = largest;
+            __syncthreads();
+            largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+            if (tid <= ((c1 - 1) >> bs_log) - e0) {
+                const float w = largest > 0.0f ? fmaxf(sv * (kPScale / largest), 0x1p-60f) : 1.0f;
+                ent[tid] = make_float4(sk, __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
             }
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint8_t* vb = a.v_codes + place(t0 + 32 * (wave >> 1) + 16 * h, limit);
-#pragma unroll
-                for (int i = 0; i < VL; i++) {
-                    const uint32_t c = 4 * (v_word + 32 * i), at = c < dim ? c : 0;
-                    if (limit == 15) {
-                        const uint32_t v0 = v_row * dim + at;
-#pragma unroll
-                        for (int r = 0; r < 4; r++) vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(vb + (size_t)r * dim + v0);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; r++) vr[i][4 * h + r] = *reinterpret_cast<const uint32_t*>(vb + min(v_row + r, limit) * dim + at);
-                    }
-                }
-            }
-        };
-        // the codes in registers become 16-bit floats in LDS, piece by piece: eight of a row of keys, or eight of a column of values
-        constexpr int kPieces = 2 * KL + 4 * VL;
-        auto store_piece = [&](int buf, int j) {
-            if (j < 2 * KL) {
-                const int i = j / 2, half = j % 2;
-                *reinterpret_cast<f16x8*>(&keys[buf][(16 * wave + k_row) * kKeyLd + 64 * i + 16 * (lane & 3) + 8 * half]) = decode8<CODES>(kr[i][2 * half], kr[i][2 * half + 1]);
-            } else {
-                const int i = (j - 2 * KL) / 4, col = (j - 2 * KL) % 4;
-                const uint32_t c = 4 * (v_word + 32 * i);
-                f16x8 v[4];
-                decode_columns<CODES>(vr[i], v);
-                if (DP % 128 == 0 || c < DP) *reinterpret_cast<f16x8*>(&vals[buf][val_at(c + col, oct)]) = v[col];
-            }
-        };
-        auto store = [&](int buf) {
-#pragma unroll
-            for (int j = 0; j < kPieces; j++) store_piece(buf, j);
-        };
-        auto compute = [&](uint32_t t0, int buf) {
-            if (t0 >= most) {                                   // none of this wavefront's rows sees the tile
-                if constexpr (NBUF == 2) store(buf ^ 1);
-                return;
-            }
-            f32x4 s[MT][4];
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const f16x8 k = *reinterpret_cast<const f16x8*>(&keys[buf][(16 * t + m) * kKeyLd + 32 * ks + 8 * g]);
+            if (largest > 0.0f) {
+                if (unit_v > 0.0f && unit_v != largest) {       // outputs so far are in units of the last table's largest scale
+                    const float change = unit_v / largest;
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                        for (int qt = 0; qt < QT; qt++)
-                            s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][t] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                        for (int i = 0; i < DT; i++) o[mt][i] *= change;
                 }
-            float4 x[4];
-            bool gone[4], any_gone = false;
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                x[t] = ent[(min(t0 + 16 * t, c1 - 1) >> bs_log) - e0];
-                gone[t] = __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].x)) >> 31;
-                any_gone |= gone[t];
+                unit_v = largest;
             }
-            const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || any_gone;
-            float f[MT][4], ref[MT];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float local = -__builtin_inff();
-                if (ragged) {
-                    const int left = (int)(min(seen[mt], c1) - t0 - 4 * g);         // (both are below 2^31)
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) s[mt][t][r] = 16 * t + r < left && !gone[t] ? s[mt][t][r] : -__builtin_inff();
-                }
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    f[mt][t] = fmaxf(x[t].x * factor[mt], 0x1p-126f);               // (not 0, which masked scores would make NaN)
-                    local = fmaxf(local, f[mt][t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
-                }
-                if (__ballot(local > top[mt] + kLead)) {
-                    const float now = fmaxf(top[mt], max_over_groups(local));
-                    const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
-                    top[mt] = now;
-                    sum[mt] *= shrink;
-#pragma unroll
-                    for (int i = 0; i < DT; i++) o[mt][i] *= shrink;
-                }
-                ref[mt] = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
-            }
-            // the two halves of the tile: weights of one while the other's meet the values, and the next tile's codes become
-            // 16-bit floats meanwhile (their loads were issued before the scores)
-            f16x8 p[2][MT][PT];
-            auto weigh = [&](int mt, int t) {
-                const float by = x[t].y - ref[mt];
-                float part_sum = 0.0f;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][t][r], f[mt][t], by));
-                    part_sum += w;
-                    const _Float16 hi = (_Float16)w;
-                    p[t / 2][mt][0][4 * (t % 2) + r] = hi;
-                    if constexpr (PT == 2) p[t / 2][mt][1][4 * (t % 2) + r] = (_Float16)(w - (float)hi);
-                }
-                sum[mt] = __builtin_fmaf(part_sum, x[t].z, sum[mt]);
-            };
-            auto meet = [&](int h, int i) {
-                const f16x8 v = *reinterpret_cast<const f16x8*>(&vals[buf][val_at(16 * i + m, 4 * h + g)]);
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int pt = 0; pt < PT; pt++) o[mt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[h][mt][pt], o[mt][i], 0, 0, 0);
-            };
-#pragma unroll
-            for (int j = 0; j < 2 * MT; j++) weigh(j / 2, j % 2);
-#pragma unroll
-            for (int i = 0; i < DT; i++) {
-                meet(0, i);
-#pragma unroll
-                for (int j = i * 2 * MT / DT; j < (i + 1) * 2 * MT / DT; j++) weigh(j / 2, 2 + j % 2);
-            }
-#pragma unroll
-            for (int i = 0; i < DT; i++) {
-                meet(1, i);
-                if constexpr (NBUF == 2) {
-#pragma unroll
-                    for (int j = i * kPieces / DT; j < (i + 1) * kPieces / DT; j++) store_piece(buf ^ 1, j);
-                }
-            }
-        };
-
-        fetch(c0);
-        store(0);
-        __syncthreads();
-        int buf = 0;
-        for (uint32_t t0 = c0; t0 < c1; t0 += kTokens) {
-            if (t0 + kTokens < c1) fetch(t0 + kTokens);
-            compute(t0, buf);
-            if constexpr (NBUF == 1) {                          // the only buffer is about to be overwritten
-                __syncthreads();
-                store(0);
-            } else {
-                buf ^= 1;
-            }
+            store(0);
             __syncthreads();
+            int buf = 0;
+            for (uint32_t t0 = c0; t0 < c1; t0 += kTokens) {
+                if (t0 + kTokens < c1) fetch(t0 + kTokens);
+                compute(t0, buf);
+                if constexpr (NBUF == 1) {                      // the only buffer is about to be overwritten
+                    __syncthreads();
+                    store(0);
+                } else {
+                    buf ^= 1;
+                }
+                __syncthreads();
+            }
         }
+        c0 += kScanTokens;
+        if (c0 >= end) break;
+        __syncthreads();                                        // the table's last readers are done
+        has = open_table();
+        if (has) fetch(c0);
     }
 
     const float unit_o = unit_v / kPScale;
@@ -969,28 +975,17 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         const size_t to = (size_t)(rows.first + i) * a.q_heads + kv * group + (r - i * group);
         const float inv = l == 0.0f ? 0.0f : unit_o / l, lse = l == 0.0f ? -__builtin_inff() : top[mt] + __builtin_amdgcn_logf(l);
         if (parts.n_splits == 1) {
-            T* out = (T*)a.out + to * dim;
+            T* out = (T*)a.out + to * dim + 4 * g;
 #pragma unroll
             for (int t = 0; t < DT; t++)
-                if (16 * t < (int)dim) {
-                    const uint32_t d = 16 * t + 4 * g;
-                    if constexpr (sizeof(T) == 4) {
-                        *reinterpret_cast<float4*>(out + d) = make_float4(o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
-                    } else {
-                        u32x2 w;
-#pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            w[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(o[mt][t][2 * j] * inv)) | ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(o[mt][t][2 * j + 1] * inv)) << 16);
-                        *reinterpret_cast<u32x2*>(out + d) = w;
-                    }
-                }
+                if (16 * t < (int)dim) store4<T>(out + 16 * t, o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
             if (g == 0 && a.lse) a.lse[to] = lse * 0.6931471805599453f;
         } else {
             const size_t at = to * parts.n_splits + split;
+            float* out = parts.out + at * dim + 4 * g;
 #pragma unroll
             for (int t = 0; t < DT; t++)
-                if (16 * t < (int)dim)
-                    *reinterpret_cast<float4*>(parts.out + at * dim + 16 * t + 4 * g) = make_float4(o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
+                if (16 * t < (int)dim) store4<float>(out + 16 * t, o[mt][t][0] * inv, o[mt][t][1] * inv, o[mt][t][2] * inv, o[mt][t][3] * inv);
             if (g == 0) parts.lse[at] = lse;
         }
     }
@@ -1057,8 +1052,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials
             o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        T* out = (T*)a.out + (size_t)to * a.dim + d;
-        out[0] = from_float<T>(o.x * inv); out[1] = from_float<T>(o.y * inv); out[2] = from_float<T>(o.z * inv); out[3] = from_float<T>(o.w * inv);
+        store4<T>((T*)a.out + (size_t)to * a.dim + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     }
     if (tid == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
@@ -1088,8 +1082,7 @@ __global__ __launch_bounds__(256) void attend_join_few_kernel(AttendArgs a, Part
         o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = (T*)a.out + to * a.dim + d;
-    out[0] = from_float<T>(o.x * inv); out[1] = from_float<T>(o.y * inv); out[2] = from_float<T>(o.z * inv); out[3] = from_float<T>(o.w * inv);
+    store4<T>((T*)a.out + to * a.dim + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     if (d == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
@@ -1109,7 +1102,10 @@ template <class T> void launch_attend(const AttendArgs& a, const Cut& cut, uint3
     auto by_size = [&](auto codes, auto dp) {
         constexpr int kTileMt = dp.value <= 128 ? 2 : 1;
         if (cut.tiles) {
-            hipLaunchKernelGGL((attend_tile_kernel<T, codes.value, dp.value, kTileMt, dp.value <= 128 ? 2 : 1>), grid, dim3(256), 0, stream, a, parts, q_vec);
+            auto tiles = [&](auto mt) {
+                hipLaunchKernelGGL((attend_tile_kernel<T, codes.value, dp.value, mt.value, dp.value <= 128 ? 2 : 1>), grid, dim3(256), 0, stream, a, parts, q_vec);
+            };
+            tiles(std::integral_constant<int, kTileMt>{});
         } else if (dp.value <= 128 && cut.mt == 2) {
             if constexpr (dp.value <= 128) rows(codes, dp, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
         } else if (cut.waves == 1) {

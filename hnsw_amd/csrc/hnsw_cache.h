@@ -50,11 +50,21 @@ __device__ __forceinline__ float to_float(bf16 x) { return __uint_as_float((uint
 template <class T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ _Float16 from_float<_Float16>(float x) { return (_Float16)x; }
-template <> __device__ __forceinline__ bf16 from_float<bf16>(float x)
+template <> __device__ __forceinline__ bf16 from_float<bf16>(float x) { return bf16{__builtin_bit_cast(uint16_t, (__bf16)x)}; }
+
+// Two values as two 16-bit ones in a word (rounded to nearest, ties to even).
+template <class T> __device__ __forceinline__ uint32_t pack2(float x, float y)
 {
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return bf16{(uint16_t)((u >> 16) | 0x40u)};       // NaN stays NaN
-    return bf16{(uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16)};                       // round to nearest, ties to even
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (std::is_same_v<T, bf16>) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2));
+}
+// Four consecutive outputs (the address is a multiple of 8 bytes).
+template <class T> __device__ __forceinline__ void store4(T* to, float a, float b, float c, float d)
+{
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to) = make_float4(a, b, c, d);
+    else *reinterpret_cast<u32x2*>(to) = u32x2{pack2<T>(a, b), pack2<T>(c, d)};
 }
 
 // Eight consecutive elements of a row; VEC: the address is a multiple of 16 bytes.

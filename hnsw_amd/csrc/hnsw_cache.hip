@@ -323,16 +323,8 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
         for (int j = 0; j < 4; j++) { x[j] = lo[j] * s; x[j + 4] = hi[j] * s; }
     }
     T* to = out + row * a.dim + col;
-    if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        u32x4 w;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            w[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(x[2 * j])) | ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(x[2 * j + 1])) << 16);
-        *reinterpret_cast<u32x4*>(to) = w;
-    }
+    store4<T>(to, x[0], x[1], x[2], x[3]);
+    store4<T>(to + 4, x[4], x[5], x[6], x[7]);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
