@@ -102,14 +102,10 @@ __device__ __forceinline__ Span rows_of(const AttendArgs& a, uint32_t b)
     const int64_t lo = min(max((int64_t)a.cu_q[b], (int64_t)0), (int64_t)a.n_rows), hi = min(max((int64_t)a.cu_q[b + 1], lo), (int64_t)a.n_rows);
     return {(uint32_t)lo, (uint32_t)(hi - lo)};
 }
-__device__ __forceinline__ Span uniform(Span s)                 // the same in all lanes: say so
-{
-    return {(uint32_t)__builtin_amdgcn_readfirstlane(s.first), (uint32_t)__builtin_amdgcn_readfirstlane(s.count)};
-}
-__device__ __forceinline__ uint32_t length_of(const AttendArgs& a, uint32_t b)
+__device__ __forceinline__ uint32_t length_of(const AttendArgs& a, int32_t len)
 {
     const int64_t cap = (int64_t)a.width * a.block_tokens;
-    return (uint32_t)min(max((int64_t)a.lens[b], (int64_t)0), cap);
+    return (uint32_t)min(max((int64_t)len, (int64_t)0), cap);
 }
 // tokens that row i of a request's n rows sees
 __device__ __forceinline__ uint32_t seen_by(const AttendArgs& a, uint32_t len, uint32_t n, uint32_t i)
@@ -119,25 +115,27 @@ __device__ __forceinline__ uint32_t seen_by(const AttendArgs& a, uint32_t len, u
     return (uint32_t)min(max(s, (int64_t)0), (int64_t)len);
 }
 
-// Unit u of the rows cut into tiles of `tile` (row, head) pairs, request after request: its request and the tile within it; false
-// when there are fewer units.
-__device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_t group, uint32_t tile, uint32_t lane, uint32_t& request, uint32_t& part)
+// Unit u of the rows cut into tiles of `tile` (row, head) pairs, request after request: its request, that request's rows, and the tile
+// within it; false when there are fewer units.
+__device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_t group, uint32_t tile, uint32_t lane, uint32_t& request, Span& rows, uint32_t& part)
 {
     if (!a.cu_q) {
         const uint32_t per = (group + tile - 1) / tile;
         request = u / per;
         part = u - request * per;
+        rows = {request, 1};
         return request < a.n_requests;
     }
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.n_requests; b0 += 64) {
-        uint32_t n = 0;
-        if (b0 + lane < a.n_requests) n = (uint32_t)(((uint64_t)rows_of(a, b0 + lane).count * group + tile - 1) / tile);
-        const uint32_t upto = wave_inclusive_sum(n);
+        Span s{0, 0};
+        if (b0 + lane < a.n_requests) s = rows_of(a, b0 + lane);
+        const uint32_t n = (uint32_t)(((uint64_t)s.count * group + tile - 1) / tile), upto = wave_inclusive_sum(n);
         const unsigned long long m = __ballot(before + upto > u);
         if (m) {
             const int at = __builtin_ctzll(m);
             request = b0 + at;
+            rows = {(uint32_t)__builtin_amdgcn_readlane(s.first, at), (uint32_t)__builtin_amdgcn_readlane(s.count, at)};
             part = u - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
             return true;
         }
@@ -253,8 +251,8 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
         count = 1;
     } else {
         uint32_t part;
-        if (!unit_of(a, unit, group, 16 * MT, lane, b, part)) return;
-        const Span s = uniform(rows_of(a, b));
+        Span s;
+        if (!unit_of(a, unit, group, 16 * MT, lane, b, s, part)) return;
         first = s.first;
         count = s.count;
         r0 = part * 16 * MT;
@@ -262,17 +260,9 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     const uint32_t n_r = count * group;                         // (fits: n_rows * q_heads < 2^24)
     if (r0 >= n_r) return;
 
-    // the rows of this lane's columns: their queries, and what they see
-    RawQuery<T, KS> raw[MT];
-    uint32_t seen[MT], least = 0xffffffffu, most = 0;
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const uint32_t r = r0 + 16 * mt + m;
-        const bool there = r < n_r;
-        const uint32_t i = there ? r / group : 0, h = head * group + (there ? r - i * group : 0);
-        load_query<T, KS>(a, there, first + i, h, q_vec, [&](int s) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); }, raw[mt]);
-    }
-    // the first table's block numbers, or ids: asked for before the length is there to say how many count
+    // the length, the first table's block numbers (or ids) and the queries, asked for together (loads come back in order, and the queries
+    // are needed last)
+    const int32_t len_raw = a.lens[b];
     const uint32_t begin = split * parts.chunk;
     uint32_t early[kMine];
 #pragma unroll
@@ -286,7 +276,17 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
             if (tid < kEntries && i < a.width) early[e] = (uint32_t)a.table[(size_t)b * a.width + i];
         }
     }
-    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
+    // the rows of this lane's columns: their queries, and what they see
+    RawQuery<T, KS> raw[MT];
+    uint32_t seen[MT], least, most;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const uint32_t r = r0 + 16 * mt + m;
+        const bool there = r < n_r;
+        const uint32_t i = there ? r / group : 0, h = head * group + (there ? r - i * group : 0);
+        load_query<T, KS>(a, there, first + i, h, q_vec, [&](int s) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); }, raw[mt]);
+    }
+    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, len_raw));
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
         const uint32_t r = r0 + 16 * mt + m;
@@ -696,10 +696,14 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
     const uint32_t group = a.q_heads / a.n_heads;
     constexpr uint32_t kRows = kWaves * 16 * MT;
     uint32_t b, part;
-    if (!unit_of(a, unit, group, kRows, lane, b, part)) return;
-    const Span rows = uniform(rows_of(a, b));
+    Span rows;
+    if (!unit_of(a, unit, group, kRows, lane, b, rows, part)) return;
     const uint32_t n_r = rows.count * group, r0 = part * kRows + wave * 16 * MT;
-    // queries and the first table's block numbers: asked for before the length is there
+    // the length, the first table's block numbers and the queries, asked for together (loads come back in order, and the queries are
+    // needed last)
+    const int32_t len_raw = a.lens[b];
+    const uint32_t begin = split * parts.chunk, e_begin = begin >> bs_log;
+    const uint32_t early = e_begin + tid < a.width ? (uint32_t)a.table[(size_t)b * a.width + e_begin + tid] : ~0u;
     RawQuery<T, KS> raw[MT];
     uint32_t seen[MT];
 #pragma unroll
@@ -710,9 +714,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
         seen[mt] = i;
         load_query<T, KS>(a, there, rows.first + i, h, q_vec, [&](int s) { return 32 * s + 8 * g; }, raw[mt]);
     }
-    const uint32_t begin = split * parts.chunk, e_begin = begin >> bs_log;
-    const uint32_t early = e_begin + tid < a.width ? (uint32_t)a.table[(size_t)b * a.width + e_begin + tid] : ~0u;
-    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, b));
+    const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, len_raw));
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) seen[mt] = r0 + 16 * mt + m < n_r ? seen_by(a, len, rows.count, seen[mt]) : 0;
     // (rows follow one another in what they see; a wavefront without rows sees nothing)
@@ -996,7 +998,7 @@ __device__ __forceinline__ uint32_t chunks_of(const AttendArgs& a, const Partial
 {
     if (a.found) return parts.n_splits;
     const Span s = rows_of(a, b);
-    const uint32_t sees = seen_by(a, length_of(a, b), s.count, row - s.first);
+    const uint32_t sees = seen_by(a, length_of(a, a.lens[b]), s.count, row - s.first);
     return min(parts.n_splits, (uint32_t)(((uint64_t)sees + parts.chunk - 1) / parts.chunk));
 }
 
