@@ -2,3 +2,4 @@
 from .cache import Plan, TokenCache, cache_plan  # noqa: F401
 from .flatgraph import FlatGraph  # noqa: F401
 from .index import HNSW, Neighbors  # noqa: F401
+from .memory import TokenMemory  # noqa: F401
