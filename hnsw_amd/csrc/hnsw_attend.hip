@@ -59,6 +59,7 @@ static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_
         chunk = std::min<uint64_t>(total / 768, 4096);
         chunk = std::max<uint64_t>((chunk + 127) / 128 * 128, 128);
     }
+    chunk = std::max<uint64_t>(chunk, ((uint64_t)items / 32768 + 127) / 128 * 128);      // (the chunks are a grid's second extent, below 2^16)
     c.chunk = (uint32_t)std::min<uint64_t>(chunk, 0x80000000ull);
     c.n_splits = std::max<uint32_t>(1, (uint32_t)(((uint64_t)items + c.chunk - 1) / c.chunk));
     return c;
@@ -104,7 +105,7 @@ void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows,
     const uint64_t need = workspace_of(cut, n_rows, q_heads, c->dim);
     if (need > workspace_bytes || (need && !workspace)) throw std::invalid_argument(std::string(who) + ": the workspace is too small");
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) throw std::invalid_argument(std::string(who) + ": the workspace must be aligned to 16 bytes");
-    if ((uint64_t)cut.units * cut.heads >= 1ull << 24 || cut.n_splits > 65535u) throw std::invalid_argument(std::string(who) + ": too much work for one call");
+    if ((uint64_t)cut.units * cut.heads >= 1ull << 24) throw std::invalid_argument(std::string(who) + ": too much work for one call");
     const OnDevice on(device);
     if (row_type == HNSW_AMD_TYPE_F32) launch_attend<float>(a, cut, c->codes, (float*)workspace, (hipStream_t)stream);
     else if (row_type == HNSW_AMD_TYPE_F16) launch_attend<_Float16>(a, cut, c->codes, (float*)workspace, (hipStream_t)stream);

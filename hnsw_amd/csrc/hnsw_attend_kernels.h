@@ -384,10 +384,10 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t start = min(c0 + 32 * j + 16 * h, c1 - 1);
-                uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
-                if (base == ~0u) base = safe;                   // (stale codes can be NaN, which a weight of 0 would not remove)
-                w.at[h] = (uint64_t)(base + (start & (bs - 1))) * dim;
-                w.limit[h] = min(c1 - 1 - start, 15u);
+                const uint32_t base = __builtin_amdgcn_readfirstlane(ent_row[(start >> bs_log) - e0]);
+                // (no block: one live token over and over; stale codes can be NaN, which a weight of 0 would not remove)
+                w.at[h] = (uint64_t)(base == ~0u ? safe : base + (start & (bs - 1))) * dim;
+                w.limit[h] = base == ~0u ? 0u : min(c1 - 1 - start, 15u);
             }
         }
         return w;
@@ -482,9 +482,8 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
             __syncthreads();
 #pragma unroll
             for (int w = 0; w < NW; w++) largest = fmaxf(largest, red[w]);
-            const float per_v = largest > 0.0f ? kPScale / largest : 0.0f;
-            if (largest > 0.0f) {
-                if (unit_v > 0.0f && unit_v != largest) {       // outputs so far are in units of the last table's largest scale
+            if (largest > unit_v) {                             // outputs are in units of the largest scale so far
+                if (unit_v > 0.0f) {                            // (never the other way: outputs in units of a block of zeros' scale would overflow)
                     const float change = unit_v / largest;
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
@@ -493,6 +492,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
                 }
                 unit_v = largest;
             }
+            const float per_v = unit_v > 0.0f ? kPScale / unit_v : 0.0f;
 
             auto take = [&](auto buf, uint32_t j) {
                 const uint32_t i0 = 32 * j, ahead = j + DEPTH * NW;
@@ -749,17 +749,19 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
 #pragma unroll
     for (int i = 0; i < VL; i++) v_off[i] = v_row * dim + (4 * (v_word + 32 * i) < dim ? 4 * (v_word + 32 * i) : 0);
     // The next tile's codes: this wavefront's keys are 16 tokens of one block, its values the octets of two runs of 16 tokens.  (Tokens
-    // behind the last one are the last one; those of no block are some live token: stale codes can be NaN, which a weight of 0 would
-    // not remove.)
+    // behind the last one are the last one; those of no block are one live token over and over: stale codes can be NaN, which a weight
+    // of 0 would not remove.)
     auto fetch = [&](uint32_t t0) {
         const uint32_t last = c1 - 1, kt = min(t0 + 16 * wave, last), vt0 = min(t0 + 32 * (wave >> 1), last), vt1 = min(t0 + 32 * (wave >> 1) + 16, last);
-        const uint32_t ek = ent_row[(kt >> bs_log) - e0], ev0 = ent_row[(vt0 >> bs_log) - e0], ev1 = ent_row[(vt1 >> bs_log) - e0];
-        auto codes_at = [&](const uint8_t* codes, uint32_t entry, uint32_t pos) {
-            const uint32_t base = __builtin_amdgcn_readfirstlane(entry);
-            return codes + (uint64_t)((base == ~0u ? safe : base) + (pos & (bs - 1))) * dim;
+        uint32_t ek = ent_row[(kt >> bs_log) - e0], ev0 = ent_row[(vt0 >> bs_log) - e0], ev1 = ent_row[(vt1 >> bs_log) - e0];
+        ek = __builtin_amdgcn_readfirstlane(ek);
+        ev0 = __builtin_amdgcn_readfirstlane(ev0);
+        ev1 = __builtin_amdgcn_readfirstlane(ev1);
+        auto codes_at = [&](const uint8_t* codes, uint32_t base, uint32_t pos) {
+            return codes + (uint64_t)(base == ~0u ? safe : base + (pos & (bs - 1))) * dim;
         };
         const uint8_t *kb = codes_at(a.k_codes, ek, kt), *vb0 = codes_at(a.v_codes, ev0, vt0), *vb1 = codes_at(a.v_codes, ev1, vt1);
-        if (t0 + kTokens <= c1) {
+        if (t0 + kTokens <= c1 && ek != ~0u && ev0 != ~0u && ev1 != ~0u) {
 #pragma unroll
             for (int i = 0; i < KL; i++) kr[i] = *reinterpret_cast<const u32x4*>(kb + k_off[i]);
 #pragma unroll
@@ -770,7 +772,8 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                     vr[i][4 + r] = *reinterpret_cast<const uint32_t*>(vb1 + (size_t)r * dim + v_off[i]);
                 }
         } else {
-            const uint32_t k_back = k_row - min(k_row, last - kt);                  // rows that are not there
+            const uint32_t k_back = k_row - min(k_row, ek == ~0u ? 0u : last - kt);                 // rows that are not there
+            const uint32_t v_left0 = ev0 == ~0u ? 0u : last - vt0, v_left1 = ev1 == ~0u ? 0u : last - vt1;
 #pragma unroll
             for (int i = 0; i < KL; i++) kr[i] = *reinterpret_cast<const u32x4*>(kb + (k_off[i] - k_back * dim));
 #pragma unroll
@@ -778,8 +781,8 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const uint32_t row = v_row + r;
-                    vr[i][r] = *reinterpret_cast<const uint32_t*>(vb0 + (v_off[i] - v_row * dim + min(row, last - vt0) * dim));
-                    vr[i][4 + r] = *reinterpret_cast<const uint32_t*>(vb1 + (v_off[i] - v_row * dim + min(row, last - vt1) * dim));
+                    vr[i][r] = *reinterpret_cast<const uint32_t*>(vb0 + (v_off[i] - v_row * dim + min(row, v_left0) * dim));
+                    vr[i][4 + r] = *reinterpret_cast<const uint32_t*>(vb1 + (v_off[i] - v_row * dim + min(row, v_left1) * dim));
                 }
         }
     };
@@ -931,12 +934,8 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
             if (lane == 0) red[wave] = largest;
             __syncthreads();
             largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-            if (tid <= ((c1 - 1) >> bs_log) - e0) {
-                const float w = largest > 0.0f ? fmaxf(sv * (kPScale / largest), 0x1p-60f) : 1.0f;
-                ent[tid] = make_float4(sk, __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
-            }
-            if (largest > 0.0f) {
-                if (unit_v > 0.0f && unit_v != largest) {       // outputs so far are in units of the last table's largest scale
+            if (largest > unit_v) {                             // outputs are in units of the largest scale so far
+                if (unit_v > 0.0f) {
                     const float change = unit_v / largest;
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
@@ -944,6 +943,10 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Parti
                         for (int i = 0; i < DT; i++) o[mt][i] *= change;
                 }
                 unit_v = largest;
+            }
+            if (tid <= ((c1 - 1) >> bs_log) - e0) {
+                const float w = unit_v > 0.0f ? fmaxf(sv * (kPScale / unit_v), 0x1p-60f) : 1.0f;
+                ent[tid] = make_float4(sk, __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
             }
             store(0);
             __syncthreads();

@@ -395,6 +395,110 @@ def test_blocks_that_are_none(codes):
     _compare(s, rows, out, lse, lambda r, h: (owner[r], np.arange(lens[owner[r]] - new[owner[r]] + r - cu[owner[r]] + 1)), 64 ** -0.5)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 192])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_blocks_that_are_none_before_one_that_is_begun(dim, dtype):
+    """The only block that exists holds few tokens; what lies behind those (codes that are NaN) does not reach the outputs, though tokens of
+    no block read something."""
+    lens, block = [2 * 128 + 5, 70], 128
+    s = Setup(lens, 2, block, dim, E4)
+    s.table[0, :2] = torch.tensor([-1, 10 ** 6])
+    s.d_table = s.table.cuda()
+    q = _queries(2, 4, dim, dtype)
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens)
+    _compare(s, q, out, lse, lambda r, h: (r, np.arange(lens[r])), dim ** -0.5)
+    for new in ([30, 0], [100, 60]):                                 # in registers, and through LDS
+        rows, cu = _queries(sum(new), 4, dim, dtype), np.concatenate([[0], np.cumsum(new)])
+        out, lse = s.cache.attend(rows, s.d_table, s.d_lens, cu_q=_gpu(cu))
+        owner = np.repeat(np.arange(2), new)
+        _compare(s, rows, out, lse, lambda r, h: (owner[r], np.arange(lens[owner[r]] - new[owner[r]] + r - cu[owner[r]] + 1)), dim ** -0.5)  # noqa: B023
+
+
+@pytest.mark.parametrize("codes", [I8, E4])
+def test_tables_whose_values_are_zeros(codes):
+    """Blocks of zeros have the least scale there is, 2^-100; behind thousands of other tokens they fill a table of their own."""
+    lens, dim = [14000], 64
+    s = Setup(lens, 1, 16, dim, codes)
+    vs = s.cache.v_scale.cpu() * 2.0 ** 20
+    s.largest *= 2.0 ** 20
+    zeros = s.table[0, 256:256 * 3].long()
+    s.cache.v_codes.view(torch.int8)[zeros.cuda()] = 0
+    vs[zeros] = 2.0 ** -100
+    s.cache.v_scale.copy_(vs)
+    s.v64 = s.cache.v_codes.cpu().double() * vs.double()[:, :, None, None]
+    for rows in (1, 300):                                            # (a hint of one token: nothing is cut)
+        q = _queries(rows, 8, dim, BF16)
+        cu = None if rows == 1 else _gpu([0, rows])
+        out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=cu, max_len=1)
+        _compare(s, q, out, lse, lambda r, h: (0, np.arange(lens[0] - rows + r + 1)), dim ** -0.5, pick=[0, rows - 1])  # noqa: B023
+    # lists of 1024 entries and more: first the others, then zeros, and the other way
+    some = np.random.default_rng(0)
+    full, none = some.permutation(4096)[:1024], 4096 + some.permutation(8000)[:1024]
+    ids = np.stack([np.concatenate([full, none]), np.concatenate([none, full])])[None].repeat(800, 0).astype(np.int32)
+    q = _queries(800, 2, dim, BF16)
+    s1 = s.cache.attend_found(q, s.d_table, s.d_lens, _gpu(ids), cu_q=_gpu([0, 800]), causal=False)
+    _compare(s, q, *s1, lambda r, h: (0, ids[r, h]), dim ** -0.5, pick=[0, 17, 799])
+
+
+def test_every_row_in_one_of_as_many_requests():
+    """As many rows as requests, but not one each."""
+    lens = [40, 90, 7, 1, 0]
+    s = Setup(lens, 1, 16, 64, I8)
+    q = _queries(5, 20, 64, BF16)
+    for cu in ([0, 0, 5, 5, 5, 5], [0, 2, 2, 2, 5, 5], [0, 0, 0, 0, 0, 5]):
+        owner = np.searchsorted(cu, np.arange(5), side="right") - 1
+        out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=_gpu(cu))
+        see = lambda r: max(0, lens[owner[r]] - (cu[owner[r] + 1] - cu[owner[r]]) + r - cu[owner[r]] + 1)  # noqa: E731, B023
+        _compare(s, q, out, lse, lambda r, h: (owner[r], np.arange(see(r))), 64 ** -0.5)
+
+
+def test_queries_that_are_not_numbers_stay_alone():
+    """A row with a NaN or an infinity gives no number, and its neighbours in the same tile what they give without it."""
+    s = Setup([300], 1, 16, 64, I8)
+    for rows in (16, 200):
+        q = _queries(rows, 2, 64, BF16)
+        want, want_lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=_gpu([0, rows]))
+        bad = q.clone()
+        bad[3, 1, 5], bad[9, 0, 0] = float("nan"), float("inf")
+        out, lse = s.cache.attend(bad, s.d_table, s.d_lens, cu_q=_gpu([0, rows]))
+        for r, h in ((3, 1), (9, 0)):
+            assert bool(out[r, h].isnan().all()) and bool(lse[r, h].isnan())
+            out[r, h], lse[r, h] = want[r, h], want_lse[r, h]
+        assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -7, atol=1e-3) and torch.allclose(lse, want_lse, rtol=1e-5, atol=1e-5)
+
+
+def test_a_table_of_a_hundred_million_tokens():
+    """The lengths are not known to the host, and the table is as wide as it may be."""
+    s = Setup([700, 20], 1, 256, 64, I8, width=(2 ** 31 - 1) // 256)
+    q = _queries(2, 2, 64, BF16)
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens)
+    _compare(s, q, out, lse, lambda r, h: (r, np.arange(s.lens[r])), 64 ** -0.5)
+
+
+def test_rows_behind_the_last_request_are_left_as_they_are():
+    s = Setup([300, 20], 2, 16, 64, I8)
+    for new, total in (([3, 2], 9), ([200, 10], 260)):
+        q, cu = _queries(total, 4, 64, BF16), _gpu(np.concatenate([[0], np.cumsum(new)]))
+        ids = _gpu(np.random.default_rng(1).integers(0, 300, (total, 2, 1500)).astype(np.int32))
+        for found in (False, True):
+            out, lse = torch.full((total, 4, 64), 7.0, dtype=BF16, device="cuda"), torch.full((total, 4), 7.0, device="cuda")
+            c = s.cache
+            desc = capi.TokenCacheC(c.k_codes.data_ptr(), c.v_codes.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.n_blocks, c.n_heads, c.block_tokens, c.dim, capi.CODES_I8)
+            L, at = capi.lib(), ctypes.byref(desc)
+            front = (at, q.data_ptr(), total, 4, q.stride(0), q.stride(1), capi.TYPE_BF16, s.d_table.data_ptr(), s.d_table.shape[1], s.d_lens.data_ptr(), 2, cu.data_ptr(), 1)
+            if found:
+                bytes_ = L.hnsw_amd_cache_attend_found_workspace(at, total, 4, 2, 1500)
+                work = torch.empty(max(bytes_, 16), dtype=torch.uint8, device="cuda")
+                rc = L.hnsw_amd_cache_attend_found_device(*front, ids.data_ptr(), 2, 1500, 0.125, out.data_ptr(), lse.data_ptr(), work.data_ptr(), bytes_, 0, torch.cuda.current_stream().cuda_stream)
+            else:
+                bytes_ = L.hnsw_amd_cache_attend_workspace(at, total, 4, 2, s.d_table.shape[1], 0)
+                work = torch.empty(max(bytes_, 16), dtype=torch.uint8, device="cuda")
+                rc = L.hnsw_amd_cache_attend_device(*front, 0.125, 0, out.data_ptr(), lse.data_ptr(), work.data_ptr(), bytes_, 0, torch.cuda.current_stream().cuda_stream)
+            capi.check(rc)
+            n = sum(new)
+            assert bool((out[n:] == 7.0).all()) and bool((lse[n:] == 7.0).all()) and not bool((lse[:n] == 7.0).any())
+
+
 def test_lengths_that_are_none():
     """A negative length counts as 0, one beyond the table as the table's end."""
     s = Setup([64, 64, 64], 1, 16, 64, I8)
@@ -554,6 +658,55 @@ def test_a_decoding_step_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
         assert torch.equal(caught["lens"], eager["lens"]) and torch.equal(caught["table"], eager["table"])
         assert torch.isfinite(want[0]).all() and want[0].abs().sum() > 0
+
+
+def test_a_plan_of_many_requests_captured():
+    """The largest call there is, in a graph that is replayed with other lengths."""
+    n, block, rng = 8192, 16, random.Random(5)
+    lens = [rng.randint(0, 40) for _ in range(n)]
+    d = dict(lens=_gpu(lens), grow=_gpu([0] * n), table=torch.full((n, 6), -1, dtype=torch.int32, device="cuda"), ring=torch.arange(4 * n, dtype=torch.int32).cuda(),
+             state=_gpu([0, 4 * n], torch.int64))
+    plan_ = lambda: cache_plan(d["lens"], d["grow"], d["table"], d["ring"], d["state"], block_tokens=block, n_slots=3 * n)  # noqa: E731
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p = plan_()
+    table, ring, state = [[-1] * 6 for _ in range(n)], list(range(4 * n)), [0, 4 * n]
+    lens = [0] * n
+    for step in range(4):
+        grow = [rng.randint(0, 3) if rng.random() < 0.9 or not step else -1 for _ in range(n)]
+        d["lens"].copy_(_gpu(lens))
+        d["grow"].copy_(_gpu(grow))
+        d["state"].copy_(_gpu(state, torch.int64))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        slots, cu, lens, state, status, table, ring = ref.plan(lens, grow, table, ring, state, block, 3 * n)
+        assert p.status.item() == status == 0 and p.slots.tolist() == slots and p.cu_new.tolist() == cu and p.lens.tolist() == lens
+        assert p.state.tolist() == state and d["table"].tolist() == table and d["ring"].tolist() == ring
+
+
+def test_two_graphs_of_split_work_at_once():
+    """Each graph has a workspace of its own, so that their replays may overlap."""
+    s = Setup([5000, 3000], 2, 32, 128, I8)
+    q = [_queries(2, 4, 128, BF16, seed=i) for i in range(2)]
+    want = [s.cache.attend(x, s.d_table, s.d_lens, max_len=20000) for x in q]
+    graphs, outs = [], []
+    for x in q:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(s.cache.attend(x, s.d_table, s.d_lens, max_len=20000))
+    streams = [torch.cuda.Stream() for _ in q]
+    for _ in range(5):
+        for o in outs:
+            o[0].zero_()
+            o[1].zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
 
 
 def test_python_refuses():
