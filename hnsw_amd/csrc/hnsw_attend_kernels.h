@@ -674,7 +674,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
 // into the exponent instead of being multiplied in: weights are 2^(score - maximum + log2 of the scale over the table's largest), their
 // sum is put right by the inverse per 16 tokens.
 template <class T, int CODES, int DP, int MT, int NBUF>
-__global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
+__global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
 {
     constexpr int KS = DP / 32, DT = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
     constexpr int kTokens = 64, kKeyLd = DP + 8;                 // 16-bit elements
@@ -1105,12 +1105,12 @@ template <class T> void launch_attend(const AttendArgs& a, const Cut& cut, uint3
         else hipLaunchKernelGGL((attend_rows_kernel<T, codes.value, dp.value, mt.value, nw.value, false>), grid, dim3(64 * nw.value), 0, stream, a, parts, cut.heads, q_vec);
     };
     auto by_size = [&](auto codes, auto dp) {
-        constexpr int kTileMt = dp.value <= 128 ? 2 : 1;
         if (cut.tiles) {
             auto tiles = [&](auto mt) {
                 hipLaunchKernelGGL((attend_tile_kernel<T, codes.value, dp.value, mt.value, dp.value <= 128 ? 2 : 1>), grid, dim3(256), 0, stream, a, parts, q_vec);
             };
-            tiles(std::integral_constant<int, kTileMt>{});
+            if (dp.value <= 128 && cut.mt == 2) tiles(std::integral_constant<int, dp.value <= 128 ? 2 : 1>{});
+            else tiles(std::integral_constant<int, 1>{});
         } else if (dp.value <= 128 && cut.mt == 2) {
             if constexpr (dp.value <= 128) rows(codes, dp, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
         } else if (cut.waves == 1) {

@@ -395,6 +395,19 @@ def test_blocks_that_are_none(codes):
     _compare(s, rows, out, lse, lambda r, h: (owner[r], np.arange(lens[owner[r]] - new[owner[r]] + r - cu[owner[r]] + 1)), 64 ** -0.5)
 
 
+@pytest.mark.parametrize("dim,codes,dtype,causal", [(16, I8, F32, True), (64, E4, BF16, True), (80, I8, F16, True), (128, I8, BF16, True), (128, E4, F32, False), (112, E4, F16, False), (96, I8, BF16, True)])
+def test_many_rows_cut_for_longer_requests_than_there_are(dim, codes, dtype, causal):
+    """The table is for 20000 tokens and the host knows no lengths: 128 rows a workgroup and chunks that most requests do not reach."""
+    lens, new = [130, 1500, 64, 0, 601], [40, 200, 64, 3, 1]
+    s = Setup(lens, 2, 16, dim, codes, width=1250)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    owner = np.repeat(np.arange(5), new)
+    q = _queries(int(cu[-1]), 6, dim, dtype)
+    see = lambda r: max(0, lens[owner[r]] - new[owner[r]] + r - cu[owner[r]] + 1) if causal else lens[owner[r]]  # noqa: E731
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=_gpu(cu), causal=causal)
+    _compare(s, q, out, lse, lambda r, h: (owner[r], np.arange(see(r))), dim ** -0.5)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 192])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_blocks_that_are_none_before_one_that_is_begun(dim, dtype):
