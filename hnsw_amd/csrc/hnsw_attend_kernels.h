@@ -670,26 +670,31 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
 // [dim][token] (the eight tokens of a matrix operand next to each other, the pieces of a row in an order that differs by row to
 // the same end), while the next tile's codes are on their way to registers: each wavefront moves the keys of 16 tokens and a quarter
 // of the values' octets, so that the blocks they lie in are scalars.
+// HALVES = 2: twice the wavefronts, which take the tiles in turn and join at the end: half the steps of one after the other where
+// workgroups are too few to hide them.  (Up to 64 dims, where two such workgroups fit a compute unit: 163 rows each of eight requests over
+// 1000 tokens, 16 heads, 37.4 -> 34.3 us.  At 128 dims only one fits, and the rounds cost more than the steps: 300 rows each of four over 700
+// tokens, 43.8 -> 51.3.)
 // Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel, but that a block's value scale goes
 // into the exponent instead of being multiplied in: weights are 2^(score - maximum + log2 of the scale over the table's largest), their
 // sum is put right by the inverse per 16 tokens.
-template <class T, int CODES, int DP, int MT, int NBUF>
-__global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
+template <class T, int CODES, int DP, int MT, int NBUF, int HALVES>
+__global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
 {
     constexpr int KS = DP / 32, DT = DP / 16, QT = kQTerms<T>, PT = kPTerms<T>;
     constexpr int kTokens = 64, kKeyLd = DP + 8;                 // 16-bit elements
     constexpr int KL = DP / 64, VL = (DP + 127) / 128;          // 16-byte pieces of keys, and words x 8 tokens of values, that a thread moves
     constexpr uint32_t kEntries = kScanTokens / 16 + 1;
-    static_assert(kScanTokens / 16 <= 256);
-    __shared__ uint32_t ent_row[kEntries], some[kWaves];        // first row of a block's codes, in rows of dim bytes; ~0: of no block
-    __shared__ float red[kWaves];
+    static_assert(kScanTokens / 16 <= 256 && (HALVES == 1 || NBUF == 2));
+    constexpr int kAll = kWaves * HALVES;                       // wavefronts
+    __shared__ uint32_t ent_row[kEntries], some[kAll];        // first row of a block's codes, in rows of dim bytes; ~0: of no block
+    __shared__ float red[kAll];
     __shared__ __align__(16) float4 ent[kEntries];              // key scale, log2 of the weights' factor, its inverse; key scale -1: there is no block
-    __shared__ __align__(16) _Float16 keys[NBUF][kTokens * kKeyLd];
-    __shared__ __align__(16) _Float16 vals[NBUF][DP * kTokens];
+    __shared__ __align__(16) _Float16 keys[NBUF * HALVES][kTokens * kKeyLd];
+    __shared__ __align__(16) _Float16 vals[NBUF * HALVES][DP * kTokens];
     auto val_at = [](uint32_t d, uint32_t oct) { return d * kTokens + 8 * (oct ^ ((d >> 1) & 7)); };
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t of_all = __builtin_amdgcn_readfirstlane(tid >> 6), wave = of_all % kWaves, half = of_all / kWaves;
     const uint32_t kv = blockIdx.x % a.n_heads, split = blockIdx.y;
     const uint32_t unit = gridDim.x / a.n_heads - 1 - blockIdx.x / a.n_heads;   // the last rows of a prompt see the most: first
     const uint32_t dim = a.dim, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs);
@@ -703,7 +708,7 @@ __global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_
     // needed last)
     const int32_t len_raw = a.lens[b];
     const uint32_t begin = split * parts.chunk, e_begin = begin >> bs_log;
-    const uint32_t early = e_begin + tid < a.width ? (uint32_t)a.table[(size_t)b * a.width + e_begin + tid] : ~0u;
+    const uint32_t early = tid < kEntries && e_begin + tid < a.width ? (uint32_t)a.table[(size_t)b * a.width + e_begin + tid] : ~0u;
     RawQuery<T, KS> raw[MT];
     uint32_t seen[MT];
 #pragma unroll
@@ -804,9 +809,9 @@ __global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_
 #pragma unroll
         for (int j = 0; j < kPieces; j++) store_piece(buf, j);
     };
-    auto compute = [&](uint32_t t0, int buf) {
-        if (t0 >= most) {                                   // none of this wavefront's rows sees the tile
-            if constexpr (NBUF == 2) store(buf ^ 1);
+    auto compute = [&](uint32_t t0, int buf, int other) {
+        if (t0 >= most || (HALVES == 2 && t0 >= c1)) {                                   // none of this wavefront's rows sees the tile
+            if constexpr (NBUF == 2) store(other);
             return;
         }
         float4 x[4];
@@ -900,7 +905,7 @@ __global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_
             meet(DT + i);
             if constexpr (NBUF == 2) {
 #pragma unroll
-                for (int j = i * kPieces / DT; j < (i + 1) * kPieces / DT; j++) store_piece(buf ^ 1, j);
+                for (int j = i * kPieces / DT; j < (i + 1) * kPieces / DT; j++) store_piece(other, j);
             }
         }
     };
@@ -913,16 +918,18 @@ __global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_
         bh = blk < a.n_blocks ? blk * a.n_heads + kv : ~0u;
         if (mine) ent_row[tid] = bh == ~0u ? ~0u : bh << bs_log;
         const unsigned long long fine = __ballot(bh != ~0u);
-        if (lane == 0) some[wave] = fine ? (__builtin_amdgcn_readlane(bh, __builtin_ctzll(fine)) << bs_log) + 1 : 0;
+        if (lane == 0) some[of_all] = fine ? (__builtin_amdgcn_readlane(bh, __builtin_ctzll(fine)) << bs_log) + 1 : 0;
         __syncthreads();
         safe = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) safe = safe ? safe : some[w];
+        for (int w = 0; w < kAll; w++) safe = safe ? safe : some[w];
         safe = __builtin_amdgcn_readfirstlane(safe);
         return safe-- != 0;
     };
     bool has = begin < end && open_table();                     // (the same in all threads)
-    if (has) fetch(c0);
+    // (with two halves of the wavefronts these take tiles in turn)
+    auto first_tile = [&]() { if (HALVES == 1 || c0 + half * kTokens < c1) fetch(c0 + half * kTokens); };
+    if (has) first_tile();
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
     while (c0 < end) {
@@ -931,9 +938,10 @@ __global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_
             // counts as 2^-60 of it: weights that vanish as 16-bit floats)
             const float sk = bh != ~0u ? a.k_scale[bh] : -1.0f, sv = bh != ~0u ? a.v_scale[bh] : 0.0f;
             float largest = wave_max_not_negative(sv);
-            if (lane == 0) red[wave] = largest;
+            if (lane == 0) red[of_all] = largest;
             __syncthreads();
-            largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+            for (int w = 0; w < kAll; w++) largest = fmaxf(largest, red[w]);
             if (largest > unit_v) {                             // outputs are in units of the largest scale so far
                 if (unit_v > 0.0f) {
                     const float change = unit_v / largest;
@@ -948,12 +956,14 @@ __global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_
                 const float w = unit_v > 0.0f ? fmaxf(sv * (kPScale / unit_v), 0x1p-60f) : 1.0f;
                 ent[tid] = make_float4(sk, __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
             }
-            store(0);
+            const int own = NBUF * half;                        // this half's buffers
+            store(own);
             __syncthreads();
             int buf = 0;
-            for (uint32_t t0 = c0; t0 < c1; t0 += kTokens) {
-                if (t0 + kTokens < c1) fetch(t0 + kTokens);
-                compute(t0, buf);
+            for (uint32_t first = c0; first < c1; first += HALVES * kTokens) {
+                const uint32_t t0 = first + half * kTokens, next = t0 + HALVES * kTokens;
+                if (next < c1) fetch(next);
+                compute(t0, own + buf, own + (buf ^ 1));
                 if constexpr (NBUF == 1) {                      // the only buffer is about to be overwritten
                     __syncthreads();
                     store(0);
@@ -967,7 +977,39 @@ __global__ __launch_bounds__(256, DP == 64 && MT == 1 ? 3 : 2) void attend_tile_
         if (c0 >= end) break;
         __syncthreads();                                        // the table's last readers are done
         has = open_table();
-        if (has) fetch(c0);
+        if (has) first_tile();
+    }
+
+    if constexpr (HALVES == 2) {
+        // the second half's softmaxes go to the first through the tiles' memory, lane by lane
+        constexpr int kLd = MT * (4 * DT + 2);
+        static_assert(sizeof(keys) >= 256 * kLd * 4);
+        float* mine = reinterpret_cast<float*>(&keys[0][0]) + wave * 64 + lane;
+        __syncthreads();
+        if (half == 1) {
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                mine[256 * (mt * (4 * DT + 2))] = top[mt];
+                mine[256 * (mt * (4 * DT + 2) + 1)] = sum[mt];
+#pragma unroll
+                for (int i = 0; i < DT; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) mine[256 * (mt * (4 * DT + 2) + 2 + 4 * i + r)] = o[mt][i][r];
+            }
+        }
+        __syncthreads();
+        if (half == 1) return;
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            const float there = mine[256 * (mt * (4 * DT + 2))], now = fmaxf(top[mt], there), ref = now == -__builtin_inff() ? 0.0f : now;
+            const float x = __builtin_amdgcn_exp2f(top[mt] - ref), y = __builtin_amdgcn_exp2f(there - ref);
+            top[mt] = now;
+            sum[mt] = sum[mt] * x + mine[256 * (mt * (4 * DT + 2) + 1)] * y;
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) o[mt][i][r] = o[mt][i][r] * x + mine[256 * (mt * (4 * DT + 2) + 2 + 4 * i + r)] * y;
+        }
     }
 
     const float unit_o = unit_v / kPScale;
@@ -1107,7 +1149,8 @@ template <class T> void launch_attend(const AttendArgs& a, const Cut& cut, uint3
     auto by_size = [&](auto codes, auto dp) {
         if (cut.tiles) {
             auto tiles = [&](auto mt) {
-                hipLaunchKernelGGL((attend_tile_kernel<T, codes.value, dp.value, mt.value, dp.value <= 128 ? 2 : 1>), grid, dim3(256), 0, stream, a, parts, q_vec);
+                constexpr int kHalves = mt.value == 1 && dp.value == 64 ? 2 : 1;
+                hipLaunchKernelGGL((attend_tile_kernel<T, codes.value, dp.value, mt.value, dp.value <= 128 ? 2 : 1, kHalves>), grid, dim3(256 * kHalves), 0, stream, a, parts, q_vec);
             };
             if (dp.value <= 128 && cut.mt == 2) tiles(std::integral_constant<int, dp.value <= 128 ? 2 : 1>{});
             else tiles(std::integral_constant<int, 1>{});
