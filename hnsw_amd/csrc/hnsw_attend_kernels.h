@@ -1048,21 +1048,31 @@ __device__ __forceinline__ uint32_t chunks_of(const AttendArgs& a, const Partial
 }
 
 // The chunks' outputs of a row and head become one: weights 2^(lse - largest).  One workgroup each: dim / 4 lanes take a chunk, so that
-// 256 / (dim / 4) chunks are read at a time.
+// 256 / (dim / 4) chunks are read at a time.  What bounds this is the chain of loads that wait for one another, so the first 8 chunks of
+// every lane are asked for before it is known how many there are (the workspace holds all of them; what was not written is not used).
+// (2 rows of 64 heads of 128 dims in 49 chunks: 5.1 us, 6.0 with the loads one after the other.)
 template <class T>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials parts)
 {
+    constexpr uint32_t kFirst = 8;
     __shared__ float red[kWaves], weight[256];
     __shared__ __align__(16) float4 out_s[256];
     const uint32_t tid = threadIdx.x, lane = tid & 63, to = blockIdx.x, row = to / a.q_heads;
-    const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
-    if (b >= a.n_requests) return;
-    const uint32_t n = chunks_of(a, parts, b, row);
     const float* lse = parts.lse + (size_t)to * parts.n_splits;
     const float* x = parts.out + (size_t)to * parts.n_splits * a.dim;
     const uint32_t lanes = a.dim / 4, per = 256 / lanes, mine = tid / lanes, d = (tid - mine * lanes) * 4;
-    float top = -__builtin_inff();
-    for (uint32_t i = tid; i < n; i += 256) top = fmaxf(top, lse[i]);
+    const float first_lse = tid < parts.n_splits ? lse[tid] : 0.0f;
+    float4 first[kFirst];
+#pragma unroll
+    for (uint32_t j = 0; j < kFirst; j++) {
+        const uint32_t i = mine + j * per;
+        first[j] = mine < per && i < parts.n_splits && i < 256 ? *reinterpret_cast<const float4*>(x + (size_t)i * a.dim + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
+    if (b >= a.n_requests) return;
+    const uint32_t n = chunks_of(a, parts, b, row);
+    float top = tid < n ? first_lse : -__builtin_inff();
+    for (uint32_t i = tid + 256; i < n; i += 256) top = fmaxf(top, lse[i]);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
     if (lane == 0) red[tid >> 6] = top;
@@ -1071,20 +1081,23 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials
     const float ref = top == -__builtin_inff() ? 0.0f : top;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f;
+    auto add = [&](float f, const float4& y) { o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w; };
     for (uint32_t i0 = 0; i0 < n; i0 += 256) {
-        const float w = i0 + tid < n ? __builtin_amdgcn_exp2f(lse[i0 + tid] - ref) : 0.0f;
+        const float w = i0 + tid < n ? __builtin_amdgcn_exp2f((i0 ? lse[i0 + tid] : first_lse) - ref) : 0.0f;
         l += w;
         __syncthreads();
         weight[tid] = w;
         __syncthreads();
         const uint32_t here = min(n - i0, 256u);
-        if (mine < per)
+        if (mine < per) {
+            uint32_t i = mine;
+            if (i0 == 0)
+#pragma unroll
+                for (uint32_t j = 0; j < kFirst; j++, i += per)
+                    if (i < here) add(weight[i], first[j]);
 #pragma unroll 4
-            for (uint32_t i = mine; i < here; i += per) {
-                const float4 y = *reinterpret_cast<const float4*>(x + (size_t)(i0 + i) * a.dim + d);
-                const float f = weight[i];
-                o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
-            }
+            for (; i < here; i += per) add(weight[i], *reinterpret_cast<const float4*>(x + (size_t)(i0 + i) * a.dim + d));
+        }
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
@@ -1104,30 +1117,39 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Partials
     if (tid == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
-// The same for few chunks: dim / 4 lanes take a row and head, and all of its chunks one after the other.
+// The same for few chunks: dim / 4 lanes take a row and head, and all of its chunks (2048 rows of 128 dims in 2 chunks: 4.8 us; 204 of 96 dims in 8: 3.9, 4.7 one after the other).
+constexpr uint32_t kFewChunks = 8;
 template <class T>
 __global__ __launch_bounds__(256) void attend_join_few_kernel(AttendArgs a, Partials parts)
 {
     const uint32_t lanes = a.dim / 4, per = 256 / lanes, mine = threadIdx.x / lanes, d = (threadIdx.x - mine * lanes) * 4;
     const uint64_t to = (uint64_t)blockIdx.x * per + mine;
     if (mine >= per || to >= (uint64_t)a.n_rows * a.q_heads) return;
+    const float* lse = parts.lse + to * parts.n_splits;
+    const float* x = parts.out + to * parts.n_splits * a.dim + d;
+    float4 y[kFewChunks];
+    float ls[kFewChunks];
+#pragma unroll
+    for (uint32_t i = 0; i < kFewChunks; i++) {
+        ls[i] = i < parts.n_splits ? lse[i] : 0.0f;
+        y[i] = i < parts.n_splits ? *reinterpret_cast<const float4*>(x + (size_t)i * a.dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     const uint32_t row = (uint32_t)(to / a.q_heads);
     const uint32_t b = a.cu_q ? request_of(a.cu_q, a.n_requests, row) : row;
     if (b >= a.n_requests) return;
     const uint32_t n = chunks_of(a, parts, b, row);
-    const float* lse = parts.lse + to * parts.n_splits;
-    const float* x = parts.out + to * parts.n_splits * a.dim + d;
     float top = -__builtin_inff(), l = 0.0f;
-    for (uint32_t i = 0; i < n; i++) top = fmaxf(top, lse[i]);
+#pragma unroll
+    for (uint32_t i = 0; i < kFewChunks; i++) top = i < n ? fmaxf(top, ls[i]) : top;
     const float ref = top == -__builtin_inff() ? 0.0f : top;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-    for (uint32_t i = 0; i < n; i++) {
-        const float4 y = *reinterpret_cast<const float4*>(x + (size_t)i * a.dim);
-        const float f = __builtin_amdgcn_exp2f(lse[i] - ref);
-        l += f;
-        o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
-    }
+#pragma unroll
+    for (uint32_t i = 0; i < kFewChunks; i++)
+        if (i < n) {
+            const float f = __builtin_amdgcn_exp2f(ls[i] - ref);
+            l += f;
+            o.x += f * y[i].x; o.y += f * y[i].y; o.z += f * y[i].z; o.w += f * y[i].w;
+        }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     store4<T>((T*)a.out + to * a.dim + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     if (d == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
@@ -1174,8 +1196,8 @@ template <class T> void launch_attend(const AttendArgs& a, const Cut& cut, uint3
     else by_dim(std::integral_constant<int, HNSW_AMD_CODES_E4M3>{});
     check_launch(who);
     if (cut.n_splits > 1) {
-        // few chunks: many rows to a workgroup (20480 rows of 64 dims in 2 chunks: 4 us, 38 with a workgroup each)
-        if (cut.n_splits <= 8) {
+        // few chunks: many rows to a workgroup (20480 rows of 64 dims in 2 chunks: 5.6 us, 38 with a workgroup each)
+        if (cut.n_splits <= kFewChunks) {
             const uint32_t per = 256 / (a.dim / 4);
             hipLaunchKernelGGL((attend_join_few_kernel<T>), dim3((a.n_rows * a.q_heads + per - 1) / per), dim3(256), 0, stream, a, parts);
         } else {
