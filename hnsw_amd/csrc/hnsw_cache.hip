@@ -164,32 +164,26 @@ __device__ __forceinline__ int scale_exponent(float peak, float most)
     return e;
 }
 
-// WPR wavefronts per (run of rows that lie next to each other in one block, head, keys or values).  First the rows' largest value, which
-// gives the block's scale; where that raises the scale of a block that held earlier tokens, their codes move to it; then the rows'
-// codes.  The first rows stay in registers between the two.  Single tokens (WPR = 1, one row a wavefront) are latency: the row is
-// asked for together with the slots, then the block's scale.  Prompts (WPR = 4, a block's worth of rows a workgroup) are memory.
+// Four wavefronts take a.span rows of one head's keys or values, run by run (a run: rows that lie next to each other in one block).  First the
+// rows' largest value, which gives the block's scale; where that raises the scale of a block that held earlier tokens, their codes move to it;
+// then the rows' codes.  What a wavefront has looked at first stays in its registers between the two.  Short runs (single tokens of many
+// requests) are latency: a wavefront takes each by itself.  Long runs (prompts) are memory: all four wavefronts take each.
 // A power of two as scale makes x / scale exact, so a code is ONE rounding of x, and moving codes to a larger scale one more.
-template <class T, int CODES, bool VEC, int WPR>
+template <class T, int CODES, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
 {
-    constexpr int kKeep = WPR == 1 ? 1 : 4;                     // passes over the rows whose values are kept
-    const uint32_t lane = threadIdx.x & 63, sub = WPR == 1 ? 0 : threadIdx.x >> 6;
-    const uint64_t unit = WPR == 1 ? (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-    const uint32_t part = (uint32_t)(unit % 2), head = (uint32_t)(unit / 2 % a.n_heads);
-    const uint64_t t0 = unit / 2 / a.n_heads * a.span;
-    if (t0 >= a.n_rows) return;
+    constexpr int kKeep = 4;                                    // passes over the rows whose values are kept
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t part = blockIdx.x % 2, head = blockIdx.x / 2 % a.n_heads;
+    const uint64_t t0 = (uint64_t)(blockIdx.x / 2 / a.n_heads) * a.span;
     __shared__ float peaks[4];
     const uint32_t bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs), dim = a.dim, lanes_per_row = dim / 8, rows_per_wave = 64 / lanes_per_row;
-    const uint32_t wave_row = lane / lanes_per_row, my_row = sub * rows_per_wave + wave_row, my_col = (lane - wave_row * lanes_per_row) * 8;
-    const uint32_t step = rows_per_wave * WPR;
+    const uint32_t wave_row = lane / lanes_per_row, my_col = (lane - wave_row * lanes_per_row) * 8;
     const bool active = wave_row < rows_per_wave;
     const int64_t n_slots = (int64_t)a.n_blocks << bs_log;
     const T* rows = (const T*)a.rows[part];
     const int64_t row_stride = a.row_stride[part], col = a.head_stride[part] * head + my_col;
-
-    float kept[kKeep][8];
-    auto load = [&](uint32_t row0, uint32_t r, float (&x)[8]) { load8<T, VEC>(rows + (int64_t)(row0 + r) * row_stride + col, x); };
-    if (WPR == 1 && active && t0 + my_row < a.n_rows) load((uint32_t)t0, my_row, kept[0]);
+    auto load = [&](uint32_t row, float (&x)[8]) { load8<T, VEC>(rows + (int64_t)row * row_stride + col, x); };
 
     const uint32_t end = (uint32_t)(t0 + a.span < a.n_rows ? t0 + a.span : a.n_rows);
     for (uint32_t base = (uint32_t)t0; base < end; base += 62) {
@@ -202,25 +196,17 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
         const unsigned long long follow = __ballot(follows);
         unsigned long long firsts = __ballot(valid && !follows) & ~(1ull << 63) & ~1ull;
         if (end - base < 62) firsts &= (2ull << (end - base)) - 1;
-        while (firsts) {
-            const int l = __builtin_ctzll(firsts);
-            firsts &= firsts - 1;
-            const uint32_t row0 = base + l - 1;
+
+        // The run of n rows that begins in lane l, by wavefront `sub` of `of`.
+        auto take = [&](int l, uint32_t n, uint32_t sub, auto of) {
+            constexpr uint32_t kOf = of.value;
+            const uint32_t row0 = base + l - 1, my_row = sub * rows_per_wave + wave_row, step = rows_per_wave * kOf;
             const int64_t slot = ((int64_t)__builtin_amdgcn_readlane((int)(slot_l >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)slot_l, l);
             const uint32_t block = (uint32_t)(slot >> bs_log), off = (uint32_t)(slot & (bs - 1));
             float* scale = a.scale[part] + (size_t)block * a.n_heads + head;
             uint8_t* codes = a.codes[part] + ((size_t)block * a.n_heads + head) * bs * dim;
             const float before = *scale;
-            uint32_t n = 1 + (l < 63 ? (uint32_t)__builtin_ctzll(~(follow >> (l + 1))) : 0);
-            if (l + n == 64)                                    // the run goes on behind what the wavefront has in view
-                for (;;) {
-                    const uint32_t i = n + lane;
-                    const bool more = off + i < bs && (uint64_t)row0 + i < a.n_rows && a.slots[row0 + i] == slot + i;
-                    const unsigned long long more_l = __ballot(more);
-                    if (more_l != ~0ull) { n += (uint32_t)__builtin_ctzll(~more_l); break; }
-                    n += 64;
-                }
-            float peak = 0.0f;
+            float kept[kKeep][8], peak = 0.0f;
             auto look = [&](const float (&x)[8]) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -229,21 +215,20 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
                 }
             };
             if (active) {
-                if (WPR > 1)
 #pragma unroll
-                    for (int i = 0; i < kKeep; i++)
-                        if (my_row + i * step < n) load(row0, my_row + i * step, kept[i]);
+                for (int i = 0; i < kKeep; i++)
+                    if (my_row + i * step < n) load(row0 + my_row + i * step, kept[i]);
 #pragma unroll
                 for (int i = 0; i < kKeep; i++)
                     if (my_row + i * step < n) look(kept[i]);
                 for (uint32_t r = my_row + kKeep * step; r < n; r += step) {
                     float x[8];
-                    load(row0, r, x);
+                    load(row0 + r, x);
                     look(x);
                 }
             }
             peak = wave_max_not_negative(peak);
-            if constexpr (WPR > 1) {
+            if constexpr (kOf > 1) {
                 if (lane == 0) peaks[sub] = peak;
                 __syncthreads();
                 peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
@@ -259,7 +244,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
             const float now = ldexpf(1.0f, e);
             if (held && now != before) {
                 const float ratio = before / now;
-                for (uint32_t i = sub * 64 + lane; i < bs * dim / 4; i += 64 * WPR) {
+                for (uint32_t i = sub * 64 + lane; i < bs * dim / 4; i += 64 * kOf) {
                     const uint32_t o = i * 4 / dim;
                     if (o >= off && o < off + n) continue;                          // about to be written
                     float x[4];
@@ -283,12 +268,36 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
                     if (my_row + i * step < n) write(my_row + i * step, kept[i]);
                 for (uint32_t r = my_row + kKeep * step; r < n; r += step) {
                     float x[8];
-                    load(row0, r, x);
+                    load(row0 + r, x);
                     write(r, x);
                 }
             }
-            if constexpr (WPR > 1) __syncthreads();             // (all have read the old scale and the peaks)
+            if constexpr (kOf > 1) __syncthreads();             // (all have read the old scale and the peaks)
             if (lane == 0 && sub == 0) *scale = now;
+        };
+        auto run_of = [&](int l) {
+            uint32_t n = 1 + (uint32_t)__builtin_ctzll(~(follow >> (l + 1)));
+            if (l + n == 64) {                                  // the run goes on behind what the wavefront has in view
+                const int64_t slot = ((int64_t)__builtin_amdgcn_readlane((int)(slot_l >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)slot_l, l);
+                const uint32_t row0 = base + l - 1, off = (uint32_t)(slot & (bs - 1));
+                for (;;) {
+                    const uint32_t i = n + lane;
+                    const bool more = off + i < bs && (uint64_t)row0 + i < a.n_rows && a.slots[row0 + i] == slot + i;
+                    const unsigned long long more_l = __ballot(more);
+                    if (more_l != ~0ull) { n += (uint32_t)__builtin_ctzll(~more_l); break; }
+                    n += 64;
+                }
+            }
+            return n;
+        };
+        // (the same runs in the same order in all four wavefronts, so that all of them meet at the barriers)
+        uint32_t turn = 0;
+        while (firsts) {
+            const int l = __builtin_ctzll(firsts);
+            firsts &= firsts - 1;
+            const uint32_t n = run_of(l);
+            if (n > 2 * rows_per_wave) take(l, n, wave, std::integral_constant<int, 4>{});
+            else if (turn++ % 4 == wave) take(l, n, 0u, std::integral_constant<int, 1>{});
         }
     }
 }
@@ -387,25 +396,21 @@ void cache_append(const hnsw_amd_token_cache* c, const void* k, const void* v, u
     const OnDevice on(device);
     AppendArgs a{{(uint8_t*)c->k_codes, (uint8_t*)c->v_codes}, {c->k_scale, c->v_scale}, {k, v}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride},
                  slots, n_rows, c->n_blocks, c->n_heads, c->block_tokens, c->dim, 1};
-    // Few rows: a wavefront looks at one row each, so that single tokens of many requests run side by side.  Many rows (a prompt): a
-    // workgroup looks at a block's worth, most of which are one run.
-    const bool many = (uint64_t)n_rows * c->n_heads > 16384;
-    if (many) a.span = c->block_tokens;
-    const uint64_t units = (uint64_t)((n_rows + a.span - 1) / a.span) * c->n_heads * 2, groups = many ? units : (units + 3) / 4;
+    // A workgroup looks at four rows, so that single tokens run side by side, at more where that would be more than 1024 workgroups, at up to 64
+    // (a prompt, of whose runs each is then one workgroup's).  64 rows, 8 heads of 128 dims: 8.8 us with 4 (and reading them back), 12.3 with 16; 600 rows of three prompts:
+    // 11.9 with 4, 10.2 with 8; 4000 single rows: 194 with 4, 186 with 32 (with reading the blocks back, 130 of it); 24000 rows of three
+    // prompts: 118 with 16, 81 with 64.
+    const uint64_t share = (uint64_t)n_rows * c->n_heads * 2 / 1024;
+    a.span = share < 8 ? 4 : share < 16 ? 8 : share < 32 ? 16 : share < 64 ? 32 : 64;
+    const uint64_t groups = (uint64_t)((n_rows + a.span - 1) / a.span) * c->n_heads * 2;
     if (groups >= 1ull << 24) throw std::invalid_argument("cache_append: too many rows and heads for one call");
     by_types(row_type, c->codes, [&](auto t, auto codes) {
         using T = decltype(t);
         const int64_t step = 16 / (int64_t)sizeof(T);
         const bool vec = aligned16(k) && aligned16(v) && k_row_stride % step == 0 && k_head_stride % step == 0 && v_row_stride % step == 0 && v_head_stride % step == 0;
-        auto go = [&](auto v, auto wpr) {
-            hipLaunchKernelGGL((append_kernel<T, codes.value, v.value, wpr.value>), dim3((uint32_t)groups), dim3(256), 0, (hipStream_t)stream, a);
-        };
-        auto by_rows = [&](auto v) {
-            if (many) go(v, std::integral_constant<int, 4>{});
-            else go(v, std::integral_constant<int, 1>{});
-        };
-        if (vec) by_rows(std::true_type{});
-        else by_rows(std::false_type{});
+        auto go = [&](auto v) { hipLaunchKernelGGL((append_kernel<T, codes.value, v.value>), dim3((uint32_t)groups), dim3(256), 0, (hipStream_t)stream, a); };
+        if (vec) go(std::true_type{});
+        else go(std::false_type{});
     });
     check_launch("cache_append");
 }
