@@ -44,6 +44,8 @@ __device__ __forceinline__ uint32_t last_not_after(const uint32_t* pre, uint32_t
 // launch that would wait for them) and then takes its share of the slots, table entries and returned blocks.  Nothing that a
 // workgroup reads is written by another: lengths and ring state go to buffers of their own, the table is written only beyond
 // what the requests held, and the ring only behind its tail, where no free block lies.
+// What bounds it is the chain of loads that wait for one another: lengths, table or ring, slots.  (64 requests, a token each: 6.0 us;
+// 1000 requests, 318000 tokens, 2.8 MB: 10.7 us.)
 __global__ void plan_kernel(PlanArgs a)
 {
     extern __shared__ uint32_t lds[];
@@ -169,6 +171,8 @@ __device__ __forceinline__ int scale_exponent(float peak, float most)
 // then the rows' codes.  What a wavefront has looked at first stays in its registers between the two.  Short runs (single tokens of many
 // requests) are latency: a wavefront takes each by itself.  Long runs (prompts) are memory: all four wavefronts take each.
 // A power of two as scale makes x / scale exact, so a code is ONE rounding of x, and moving codes to a larger scale one more.
+// (64 rows of 8 heads of 128 dims: 3.9 us.  Three prompts, 21500 rows, 132 MB: 45 us, 2.9 TB/s: slots, rows, largest value and codes follow
+// one another in a workgroup, and five workgroups a compute unit hide most of that.)
 template <class T, int CODES, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
 {
@@ -310,7 +314,7 @@ struct ReadArgs {
     uint32_t n_rows, n_blocks, n_heads, block_tokens, dim;
 };
 
-// Eight values a lane; blockIdx.y: keys or values.
+// Eight values a lane; blockIdx.y: keys or values.  Bound by memory (21500 rows in 32 bits, 220 MB: 41 us, 5.4 TB/s).
 template <class T, int CODES>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
 {
@@ -368,7 +372,7 @@ void cache_plan(const int32_t* lens, const int32_t* grow, uint32_t n_requests, i
     if (lens == lens_out || state == state_out) throw std::invalid_argument("cache_plan: the new lengths and ring state need buffers of their own");
     const OnDevice on(device);
     // A slot a thread, or four in a row where there are more than a few workgroups of them; 512 workgroups at most.  (64 requests, one slot
-    // each: 6.0 us, 7.5 with four.  1000 requests, 350000 slots: 10.7 us, 11.9 with one; 14.3 with workgroups of 1024 whose first threads do
+    // each: 6.0 us, 7.5 with four.  1000 requests, 318000 slots: 10.7 us, 11.9 with one; 14.3 with workgroups of 1024 whose first threads do
     // all the other work.)
     const uint32_t per = n_slots > 4096 ? 4 : 1;
     auto whole = [](uint64_t x) { return (x + 63) / 64 * 64; };
@@ -396,10 +400,10 @@ void cache_append(const hnsw_amd_token_cache* c, const void* k, const void* v, u
     const OnDevice on(device);
     AppendArgs a{{(uint8_t*)c->k_codes, (uint8_t*)c->v_codes}, {c->k_scale, c->v_scale}, {k, v}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride},
                  slots, n_rows, c->n_blocks, c->n_heads, c->block_tokens, c->dim, 1};
-    // A workgroup looks at four rows, so that single tokens run side by side, at more where that would be more than 1024 workgroups, at up to 64
-    // (a prompt, of whose runs each is then one workgroup's).  64 rows, 8 heads of 128 dims: 8.8 us with 4 (and reading them back), 12.3 with 16; 600 rows of three prompts:
-    // 11.9 with 4, 10.2 with 8; 4000 single rows: 194 with 4, 186 with 32 (with reading the blocks back, 130 of it); 24000 rows of three
-    // prompts: 118 with 16, 81 with 64.
+    // A workgroup looks at four rows, so that single tokens run side by side; at more where that would be more than 1024 workgroups, up to 64
+    // (a prompt, of whose runs each is one workgroup's).  Measured with reading the blocks back behind it, 8 heads of 128 dims: 64 single
+    // rows 8.8 us with 4, 12.3 with 16; 600 rows of three prompts 11.9 with 4, 10.2 with 8; 4000 single rows 194 with 4, 186 with 32; 21500
+    // rows of three prompts 118 with 16, 80 with 64.
     const uint64_t share = (uint64_t)n_rows * c->n_heads * 2 / 1024;
     a.span = share < 8 ? 4 : share < 16 ? 8 : share < 32 ? 16 : share < 64 ? 32 : 64;
     const uint64_t groups = (uint64_t)((n_rows + a.span - 1) / a.span) * c->n_heads * 2;
