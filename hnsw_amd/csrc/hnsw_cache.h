@@ -67,22 +67,31 @@ template <class T> __device__ __forceinline__ void store4(T* to, float a, float 
     else *reinterpret_cast<u32x2*>(to) = u32x2{pack2<T>(a, b), pack2<T>(c, d)};
 }
 
-// Eight consecutive elements of a row; VEC: the address is a multiple of 16 bytes.
-template <class T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&x)[8])
+// Eight elements of a row as they lie in memory (half the registers of their values where they have 16 bits);
+// VEC: the address is a multiple of 16 bytes.
+template <class T> struct Eight {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ float operator[](int j) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+        else return to_float(__builtin_bit_cast(T, (uint16_t)(w[j >> 1] >> (16 * (j & 1)))));
+    }
+};
+template <class T, bool VEC> __device__ __forceinline__ void load8(const T* p, Eight<T>& x)
 {
-    if constexpr (VEC && sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else if constexpr (VEC) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+    if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-            x[j] = to_float(__builtin_bit_cast(T, h));
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const u32x4 w = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x.w[4 * i + j] = w[j];
         }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x.w[j] = __float_as_uint(p[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = to_float(p[j]);
+        for (int j = 0; j < 4; j++) x.w[j] = (uint32_t)__builtin_bit_cast(uint16_t, p[2 * j]) | (uint32_t)__builtin_bit_cast(uint16_t, p[2 * j + 1]) << 16;
     }
 }
 

@@ -171,8 +171,8 @@ __device__ __forceinline__ int scale_exponent(float peak, float most)
 // then the rows' codes.  What a wavefront has looked at first stays in its registers between the two.  Short runs (single tokens of many
 // requests) are latency: a wavefront takes each by itself.  Long runs (prompts) are memory: all four wavefronts take each.
 // A power of two as scale makes x / scale exact, so a code is ONE rounding of x, and moving codes to a larger scale one more.
-// (64 rows of 8 heads of 128 dims: 3.9 us.  Three prompts, 21500 rows, 132 MB: 45 us, 2.9 TB/s: slots, rows, largest value and codes follow
-// one another in a workgroup, and five workgroups a compute unit hide most of that.)
+// (64 rows of 8 heads of 128 dims: 3.9 us.  Three prompts, 21500 rows, 132 MB: 40 us, 3.3 TB/s: slots, rows, largest value and codes follow
+// one another in a workgroup, and seven workgroups a compute unit hide most of that; five, with the rows kept as 32-bit values: 45 us.)
 template <class T, int CODES, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
 {
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
     const int64_t n_slots = (int64_t)a.n_blocks << bs_log;
     const T* rows = (const T*)a.rows[part];
     const int64_t row_stride = a.row_stride[part], col = a.head_stride[part] * head + my_col;
-    auto load = [&](uint32_t row, float (&x)[8]) { load8<T, VEC>(rows + (int64_t)row * row_stride + col, x); };
+    auto load = [&](uint32_t row, Eight<T>& x) { load8<T, VEC>(rows + (int64_t)row * row_stride + col, x); };
 
     const uint32_t end = (uint32_t)(t0 + a.span < a.n_rows ? t0 + a.span : a.n_rows);
     for (uint32_t base = (uint32_t)t0; base < end; base += 62) {
@@ -210,8 +210,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
             float* scale = a.scale[part] + (size_t)block * a.n_heads + head;
             uint8_t* codes = a.codes[part] + ((size_t)block * a.n_heads + head) * bs * dim;
             const float before = *scale;
-            float kept[kKeep][8], peak = 0.0f;
-            auto look = [&](const float (&x)[8]) {
+            Eight<T> kept[kKeep];
+            float peak = 0.0f;
+            auto look = [&](const Eight<T>& x) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float y = fabsf(x[j]);
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
                 for (int i = 0; i < kKeep; i++)
                     if (my_row + i * step < n) look(kept[i]);
                 for (uint32_t r = my_row + kKeep * step; r < n; r += step) {
-                    float x[8];
+                    Eight<T> x;
                     load(row0 + r, x);
                     look(x);
                 }
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
                 }
             }
             const float inv = ldexpf(1.0f, -e);
-            auto write = [&](uint32_t r, const float (&x)[8]) {
+            auto write = [&](uint32_t r, const Eight<T>& x) {
                 float lo[4], hi[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) { lo[j] = x[j] * inv; hi[j] = x[j + 4] * inv; }
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
                 for (int i = 0; i < kKeep; i++)
                     if (my_row + i * step < n) write(my_row + i * step, kept[i]);
                 for (uint32_t r = my_row + kKeep * step; r < n; r += step) {
-                    float x[8];
+                    Eight<T> x;
                     load(row0 + r, x);
                     write(r, x);
                 }
@@ -403,7 +404,7 @@ void cache_append(const hnsw_amd_token_cache* c, const void* k, const void* v, u
     // A workgroup looks at four rows, so that single tokens run side by side; at more where that would be more than 1024 workgroups, up to 64
     // (a prompt, of whose runs each is one workgroup's).  Measured with reading the blocks back behind it, 8 heads of 128 dims: 64 single
     // rows 8.8 us with 4, 12.3 with 16; 600 rows of three prompts 11.9 with 4, 10.2 with 8; 4000 single rows 194 with 4, 186 with 32; 21500
-    // rows of three prompts 118 with 16, 80 with 64.
+    // rows of three prompts 118 with 16, 80 with 64 (72 since the rows are kept in 16 bits).
     const uint64_t share = (uint64_t)n_rows * c->n_heads * 2 / 1024;
     a.span = share < 8 ? 4 : share < 16 ? 8 : share < 32 ? 16 : share < 64 ? 32 : 64;
     const uint64_t groups = (uint64_t)((n_rows + a.span - 1) / a.span) * c->n_heads * 2;
