@@ -146,7 +146,7 @@ __device__ __forceinline__ bool unit_of(const AttendArgs& a, uint32_t u, uint32_
 
 // A query row as it lies in memory, eight elements from column col(s) on for step s (zeros behind dim, or where there is no row): the
 // loads.
-template <class T, int KS> struct RawQuery { T x[KS][8]; };
+template <class T, int KS> struct RawQuery { Eight<T> x[KS]; };
 template <class T, int KS, class Col>
 __device__ __forceinline__ void load_query(const AttendArgs& a, bool there, uint32_t row, uint32_t head, uint32_t vec, Col&& col, RawQuery<T, KS>& raw)
 {
@@ -154,21 +154,10 @@ __device__ __forceinline__ void load_query(const AttendArgs& a, bool there, uint
 #pragma unroll
     for (int s = 0; s < KS; s++) {
         const uint32_t c = col(s);
-#pragma unroll
-        for (int j = 0; j < 8; j++) raw.x[s][j] = T{};
+        raw.x[s] = Eight<T>{};
         if (there && c < a.dim) {
-            if (vec) {
-                struct alignas(16) Piece { T x[16 / sizeof(T)]; };
-#pragma unroll
-                for (int h = 0; h < (int)sizeof(T) / 2; h++) {
-                    const Piece p = *reinterpret_cast<const Piece*>(x + c + h * (16 / sizeof(T)));
-#pragma unroll
-                    for (int j = 0; j < (int)(16 / sizeof(T)); j++) raw.x[s][h * (16 / sizeof(T)) + j] = p.x[j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) raw.x[s][j] = x[c + j];
-            }
+            if (vec) load8<T, true>(x + c, raw.x[s]);
+            else load8<T, false>(x + c, raw.x[s]);
         }
     }
 }
@@ -182,14 +171,14 @@ __device__ __forceinline__ float query_operands(const AttendArgs& a, const RawQu
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(to_float(raw.x[s][j])));
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(raw.x[s][j]));
     top = max_over_groups(top);
     const int e = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float y = ldexpf(to_float(raw.x[s][CODES == HNSW_AMD_CODES_I8 ? kOrderI8[j] : j]) * sign, e);
+            const float y = ldexpf(raw.x[s][CODES == HNSW_AMD_CODES_I8 ? kOrderI8[j] : j] * sign, e);
             const _Float16 hi = (_Float16)y;
             q[s][0][j] = hi;
             if constexpr (QT == 2) q[s][1][j] = (_Float16)(y - (float)hi);
