@@ -36,7 +36,7 @@ def _binding():
 
 class Plan(NamedTuple):
     """What cache_plan returns: the new tokens' slots [n_slots] (-1 behind the last), cu_new [n + 1], the new lengths [n], the
-    ring's new [head, tail], and a status [1] that is 0 unless nothing was done (capi.PLAN_* bits)."""
+    ring's new [head, tail], and a status [1] that is 0 unless nothing was done (capi.PLAN_* bits).  The five lie in one allocation."""
     slots: object
     cu_new: object
     lens: object
@@ -75,11 +75,7 @@ class TokenCache:
 
     def read(self, slots, dtype=None):
         """(keys, values) of the slots [rows] int64: two [rows, n_heads, dim] tensors, float32 unless `dtype` says otherwise."""
-        import torch
-        types = {None: capi.TYPE_F32, torch.float32: capi.TYPE_F32, torch.float16: capi.TYPE_F16, torch.bfloat16: capi.TYPE_BF16}
-        if dtype not in types:
-            raise ValueError("read: float32, float16 or bfloat16")
-        return self._b.read(self._c, slots, types[dtype])
+        return self._b.read(self._c, slots, dtype)
 
     def attend(self, q, table, lens, *, cu_q=None, causal: bool = True, scale: float | None = None, max_len: int = 0):
         """(out, lse) of the queries q [rows, heads, dim] over all tokens of their requests; table [n, width], lens [n] int32.  Without

@@ -2,6 +2,7 @@
 // outputs, workspaces and the current stream, then the C entry points of include/hnsw_amd.h.  In Python these cost several times
 // what a launch does, and the calls of a decoding step are a launch each.  The entry points come as addresses from the library
 // that the process has loaded, which this module is not linked with.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -187,6 +188,25 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> ts)
     return t;
 }
 
+// Tensors that lie one behind the other in one allocation of `longs` 64-bit words (an allocation costs several times what a tensor does).
+class Pieces {
+public:
+    Pieces(const at::TensorOptions& options, int64_t longs) : all_(at::empty({longs}, options.dtype(at::kLong))) {}
+    at::Tensor next(at::ScalarType type, int64_t n)
+    {
+        const int64_t size = (int64_t)c10::elementSize(type);
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all_.storage()), all_.key_set(), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+        t.unsafeGetTensorImpl()->set_storage_offset(at_ / size);
+        at_ += n * size;
+        return t;
+    }
+
+private:
+    at::Tensor all_;
+    int64_t at_ = 0;                        // bytes (the longer types come first)
+};
+
 PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t n_args)
 {
     return guarded([&]() -> PyObject* {
@@ -203,9 +223,10 @@ PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t n_args)
         need(ring, "ring", at::kInt, {-1}, device);
         need(state, "state", at::kLong, {2}, device);
         if (n > 0xffffffffll || table.size(1) > 0xffffffffll || ring.size(0) > 0xffffffffll) refuse("cache_plan: an extent is out of range");
-        const at::TensorOptions longs = state.options(), words = lens.options();
-        at::Tensor slots = at::empty({n_slots}, longs), state_out = at::empty({2}, longs), cu = at::empty({n + 1}, words), lens_out = at::empty({n}, words),
-                   status = at::empty({1}, words);
+        // one allocation for the five results
+        Pieces pieces(state.options(), n_slots + 2 + (n + 1 + n + 1 + 1) / 2);
+        const at::Tensor slots = pieces.next(at::kLong, n_slots), state_out = pieces.next(at::kLong, 2), cu = pieces.next(at::kInt, n + 1),
+                         lens_out = pieces.next(at::kInt, n), status = pieces.next(at::kInt, 1);
         check(g_plan(lens.data_ptr<int32_t>(), grow.data_ptr<int32_t>(), (uint32_t)n, table.data_ptr<int32_t>(), (uint32_t)table.size(1), ring.data_ptr<int32_t>(),
                      (uint32_t)ring.size(0), state.data_ptr<int64_t>(), (uint32_t)block, (uint32_t)n_slots, slots.data_ptr<int64_t>(), cu.data_ptr<int32_t>(),
                      lens_out.data_ptr<int32_t>(), state_out.data_ptr<int64_t>(), status.data_ptr<int32_t>(), device.index(), stream_of(device)));
@@ -229,17 +250,20 @@ PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n_args)
     });
 }
 
-// read(cache, slots, type of the outputs: 0 float32, 1 float16, 2 bfloat16)
+// read(cache, slots, dtype of the outputs or None)
 PyObject* py_read(PyObject*, PyObject* const* args, Py_ssize_t n_args)
 {
     return guarded([&]() -> PyObject* {
         count_args(n_args, 3);
         const Cache& c = cache(args[0]);
         const at::Tensor& slots = tensor(args[1], "slots");
-        const uint32_t type = (uint32_t)integer(args[2], 0, 2, "type");
+        if (args[2] != Py_None && !THPDtype_Check(args[2])) refuse("read: float32, float16 or bfloat16");
+        const at::ScalarType dtype = args[2] == Py_None ? at::kFloat : reinterpret_cast<THPDtype*>(args[2])->scalar_type;
+        if (dtype != at::kFloat && dtype != at::kHalf && dtype != at::kBFloat16) refuse("read: float32, float16 or bfloat16");
+        const uint32_t type = dtype == at::kFloat ? HNSW_AMD_TYPE_F32 : dtype == at::kHalf ? HNSW_AMD_TYPE_F16 : HNSW_AMD_TYPE_BF16;
         need(slots, "slots", at::kLong, {-1}, c.device);
         if (slots.size(0) >= INT64_C(1) << 31) refuse("read: too many slots");
-        const auto options = slots.options().dtype(type == HNSW_AMD_TYPE_F32 ? at::kFloat : type == HNSW_AMD_TYPE_F16 ? at::kHalf : at::kBFloat16);
+        const auto options = slots.options().dtype(dtype);
         at::Tensor k = at::empty({slots.size(0), c.c.n_heads, c.c.dim}, options), v = at::empty({slots.size(0), c.c.n_heads, c.c.dim}, options);
         check(g_read(&c.c, slots.data_ptr<int64_t>(), (uint32_t)slots.size(0), type, k.data_ptr(), v.data_ptr(), c.device.index(), stream_of(c.device)));
         return tuple_of({k, v});
