@@ -74,9 +74,11 @@ static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_
         c.waves = 1;
         chunk = 256;
     } else if (c.mt == 1 && have < 512 && items <= 1024) {
-        // few short ones: eight wavefronts instead of chunks, which would need a second launch to be joined (one request, 8 heads of 777 tokens:
-        // 9.5 us, 10.0 in chunks)
-        c.waves = 8;
+        // few short ones: one chunk, as a second launch to join more of them would cost more than it saves (one request, 8 heads of 777
+        // tokens of 64 dims: 9.7 us, 10.2 in chunks), and eight wavefronts for it (11.1 with four) where it is not so short that they
+        // cost more in starting (100 tokens: 6.4 us, 6.0 with four) and all fit the chip at once: beyond 64 dims one such workgroup to a compute
+        // unit (48 requests of up to 1000 tokens, 8 heads of 128 dims: 23.3 us, 17.6 with four)
+        c.waves = items > 128 && have <= (dim <= 64 ? 512 : 256) ? 8 : 4;
         chunk = 1024;
     } else {
         // one round of three workgroups a compute unit, but no chunk of more than 4096: a long request among short ones is not left to
