@@ -664,7 +664,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
 // of the values' octets, so that the blocks they lie in are scalars.
 // HALVES = 2: twice the wavefronts, which take the tiles in turn and join at the end: half the steps of one after the other where
 // workgroups are too few to hide them.  (Up to 64 dims, where two such workgroups fit a compute unit: 163 rows each of eight requests over
-// 1000 tokens, 16 heads, 37.4 -> 34.3 us.  At 128 dims only one fits, and the rounds cost more than the steps: 300 rows each of four over 700
+// 1000 tokens, 16 heads: 34.3 us, 37.4 without.  At 128 dims only one fits, and the rounds cost more than the steps: 300 rows each of four over 700
 // tokens, 43.8 -> 51.3.)
 // Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel, but that a block's value scale goes
 // into the exponent instead of being multiplied in: weights are 2^(score - maximum + log2 of the scale over the largest), their
