@@ -327,24 +327,22 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
     const uint32_t part = blockIdx.y, groups = a.dim / 8;
     T* out = (T*)a.out[part];
     if (!out) return;
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x, row = i / groups;
-    const uint32_t col = (uint32_t)(i - row * groups) * 8;
-    const uint64_t t = row / a.n_heads;
-    const uint32_t head = (uint32_t)(row - t * a.n_heads);
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / groups, col = (i - row * groups) * 8, t = row / a.n_heads, head = row - t * a.n_heads;   // (below 2^32)
     if (t >= a.n_rows) return;
     const int64_t slot = a.slots[t];
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (slot >= 0 && slot < (int64_t)a.n_blocks * a.block_tokens) {
-        const uint64_t at = (uint64_t)(slot / a.block_tokens) * a.n_heads + head;
+    const uint32_t bs_log = 31 - __builtin_clz(a.block_tokens);
+    if (slot >= 0 && slot < (int64_t)a.n_blocks << bs_log) {
+        const uint64_t at = (uint64_t)(slot >> bs_log) * a.n_heads + head;
         const float s = a.scale[part][at];
-        const u32x2 w = *reinterpret_cast<const u32x2*>(a.codes[part] + (at * a.block_tokens + (uint64_t)(slot % a.block_tokens)) * a.dim + col);
+        const u32x2 w = *reinterpret_cast<const u32x2*>(a.codes[part] + ((at << bs_log) + (uint64_t)(slot & (a.block_tokens - 1))) * a.dim + col);
         float lo[4], hi[4];
         decode4<CODES>(w[0], lo);
         decode4<CODES>(w[1], hi);
 #pragma unroll
         for (int j = 0; j < 4; j++) { x[j] = lo[j] * s; x[j + 4] = hi[j] * s; }
     }
-    T* to = out + row * a.dim + col;
+    T* to = out + (uint64_t)row * a.dim + col;
     store4<T>(to, x[0], x[1], x[2], x[3]);
     store4<T>(to + 4, x[4], x[5], x[6], x[7]);
 }
@@ -379,7 +377,7 @@ void cache_plan(const int32_t* lens, const int32_t* grow, uint32_t n_requests, i
     const OnDevice on(device);
     // A slot a thread, or four in a row where there are more than a few workgroups of them; 512 workgroups at most.  (64 requests, one slot
     // each: 6.0 us, 7.5 with four.  1000 requests, 318000 slots: 10.7 us, 11.9 with one; 14.3 with workgroups of 1024 whose first threads do
-    // all the other work.)
+    // all the other work.  All of these with prefix sums that took 2 us more than they do now.)
     const uint32_t per = n_slots > 4096 ? 4 : 1;
     auto whole = [](uint64_t x) { return (x + 63) / 64 * 64; };
     const uint64_t mappers = whole((n_slots + per - 1) / per), takers = whole(n_slots / block_tokens + n_requests), others = whole(n_requests);
