@@ -17,6 +17,8 @@ struct AttendArgs {
     float scale;
     void* out;
     float* lse;
+    uint32_t group, lists;      // query heads that share a key head (a list), and lists that share a key head
+    float group_inverse;
 };
 
 struct Partials {

@@ -124,8 +124,11 @@ void cache_attend(const hnsw_amd_token_cache* c, const void* q, uint32_t n_rows,
     const char* who = found ? "cache_attend_found" : "cache_attend";
     if (!c) throw std::invalid_argument(std::string(who) + ": NULL argument");
     AttendArgs a{(const uint8_t*)c->k_codes, (const uint8_t*)c->v_codes, c->k_scale, c->v_scale, c->n_blocks, c->n_heads, c->block_tokens, c->dim,
-                 q, q_row_stride, q_head_stride, n_rows, q_heads, table, lens, cu_q, ids, width, n_requests, n_ids, id_heads, causal, found ? 1 : 0, scale, out, lse};
+                 q, q_row_stride, q_head_stride, n_rows, q_heads, table, lens, cu_q, ids, width, n_requests, n_ids, id_heads, causal, found ? 1 : 0, scale, out, lse, 0, 1, 0.0f};
     check_attend(c, a, who);
+    a.group = q_heads / (found ? id_heads : c->n_heads);
+    a.lists = found ? id_heads / c->n_heads : 1;
+    a.group_inverse = 1.0f / (float)a.group;
     check_row_type(row_type, who);
     if (n_rows == 0) return;
     const Cut cut = found ? cut_work(c->dim, n_rows, q_heads, n_rows, id_heads, n_ids, false, false)

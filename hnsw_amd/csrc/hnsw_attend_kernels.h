@@ -107,6 +107,13 @@ __device__ __forceinline__ uint32_t length_of(const AttendArgs& a, int32_t len)
     const int64_t cap = (int64_t)a.width * a.block_tokens;
     return (uint32_t)min(max((int64_t)len, (int64_t)0), cap);
 }
+// r / group of a row and head (both below 2^24: a product with the reciprocal is off by one at most)
+__device__ __forceinline__ uint32_t of_group(const AttendArgs& a, uint32_t r)
+{
+    const uint32_t q = (uint32_t)((float)r * a.group_inverse);
+    const int32_t rest = (int32_t)(r - q * a.group);
+    return rest < 0 ? q - 1 : rest >= (int32_t)a.group ? q + 1 : q;
+}
 // tokens that row i of a request's n rows sees
 __device__ __forceinline__ uint32_t seen_by(const AttendArgs& a, uint32_t len, uint32_t n, uint32_t i)
 {
@@ -190,6 +197,14 @@ __device__ __forceinline__ float query_operands(const AttendArgs& a, const RawQu
 constexpr int rows_depth(int dp, int mt, int nw) { return dp <= 128 && mt == 1 && (dp == 64 || nw != 4) ? 2 : 1; }
 constexpr int rows_waves(int dp, int mt, int nw) { return dp == 64 ? (mt == 1 ? 4 : 3) : dp == 128 && mt == 1 && rows_depth(dp, mt, nw) == 1 ? 3 : 2; }
 
+// The arguments in scalar registers, asked for together: left to themselves they are loaded where they are used first, and every line
+// of them is another wait in a chain that bounds short calls.
+__device__ __forceinline__ void arguments_now(const AttendArgs& a, const Partials& parts)
+{
+    asm volatile("" ::"s"(a.k_codes), "s"(a.v_codes), "s"(a.k_scale), "s"(a.v_scale), "s"(a.n_blocks), "s"(a.n_heads), "s"(a.dim), "s"(a.q), "s"(a.table), "s"(a.lens),
+                 "s"(a.width), "s"(a.scale), "s"(a.out), "s"(parts.chunk));
+}
+
 // Attention of few query rows over many tokens: for single tokens the codes are read once and that is the time.
 //
 // The workgroup takes one key head of one request (or one list), up to 16 * MT rows of queries and one chunk of the tokens; its
@@ -224,12 +239,13 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     __shared__ float join_m[NW][16 * MT], join_l[NW][16 * MT], red[NW];
     __shared__ uint32_t red_n[NW];
 
+    arguments_now(a, parts);
     const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t head = blockIdx.x % heads, unit = blockIdx.x / heads, split = blockIdx.y;
     const uint32_t dim = a.dim, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs);
-    const uint32_t group = a.q_heads / heads;                   // rows of a token: query heads that share this key head, or list
-    const uint32_t kv = FOUND ? head / (heads / a.n_heads) : head;
+    const uint32_t group = a.group;                             // rows of a token: query heads that share this key head, or list
+    const uint32_t kv = FOUND ? head / a.lists : head;
 
     // which rows: `first` + r / group is the query row of row r, head * group + r % group its head
     uint32_t b, first, count, r0;
@@ -275,7 +291,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     for (int mt = 0; mt < MT; mt++) {
         const uint32_t r = r0 + 16 * mt + m;
         const bool there = r < n_r;
-        const uint32_t i = there ? r / group : 0, h = head * group + (there ? r - i * group : 0);
+        const uint32_t i = there ? of_group(a, r) : 0, h = head * group + (there ? r - i * group : 0);
         load_query<T, KS>(a, there, first + i, h, q_vec, [&](int s) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); }, raw[mt]);
     }
     const uint32_t len = __builtin_amdgcn_readfirstlane(length_of(a, len_raw));
@@ -286,15 +302,15 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
             const Span s = rows_of(a, b);
             seen[mt] = seen_by(a, len, s.count, first - s.first);
         } else {
-            seen[mt] = r < n_r ? seen_by(a, len, count, r / group) : 0;
+            seen[mt] = r < n_r ? seen_by(a, len, count, of_group(a, r)) : 0;
         }
     }
     // (rows follow one another in what they see)
     if constexpr (FOUND) {
         least = most = seen[0];
     } else {
-        least = seen_by(a, len, count, r0 / group);
-        most = seen_by(a, len, count, (min(r0 + 16 * MT, n_r) - 1) / group);
+        least = seen_by(a, len, count, of_group(a, r0));
+        most = seen_by(a, len, count, of_group(a, min(r0 + 16 * MT, n_r) - 1));
     }
 
     const uint32_t all = FOUND ? a.n_ids : most;                // items: tokens, or list entries
@@ -639,7 +655,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     };
     const float unit_o = unit_v / kPScale;
     for (uint32_t r = wave; r < 16 * MT && r0 + r < n_r; r += NW) {
-        const uint32_t i = (r0 + r) / group;
+        const uint32_t i = of_group(a, r0 + r);
         const size_t to = (size_t)(first + i) * a.q_heads + head * group + (r0 + r - i * group);
         const float ref = ref_of(r);
         float l = 0.0f;
@@ -688,12 +704,13 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
     __shared__ __align__(16) _Float16 vals[NBUF * HALVES][DP * kTokens];
     auto val_at = [](uint32_t d, uint32_t oct) { return d * kTokens + 8 * (oct ^ ((d >> 1) & 7)); };
 
+    arguments_now(a, parts);
     const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const uint32_t of_all = __builtin_amdgcn_readfirstlane(tid >> 6), wave = of_all % kWaves, half = of_all / kWaves;
     const uint32_t kv = blockIdx.x % a.n_heads, split = blockIdx.y;
     const uint32_t unit = gridDim.x / a.n_heads - 1 - blockIdx.x / a.n_heads;   // the last rows of a prompt see the most: first
     const uint32_t dim = a.dim, bs = a.block_tokens, bs_log = 31 - __builtin_clz(bs);
-    const uint32_t group = a.q_heads / a.n_heads;
+    const uint32_t group = a.group;
     constexpr uint32_t kRows = kWaves * 16 * MT;
     uint32_t b, part;
     Span rows;
@@ -710,7 +727,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
     for (int mt = 0; mt < MT; mt++) {
         const uint32_t r = r0 + 16 * mt + m;
         const bool there = r < n_r;
-        const uint32_t i = there ? r / group : 0, h = kv * group + (there ? r - i * group : 0);
+        const uint32_t i = there ? of_group(a, r) : 0, h = kv * group + (there ? r - i * group : 0);
         seen[mt] = i;
         load_query<T, KS>(a, there, rows.first + i, h, q_vec, [&](int s) { return 32 * s + 8 * g; }, raw[mt]);
     }
@@ -718,11 +735,11 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) seen[mt] = r0 + 16 * mt + m < n_r ? seen_by(a, len, rows.count, seen[mt]) : 0;
     // (rows follow one another in what they see; a wavefront without rows sees nothing)
-    const uint32_t least = r0 < n_r ? seen_by(a, len, rows.count, r0 / group) : 0;
-    const uint32_t most = r0 < n_r ? seen_by(a, len, rows.count, (min(r0 + 16 * MT, n_r) - 1) / group) : 0;
+    const uint32_t least = r0 < n_r ? seen_by(a, len, rows.count, of_group(a, r0)) : 0;
+    const uint32_t most = r0 < n_r ? seen_by(a, len, rows.count, of_group(a, min(r0 + 16 * MT, n_r) - 1)) : 0;
     // what the workgroup's last row sees
     const uint32_t last_r = min((part + 1) * kRows, n_r) - 1;
-    const uint32_t all = seen_by(a, len, rows.count, last_r / group);
+    const uint32_t all = seen_by(a, len, rows.count, of_group(a, last_r));
     if (split > 0 && begin >= all) return;
     const uint32_t end = split + 1 < parts.n_splits ? min(begin + parts.chunk, all) : all;
 
@@ -1013,7 +1030,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
         const float l = sum_over_groups(sum[mt]);
         const uint32_t r = r0 + 16 * mt + m;
         if (r >= n_r) continue;
-        const uint32_t i = r / group;
+        const uint32_t i = of_group(a, r);
         const size_t to = (size_t)(rows.first + i) * a.q_heads + kv * group + (r - i * group);
         const float inv = l == 0.0f ? 0.0f : unit_o / l, lse = l == 0.0f ? -__builtin_inff() : top[mt] + __builtin_amdgcn_logf(l);
         if (parts.n_splits == 1) {
