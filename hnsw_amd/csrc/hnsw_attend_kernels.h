@@ -222,9 +222,9 @@ __device__ __forceinline__ void arguments_now(const AttendArgs& a, const Partial
 // takes that up for the others.  Sums, maxima and outputs are in 32 bits.
 // A workgroup's start is a chain of loads that wait for one another (length, table, codes; for lists: ids, table, codes): the first
 // tile's codes are asked for as soon as the table is there, and queries and scales are made ready meanwhile.
-// Measured (memory bounds the long ones, that chain the short ones): 64 requests of 1 to 8192 tokens, 8 heads of 128 dims, 540 MB: 115 us,
-// 4.7 TB/s (a large copy: 4.85); 2 requests of 150000 and more, 678 MB: 126 us, 5.4 TB/s; one request of 777 tokens, 8 heads of 64 dims: 9.8 us;
-// lists of 100 tokens, 64 requests of 32 lists, 56 MB of single rows: 18.4 us, 3.0 TB/s.
+// Measured (memory bounds the long ones, that chain the short ones): 64 requests of 1 to 8192 tokens, 8 heads of 128 dims, 540 MB: 113 us,
+// 4.8 TB/s (a large copy: 4.85); 2 requests of 150000 and more, 678 MB: 126 us, 5.4 TB/s; one request of 777 tokens, 8 heads of 64 dims: 9.4 us;
+// lists of 100 tokens, 64 requests of 32 lists, 56 MB of single rows: 17.7 us, 3.2 TB/s.
 template <class T, int CODES, int DP, int MT, int NW, bool FOUND>
 __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
 {
