@@ -152,6 +152,35 @@ def test_append_many_rows(codes):
         assert torch.equal(scale.cpu().double(), s) and torch.equal(have.cpu().double(), want)
 
 
+@pytest.mark.parametrize("rows,dim,codes,dtype", [(300, 128, I8, BF16), (1100, 128, E4, BF16), (2500, 48, I8, F32), (4500, 128, I8, F16), (9000, 16, E4, BF16), (9000, 256, I8, BF16)])
+def test_append_runs_of_all_lengths(rows, dim, codes, dtype):
+    """Single rows, short runs, whole blocks and rows without a slot, mixed, in calls of all sizes: exact, as the rows of a block lie together."""
+    heads, block, rng, gen = 4, 64, random.Random(rows + dim), torch.Generator().manual_seed(rows)
+    slots, blk = [], 0
+    while len(slots) < rows:
+        kind = rng.randrange(6)
+        n = [1, 1, rng.randint(2, 9), rng.randint(10, 63), block, 0][kind]
+        if n == 0:
+            slots += [rng.choice([-1, 2 ** 40])] * rng.randint(1, 3)
+            continue
+        off = rng.choice([0, rng.randint(0, block - n)])
+        slots += range(blk * block + off, blk * block + off + n)
+        blk += 1
+    slots = slots[:rows]
+    order = rng.sample(range(blk + 1), blk + 1)
+    slots = [order[x // block] * block + x % block if 0 <= x < blk * block else x for x in slots]
+    k0, v0 = (_values(blk + 1, heads, block, dim, codes, gen) for _ in range(2))
+    scale0 = torch.exp2(torch.randint(-9, 1, (2, blk + 1, heads), generator=gen).float())
+    new = [(torch.randn((rows, heads, dim), generator=gen) * torch.exp2(torch.randint(-4, 5, (rows, 1, 1), generator=gen).float())).to(dtype) for _ in range(2)]
+    cache = TokenCache(k0.cuda(), v0.cuda(), scale0[0].cuda(), scale0[1].cuda())
+    cache.append(new[0].cuda(), new[1].cuda(), _gpu(slots, torch.int64))
+    for got, scale, before, s0, x in ((cache.k_codes, cache.k_scale, k0, scale0[0], new[0]), (cache.v_codes, cache.v_scale, v0, scale0[1], new[1])):
+        want, want_scale = before.double(), s0.double()
+        ref.append(want, want_scale, x.double(), slots, block, codes)
+        assert torch.equal(scale.double().cpu(), want_scale)
+        assert torch.equal(got.cpu().double(), want)
+
+
 @pytest.mark.parametrize("peak", [0.0, 2.0 ** -140, 2.0 ** -100 * 127, 127.0, 127.00001, 448.0, 3.0e38, torch.finfo(F32).max])
 @pytest.mark.parametrize("codes", [I8, E4])
 def test_scale_at_the_borders(peak, codes):
