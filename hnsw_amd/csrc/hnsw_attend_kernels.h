@@ -10,16 +10,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaves = 4;                 // wavefronts of a workgroup of attend_tile_kernel and attend_join_kernel
 constexpr uint32_t kScanTokens = 4096;    // of one table of block entries in LDS (all tokens), and
 constexpr uint32_t kListTokens = 1024;    // of one table of token entries (listed tokens)
-// A softmax's reference is only moved when a score is more than this above it, in base 2: moving it costs as much as a third of a tile
-// (the outputs are multiplied by the change), and over random scores some row of 16 sees a new maximum in every second tile.
-// Probabilities relative to the reference are then up to 2^4, and what they are multiplied by before they become 16-bit floats
-// (largest 2^16) leaves room for that.
-constexpr float kLead = 4.0f;
-constexpr float kPScale = 2048.0f;
-
-template <class T> constexpr int kQTerms = sizeof(T) == 4 ? 2 : 1;                  // 16-bit floats that a query element is split into
-template <class T> constexpr int kPTerms = std::is_same_v<T, bf16> ? 1 : 2;         // and a probability
-
+// What meets the values' codes is a token's weight: its probability times its block's value scale, as a 16-bit float in units of 2^-11 of a
+// reference that each row has for itself, the largest weight it has seen.  (A row's own: next to tokens that it does not see, or that weigh
+// nothing in it, blocks of any scale leave it its precision.)  The reference is only moved when a weight is more than this above it, in base
+// 2: moving it costs as much as a third of a tile (the outputs are multiplied by the change), and over random scores some row of 16 sees a new
+// maximum in every second tile.  Weights are then below 2^15.9, and 16-bit floats go to 65504.
+constexpr float kLead = 4.9f;
+constexpr float kPScale = 2048.0f, kPScaleLog = 11.0f;
 __device__ __forceinline__ float max_over_groups(float x)       // over the four lanes that share lane & 15
 {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -34,6 +31,25 @@ __device__ __forceinline__ float sum_over_groups(float x)
     r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+template <class T> constexpr int kQTerms = sizeof(T) == 4 ? 2 : 1;                  // 16-bit floats that a query element is split into
+template <class T> constexpr int kPTerms = std::is_same_v<T, bf16> ? 1 : 2;         // and a weight
+
+// A value scale in base 2: -inf for 0, and finite where a scale is none (tokens that a row does not see weigh 2^-inf whatever it is).
+__device__ __forceinline__ float log2_of_scale(float s) { return fminf(__builtin_amdgcn_logf(s), 128.0f); }
+// log2 of a sum that is in units of 2^top (the whole parts are added first: they can be large, of opposite sign)
+__device__ __forceinline__ float log2_of_sum(float top, float l)
+{
+    return (top + (float)__builtin_amdgcn_frexp_expf(l)) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(l));
+}
+// A value scale's inverse in units of 2^11, by which a weight gives its probability back, so that one exponential gives both: the sum of the
+// probabilities is kept in units of the weights' reference, which is within 2^40 of the largest probability as long as scales are
+// within 2^40 of 1.  For others (blocks of zeros among them) this is 0: from the first such block on a wavefront sums probabilities apart, in
+// units of their own maximum.
+__device__ __forceinline__ float inverse_of_scale(float s) { return s >= 0x1p-40f && s <= 0x1p40f ? __builtin_amdgcn_rcpf(s) * (1.0f / kPScale) : 0.0f; }
+// A reference that exponents are taken relative to.  Whole where weights have two terms, so that differences to scales that are powers of
+// two are exact; the largest weight itself where they have one, so that this one, which can be nearly all of them, is a power of two.
+template <class T> __device__ __forceinline__ float reference(float x) { return kPTerms<T> == 1 ? x : floorf(x); }
 
 __device__ __forceinline__ f16x2 as_f16x2(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
 
@@ -217,9 +233,9 @@ __device__ __forceinline__ void arguments_now(const AttendArgs& a, const Partial
 // and the next tile is under way while one is computed.  Codes become 16-bit floats, which hold both kinds exactly.
 // Queries are scaled by a power of two to just under 2^15 and rounded to 16-bit floats (nothing is lost of bf16 and f16 but what
 // lies 2^-29 under the row's largest element); 32-bit queries are split into two terms.  A block's key scale multiplies the
-// scores; its value scale, over the largest of the table's, multiplies the probabilities, which as 16-bit floats in units of 2^-11
-// reach down to 2^-35 of the reference: 2^-11 of each is rounded away for bf16 rows (whose outputs keep 2^-8), and a second term
-// takes that up for the others.  Sums, maxima and outputs are in 32 bits.
+// scores, its value scale goes into the weights by way of their exponents.  Weights as 16-bit floats in units of 2^-11 reach down to
+// 2^-35 of the row's largest: 2^-12 of each is rounded away for bf16 rows (whose outputs keep 2^-9), and a second term takes that up for
+// the others.  Sums, maxima and outputs are in 32 bits.
 // A workgroup's start is a chain of loads that wait for one another (length, table, codes; for lists: ids, table, codes): the first
 // tile's codes are asked for as soon as the table is there, and queries and scales are made ready meanwhile.
 // Measured (memory bounds the long ones, that chain the short ones): 64 requests of 1 to 8192 tokens, 8 heads of 128 dims, 540 MB: 113 us,
@@ -234,9 +250,11 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     static_assert(FOUND || kTable / 16 <= kThreads);
     constexpr int kOutLd = DP + 4, kJoin = NW == 1 ? 1 : NW / 2;
     __shared__ uint32_t ent_row[kEntries];                      // first row of a block's (a token's) codes, in rows of dim bytes; ~0: of no block
-    __shared__ __align__(16) float ent_k[kEntries], ent_v[kEntries];         // its scales; key scale -1: of no block
+    // its key scale (-1: of no block), its value scale in base 2, and that one's inverse
+    __shared__ __align__(16) float ent_k[FOUND ? kEntries : 1], ent_v[FOUND ? kEntries : 1], ent_z[FOUND ? kEntries : 1];
+    __shared__ __align__(16) float4 ent[FOUND ? 1 : kEntries];
     __shared__ __align__(16) float join[kJoin][16 * MT][kOutLd];
-    __shared__ float join_m[NW][16 * MT], join_l[NW][16 * MT], red[NW];
+    __shared__ float join_m[NW][16 * MT], join_v[NW][16 * MT], join_l[NW][16 * MT];
     __shared__ uint32_t red_n[NW];
 
     arguments_now(a, parts);
@@ -320,10 +338,12 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     f16x8 q[MT][KS][QT];
     float factor[MT];                                           // of the products: scores in base 2
     f32x4 o[MT][VB];
-    float top[MT], sum[MT], unit_v = 0.0f;
+    // references of the weights, and of the sums of probabilities, which are the weights' up to the first unusual scale
+    float top_v[MT], top[MT], sum[MT];
+    bool far = false;                                           // there has been one
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
-        top[mt] = -__builtin_inff();
+        top[mt] = top_v[mt] = -__builtin_inff();
         sum[mt] = 0.0f;
 #pragma unroll
         for (int i = 0; i < VB; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -365,7 +385,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
             n = __builtin_amdgcn_readfirstlane(kept);
             if (n == 0) return false;
             __syncthreads();
-            if (tid < kTile) { ent_row[n + tid] = ent_row[n - 1]; ent_k[n + tid] = 0.0f; ent_v[n + tid] = 0.0f; }
+            if (tid < kTile) { ent_row[n + tid] = ent_row[n - 1]; ent_k[n + tid] = 0.0f; ent_v[n + tid] = -__builtin_inff(); ent_z[n + tid] = 1.0f; }
             __syncthreads();
             return true;
         } else {
@@ -467,40 +487,22 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
     while (c0 < end) {
         if (some) {
-            // the entries' scales, and the largest value scale
-            float largest = 0.0f;
+            // the entries' scales
 #pragma unroll
             for (uint32_t e = 0; e < kMine; e++) {
                 if constexpr (FOUND) {
                     if (bh[e] != ~0u) {
                         const float sv = a.v_scale[bh[e]];
                         ent_k[at[e]] = a.k_scale[bh[e]];
-                        ent_v[at[e]] = sv;
-                        largest = fmaxf(largest, sv);
+                        ent_v[at[e]] = log2_of_scale(sv);
+                        ent_z[at[e]] = inverse_of_scale(sv);
                     }
                 } else if (tid <= ((c1 - 1) >> bs_log) - e0) {
-                    const float sv = bh[0] != ~0u ? a.v_scale[bh[0]] : 0.0f;
-                    ent_k[tid] = bh[0] != ~0u ? a.k_scale[bh[0]] : -1.0f;
-                    ent_v[tid] = sv;
-                    largest = sv;
+                    const float sv = bh[0] != ~0u ? a.v_scale[bh[0]] : 1.0f;
+                    ent[tid] = make_float4(bh[0] != ~0u ? a.k_scale[bh[0]] : -1.0f, log2_of_scale(sv), inverse_of_scale(sv), 0.0f);
                 }
             }
-            largest = wave_max_not_negative(largest);
-            if (lane == 0) red[wave] = largest;
             __syncthreads();
-#pragma unroll
-            for (int w = 0; w < NW; w++) largest = fmaxf(largest, red[w]);
-            if (largest > unit_v) {                             // outputs are in units of the largest scale so far
-                if (unit_v > 0.0f) {                            // (never the other way: outputs in units of a block of zeros' scale would overflow)
-                    const float change = unit_v / largest;
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                        for (int i = 0; i < VB; i++) o[mt][i] *= change;
-                }
-                unit_v = largest;
-            }
-            const float per_v = unit_v > 0.0f ? kPScale / unit_v : 0.0f;
 
             auto take = [&](auto buf, uint32_t j) {
                 const uint32_t i0 = 32 * j, ahead = j + DEPTH * NW;
@@ -523,22 +525,28 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
                     next = locate(ahead);
                     fetch_keys(buf, ahead, next);
                 }
-                float fk[2][4], pw[2][4];                       // the scales of this lane's tokens 4g + r of both halves
-                bool gone[2] = {false, false}, ragged;
+                float fk[2][4], lv[2][4], inverse[2][4];        // the scales of this lane's tokens 4g + r of both halves
+                bool gone[2] = {false, false}, ragged, odd = false;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     if constexpr (FOUND) {
-                        const float4 x = *reinterpret_cast<const float4*>(&ent_k[i0 + 16 * h + 4 * g]), y = *reinterpret_cast<const float4*>(&ent_v[i0 + 16 * h + 4 * g]);
+                        const float4 x = *reinterpret_cast<const float4*>(&ent_k[i0 + 16 * h + 4 * g]), y = *reinterpret_cast<const float4*>(&ent_v[i0 + 16 * h + 4 * g]),
+                                     z = *reinterpret_cast<const float4*>(&ent_z[i0 + 16 * h + 4 * g]);
                         fk[h][0] = x.x; fk[h][1] = x.y; fk[h][2] = x.z; fk[h][3] = x.w;
-                        pw[h][0] = y.x * per_v; pw[h][1] = y.y * per_v; pw[h][2] = y.z * per_v; pw[h][3] = y.w * per_v;
+                        lv[h][0] = y.x; lv[h][1] = y.y; lv[h][2] = y.z; lv[h][3] = y.w;
+                        inverse[h][0] = z.x; inverse[h][1] = z.y; inverse[h][2] = z.z; inverse[h][3] = z.w;
+                        odd |= __ballot(fminf(fminf(z.x, z.y), fminf(z.z, z.w)) == 0.0f) != 0;
                     } else {
                         const uint32_t e = (min(c0 + i0 + 16 * h, c1 - 1) >> bs_log) - e0;
-                        const float x = ent_k[e], y = ent_v[e] * per_v;
+                        const float4 x = ent[e];
 #pragma unroll
-                        for (int r = 0; r < 4; r++) { fk[h][r] = x; pw[h][r] = y; }
-                        gone[h] = __builtin_amdgcn_readfirstlane(__float_as_uint(x)) >> 31;
+                        for (int r = 0; r < 4; r++) { fk[h][r] = x.x; lv[h][r] = x.y; inverse[h][r] = x.z; }
+                        gone[h] = __builtin_amdgcn_readfirstlane(__float_as_uint(x.x)) >> 31;
+                        odd |= __builtin_amdgcn_readfirstlane(__float_as_uint(x.z)) == 0;
                     }
                 }
+                const bool was_far = far;
+                far = far || odd;
                 if constexpr (FOUND) ragged = i0 + 32 > n;
                 else ragged = c0 + i0 + 32 > least || c0 + i0 + 32 > c1 || gone[0] || gone[1];
                 f16x8 p[MT][PT];
@@ -557,29 +565,52 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
                             for (int r = 0; r < 4; r++) x[h][r] = 16 * h + r < left && !gone[h] ? x[h][r] : -__builtin_inff();
                     }
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < 2; h++) {
+                        if constexpr (FOUND) {
 #pragma unroll
-                        for (int r = 0; r < 4; r++) local = fmaxf(local, x[h][r]);
-                    if (__ballot(local > top[mt] + kLead)) {    // rare after the first tile
-                        const float now = fmaxf(top[mt], max_over_groups(local));
-                        const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
-                        top[mt] = now;
-                        sum[mt] *= shrink;
+                            for (int r = 0; r < 4; r++) local = fmaxf(local, x[h][r] + lv[h][r]);
+                        } else {
+                            local = fmaxf(local, fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3])) + lv[h][0]);
+                        }
+                    }
+                    if (far || __ballot(local > top_v[mt] + kLead)) {          // rare after the first tile, but for unusual scales
+                        const float before = top_v[mt], now = fmaxf(before, reference<T>(max_over_groups(local)));
+                        const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(before - now);
+                        top_v[mt] = now;
 #pragma unroll
                         for (int i = 0; i < VB; i++) o[mt][i] *= shrink;
-                    }
-                    const float ref = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+                        if (!far) {
+                            sum[mt] *= shrink;
+                        } else {                                // the sum by itself
+                            if (!was_far) top[mt] = before;
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                            for (int i = 0; i < 8; i++) inverse[i / 4][i % 4] = 0.0f;
+                            float most_x = -__builtin_inff();
+#pragma unroll
+                            for (int i = 0; i < 8; i++) most_x = fmaxf(most_x, x[i / 4][i % 4]);
+                            const float now_x = fmaxf(top[mt], reference<T>(max_over_groups(most_x))), ref = now_x == -__builtin_inff() ? 0.0f : now_x;
+                            sum[mt] *= __builtin_amdgcn_exp2f(top[mt] - ref);
+                            top[mt] = now_x;
+#pragma unroll
+                            for (int i = 0; i < 8; i++) sum[mt] += __builtin_amdgcn_exp2f(x[i / 4][i % 4] - ref);
+                        }
+                    }
+                    // (the factor of 2^11 in the exponent costs bits of it, which 32-bit rows keep)
+                    constexpr bool kApart = sizeof(T) == 4;
+                    const float ref = (top_v[mt] == -__builtin_inff() ? 0.0f : top_v[mt]) - (kApart ? 0.0f : kPScaleLog);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float part_sum = 0.0f;
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            const float y = __builtin_amdgcn_exp2f(x[h][r] - ref);
-                            sum[mt] += y;
-                            const float w = y * pw[h][r];
+                            const float w = __builtin_amdgcn_exp2f(x[h][r] + (lv[h][r] - ref)) * (kApart ? kPScale : 1.0f);
+                            part_sum = FOUND ? __builtin_fmaf(w, inverse[h][r], part_sum) : part_sum + w;
                             const _Float16 hi = (_Float16)w;
                             p[mt][0][4 * h + r] = hi;
                             if constexpr (PT == 2) p[mt][1][4 * h + r] = (_Float16)(w - (float)hi);
                         }
+                        sum[mt] = FOUND ? sum[mt] + part_sum : __builtin_fmaf(part_sum, inverse[h][0], sum[mt]);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < VW; i++) {
@@ -616,20 +647,21 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     __syncthreads();
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
+        if (!far) top[mt] = top_v[mt];
         sum[mt] = sum_over_groups(sum[mt]);
-        if (g == 0) { join_m[wave][16 * mt + m] = top[mt]; join_l[wave][16 * mt + m] = sum[mt]; }
+        if (g == 0) { join_m[wave][16 * mt + m] = top[mt]; join_v[wave][16 * mt + m] = top_v[mt]; join_l[wave][16 * mt + m] = sum[mt]; }
     }
     __syncthreads();
-    auto ref_of = [&](uint32_t r) {
-        float x = join_m[0][r];
+    auto ref_of = [&](const float (&tops)[NW][16 * MT], uint32_t r) {
+        float x = tops[0][r];
 #pragma unroll
-        for (int w = 1; w < NW; w++) x = fmaxf(x, join_m[w][r]);
+        for (int w = 1; w < NW; w++) x = fmaxf(x, tops[w][r]);
         return x == -__builtin_inff() ? 0.0f : x;
     };
     auto put = [&](bool add) {
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            const float f = __builtin_amdgcn_exp2f(top[mt] - ref_of(16 * mt + m));
+            const float f = __builtin_amdgcn_exp2f(top_v[mt] - ref_of(join_v, 16 * mt + m));
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -653,22 +685,21 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
         for (int w = 1; w < kJoin; w++) x += join[w][r][d];
         return x;
     };
-    const float unit_o = unit_v / kPScale;
     for (uint32_t r = wave; r < 16 * MT && r0 + r < n_r; r += NW) {
         const uint32_t i = of_group(a, r0 + r);
         const size_t to = (size_t)(first + i) * a.q_heads + head * group + (r0 + r - i * group);
-        const float ref = ref_of(r);
+        const float ref = ref_of(join_m, r), ref_v = ref_of(join_v, r);
         float l = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) l += join_l[w][r] * __builtin_amdgcn_exp2f(join_m[w][r] - ref);
-        const float inv = l == 0.0f ? 0.0f : unit_o / l;
+        const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ref_v - ref - kPScaleLog) / l;
         if (parts.n_splits == 1) {
             for (uint32_t d = lane; d < dim; d += 64) ((T*)a.out)[to * dim + d] = from_float<T>(joined(r, d) * inv);
-            if (lane == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+            if (lane == 0 && a.lse) a.lse[to] = l == 0.0f ? -__builtin_inff() : log2_of_sum(ref, l) * 0.6931471805599453f;
         } else {
             const size_t at = to * parts.n_splits + split;
             for (uint32_t d = lane; d < dim; d += 64) parts.out[at * dim + d] = joined(r, d) * inv;
-            if (lane == 0) parts.lse[at] = l == 0.0f ? -__builtin_inff() : ref + __builtin_amdgcn_logf(l);
+            if (lane == 0) parts.lse[at] = l == 0.0f ? -__builtin_inff() : log2_of_sum(ref, l);
         }
     }
 }
@@ -682,9 +713,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
 // workgroups are too few to hide them.  (Up to 64 dims, where two such workgroups fit a compute unit: 163 rows each of eight requests over
 // 1000 tokens, 16 heads: 34.3 us, 37.4 without.  At 128 dims only one fits, and the rounds cost more than the steps: 300 rows each of four over 700
 // tokens, 43.8 -> 51.3.)
-// Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel, but that a block's value scale goes
-// into the exponent instead of being multiplied in: weights are 2^(score - maximum + log2 of the scale over the largest), their
-// sum is put right by the inverse per 16 tokens.
+// Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel.
 // What bounds it is issue: per tile and wavefront about 260 vector instructions and 32 exponentials (1400 cycles; the softmax 60 % of them, decoding
 // a third) and 64 matrix instructions (1000), of which the registers leave room for two wavefronts a SIMD to overlap.  Three prompts of 900 rows over
 // 4000 tokens, 32 query heads of 128 dims, 156 GFLOP: 264 to 280 us, 560 to 590 TFLOP/s.
@@ -698,8 +727,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
     static_assert(kScanTokens / 16 <= 256 && (HALVES == 1 || NBUF == 2));
     constexpr int kAll = kWaves * HALVES;                       // wavefronts
     __shared__ uint32_t ent_row[kEntries], some[kAll];        // first row of a block's codes, in rows of dim bytes; ~0: of no block
-    __shared__ float red[kAll];
-    __shared__ __align__(16) float4 ent[kEntries];              // key scale, log2 of the weights' factor, its inverse; key scale -1: there is no block
+    __shared__ __align__(16) float4 ent[kEntries];              // key scale (-1: there is no block), value scale in base 2, its inverse
     __shared__ __align__(16) _Float16 keys[NBUF * HALVES][kTokens * kKeyLd];
     __shared__ __align__(16) _Float16 vals[NBUF * HALVES][DP * kTokens];
     auto val_at = [](uint32_t d, uint32_t oct) { return d * kTokens + 8 * (oct ^ ((d >> 1) & 7)); };
@@ -746,10 +774,11 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
     f16x8 q[MT][KS][QT];
     float factor[MT];
     f32x4 o[MT][DT];
-    float top[MT], sum[MT], unit_v = 0.0f;
+    float top_v[MT], top[MT], sum[MT];                          // (as in attend_rows_kernel)
+    bool far = false;
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
-        top[mt] = -__builtin_inff();
+        top[mt] = top_v[mt] = -__builtin_inff();
         sum[mt] = 0.0f;
 #pragma unroll
         for (int i = 0; i < DT; i++) o[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -841,12 +870,15 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
                     for (int qt = 0; qt < QT; qt++)
                         s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[mt][ks][qt], ks + qt ? s[mt][t] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             }
-        bool gone[4], any_gone = false;
+        bool gone[4], any_gone = false, odd = false;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             gone[t] = __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].x)) >> 31;
             any_gone |= gone[t];
+            odd |= __builtin_amdgcn_readfirstlane(__float_as_uint(x[t].z)) == 0;
         }
+        const bool was_far = far;
+        far = far || odd;
         const bool ragged = t0 + kTokens > least || t0 + kTokens > c1 || any_gone;
         float f[MT][4], ref[MT];
 #pragma unroll
@@ -862,17 +894,34 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 f[mt][t] = fmaxf(x[t].x * factor[mt], 0x1p-126f);               // (not 0, which masked scores would make NaN)
-                local = fmaxf(local, f[mt][t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
+                const float most_s = fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3]));
+                local = fmaxf(local, __builtin_fmaf(f[mt][t], most_s, x[t].y));
             }
-            if (__ballot(local > top[mt] + kLead)) {
-                const float now = fmaxf(top[mt], max_over_groups(local));
-                const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - now);
-                top[mt] = now;
-                sum[mt] *= shrink;
+            if (far || __ballot(local > top_v[mt] + kLead)) {
+                const float before = top_v[mt], now = fmaxf(before, reference<T>(max_over_groups(local)));
+                const float shrink = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(before - now);
+                top_v[mt] = now;
 #pragma unroll
                 for (int i = 0; i < DT; i++) o[mt][i] *= shrink;
+                if (!far) {
+                    sum[mt] *= shrink;
+                } else {                                        // the sum by itself
+                    if (!was_far) top[mt] = before;
+#pragma unroll
+                    for (int t = 0; t < 4; t++) x[t].z = 0.0f;
+                    float most_x = -__builtin_inff();
+#pragma unroll
+                    for (int t = 0; t < 4; t++) most_x = fmaxf(most_x, f[mt][t] * fmaxf(fmaxf(s[mt][t][0], s[mt][t][1]), fmaxf(s[mt][t][2], s[mt][t][3])));
+                    const float now_x = fmaxf(top[mt], reference<T>(max_over_groups(most_x))), by = now_x == -__builtin_inff() ? 0.0f : now_x;
+                    sum[mt] *= __builtin_amdgcn_exp2f(top[mt] - by);
+                    top[mt] = now_x;
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) sum[mt] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][t][r], f[mt][t], -by));
+                }
             }
-            ref[mt] = top[mt] == -__builtin_inff() ? 0.0f : top[mt];
+            ref[mt] = (top_v[mt] == -__builtin_inff() ? 0.0f : top_v[mt]) - kPScaleLog;
         }
         // the two halves of the tile: weights of one while the other's meet the values, and the next tile's codes become
         // 16-bit floats meanwhile (their loads were issued before the scores)
@@ -946,28 +995,9 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
     for (int mt = 0; mt < MT; mt++) factor[mt] = query_operands<T, CODES, KS, QT>(a, raw[mt], q[mt]);
     while (c0 < end) {
         if (has) {
-            // the entries' scales; weights get a block's value scale over the largest by way of the exponent (a scale of 0 next to others
-            // counts as 2^-60 of it: weights that vanish as 16-bit floats)
-            const float sk = bh != ~0u ? a.k_scale[bh] : -1.0f, sv = bh != ~0u ? a.v_scale[bh] : 0.0f;
-            float largest = wave_max_not_negative(sv);
-            if (lane == 0) red[of_all] = largest;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kAll; w++) largest = fmaxf(largest, red[w]);
-            if (largest > unit_v) {                             // outputs are in units of the largest scale so far
-                if (unit_v > 0.0f) {
-                    const float change = unit_v / largest;
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                        for (int i = 0; i < DT; i++) o[mt][i] *= change;
-                }
-                unit_v = largest;
-            }
-            if (tid <= ((c1 - 1) >> bs_log) - e0) {
-                const float w = unit_v > 0.0f ? fmaxf(sv * (kPScale / unit_v), 0x1p-60f) : 1.0f;
-                ent[tid] = make_float4(sk, __builtin_amdgcn_logf(w), 1.0f / w, 0.0f);
-            }
+            // the entries' scales
+            const float sk = bh != ~0u ? a.k_scale[bh] : -1.0f, sv = bh != ~0u ? a.v_scale[bh] : 1.0f;
+            if (tid <= ((c1 - 1) >> bs_log) - e0) ent[tid] = make_float4(sk, log2_of_scale(sv), inverse_of_scale(sv), 0.0f);
             const int own = NBUF * half;                        // this half's buffers
             store(own);
             __syncthreads();
@@ -994,37 +1024,47 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
 
     if constexpr (HALVES == 2) {
         // the second half's softmaxes go to the first through the tiles' memory, lane by lane
-        constexpr int kLd = MT * (4 * DT + 2);
+        constexpr int kPer = 4 * DT + 3, kLd = MT * kPer;
         static_assert(sizeof(keys) >= 256 * kLd * 4);
         float* mine = reinterpret_cast<float*>(&keys[0][0]) + wave * 64 + lane;
         __syncthreads();
         if (half == 1) {
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
-                mine[256 * (mt * (4 * DT + 2))] = top[mt];
-                mine[256 * (mt * (4 * DT + 2) + 1)] = sum[mt];
+                if (!far) top[mt] = top_v[mt];
+                float* to = mine + 256 * (mt * kPer);
+                to[0] = top[mt];
+                to[256] = sum[mt];
+                to[512] = top_v[mt];
 #pragma unroll
                 for (int i = 0; i < DT; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) mine[256 * (mt * (4 * DT + 2) + 2 + 4 * i + r)] = o[mt][i][r];
+                    for (int r = 0; r < 4; r++) to[256 * (3 + 4 * i + r)] = o[mt][i][r];
             }
         }
         __syncthreads();
         if (half == 1) return;
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            const float there = mine[256 * (mt * (4 * DT + 2))], now = fmaxf(top[mt], there), ref = now == -__builtin_inff() ? 0.0f : now;
-            const float x = __builtin_amdgcn_exp2f(top[mt] - ref), y = __builtin_amdgcn_exp2f(there - ref);
-            top[mt] = now;
-            sum[mt] = sum[mt] * x + mine[256 * (mt * (4 * DT + 2) + 1)] * y;
+            const float* from = mine + 256 * (mt * kPer);
+            auto both = [](float& mine_, float there, float& x, float& y) {
+                const float now = fmaxf(mine_, there), ref = now == -__builtin_inff() ? 0.0f : now;
+                x = __builtin_amdgcn_exp2f(mine_ - ref);
+                y = __builtin_amdgcn_exp2f(there - ref);
+                mine_ = now;
+            };
+            if (!far) top[mt] = top_v[mt];
+            float x, y;
+            both(top[mt], from[0], x, y);
+            sum[mt] = sum[mt] * x + from[256] * y;
+            both(top_v[mt], from[512], x, y);
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) o[mt][i][r] = o[mt][i][r] * x + mine[256 * (mt * (4 * DT + 2) + 2 + 4 * i + r)] * y;
+                for (int r = 0; r < 4; r++) o[mt][i][r] = o[mt][i][r] * x + from[256 * (3 + 4 * i + r)] * y;
         }
     }
 
-    const float unit_o = unit_v / kPScale;
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
         const float l = sum_over_groups(sum[mt]);
@@ -1032,7 +1072,9 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
         if (r >= n_r) continue;
         const uint32_t i = of_group(a, r);
         const size_t to = (size_t)(rows.first + i) * a.q_heads + kv * group + (r - i * group);
-        const float inv = l == 0.0f ? 0.0f : unit_o / l, lse = l == 0.0f ? -__builtin_inff() : top[mt] + __builtin_amdgcn_logf(l);
+        if (!far) top[mt] = top_v[mt];
+        const float unit = top_v[mt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top_v[mt] - top[mt] - kPScaleLog);
+        const float inv = l == 0.0f ? 0.0f : unit / l, lse = l == 0.0f ? -__builtin_inff() : log2_of_sum(top[mt], l);
         if (parts.n_splits == 1) {
             T* out = (T*)a.out + to * dim + 4 * g;
 #pragma unroll

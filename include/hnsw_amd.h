@@ -297,7 +297,9 @@ int hnsw_amd_vector_data(hnsw_amd_index* h, const float** out);
  * All pointers below (but the descriptor itself) are device memory of `device`.  The calls are asynchronous on `stream` (a hipStream_t of
  * that device, NULL = its default stream), allocate nothing, wait for nothing and can be captured into a graph; calls that
  * touch different buffers may overlap.  What lies in device memory cannot be refused by the host: each call says what it
- * does with block numbers, slots and lengths that are out of range (none of them reads or writes outside the buffers). */
+ * does with block numbers, slots and lengths that are out of range (none of them reads or writes outside the buffers).
+ * The codes and scales of a request's tokens are numbers, and scales are finite and not negative (append writes no others);
+ * what a row gives that sees others is not defined. */
 enum { HNSW_AMD_CODES_I8 = 0,         /* signed bytes, -127..127 */
        HNSW_AMD_CODES_E4M3 = 1 };     /* 8-bit floats (4 exponent, 3 mantissa bits; largest 448, no infinities) */
 enum { HNSW_AMD_TYPE_F32 = 0, HNSW_AMD_TYPE_F16 = 1, HNSW_AMD_TYPE_BF16 = 2 };   /* of rows, queries and outputs */
