@@ -70,7 +70,8 @@ class TokenCache:
         return cls(k, v, torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
 
     def append(self, k, v, slots) -> None:
-        """Quantises the rows k, v [rows, n_heads, dim] into their slots [rows] int64 (as cache_plan lays them out; -1 is skipped)."""
+        """Quantises the rows k, v [rows, n_heads, dim] into their slots [rows] int64 (as cache_plan lays them out: a block's rows next to each
+        other, their slots ascending; -1 is skipped)."""
         self._b.append(self._c, k, v, slots)
 
     def read(self, slots, dtype=None):

@@ -171,12 +171,13 @@ __device__ __forceinline__ int scale_exponent(float peak, float most)
     return e;
 }
 
-// Four wavefronts take a.span rows of one head's keys or values, run by run (a run: rows that lie next to each other in one block).  First the
+// Four wavefronts take a.span rows of one head's keys or values, run by run (a run: rows whose slots follow one another in one block).  First the
 // rows' largest value, which gives the block's scale; where that raises the scale of a block that held earlier tokens, their codes move to it;
 // then the rows' codes.  What a wavefront has looked at first stays in its registers between the two.  Short runs (single tokens of many
-// requests) are latency: a wavefront takes each by itself.  Long runs (prompts) are memory: all four wavefronts take each.
+// requests) are latency: a wavefront takes each by itself.  Long runs (prompts) are memory: all four wavefronts take each, and so they do
+// with runs of one block that slots which are left out keep apart, one after the other.
 // A power of two as scale makes x / scale exact, so a code is ONE rounding of x, and moving codes to a larger scale one more.
-// (64 rows of 8 heads of 128 dims: 3.9 us.  Three prompts, 21500 rows, 132 MB: 40 us, 3.3 TB/s: slots, rows, largest value and codes follow
+// (64 rows of 8 heads of 128 dims: 4.2 us.  Three prompts, 21500 rows, 132 MB: 41.5 us, 3.2 TB/s: slots, rows, largest value and codes follow
 // one another in a workgroup, and seven workgroups a compute unit hide most of that; five, with the rows kept as 32-bit values: 45 us.)
 template <class T, int CODES, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
@@ -201,16 +202,16 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
         const int64_t slot_l = at >= 0 && at < (int64_t)a.n_rows ? a.slots[at] : -1;
         const bool valid = slot_l >= 0 && slot_l < n_slots;
         const int64_t prev_l = __shfl_up(slot_l, 1);
-        const bool follows = valid && (slot_l & (bs - 1)) != 0 && prev_l == slot_l - 1 && lane > 0;      // the row before is of the same run
-        const unsigned long long follow = __ballot(follows);
-        unsigned long long firsts = __ballot(valid && !follows) & ~(1ull << 63) & ~1ull;
+        const bool after = valid && lane > 0 && (uint64_t)(slot_l ^ prev_l) < bs && prev_l < slot_l;     // the row before is of the same block, and of
+        const unsigned long long follow = __ballot(after && prev_l == slot_l - 1);                           // the same run, or slots between the two
+        const unsigned long long behind = __ballot(after) & ~follow;                                         // are left out
+        unsigned long long firsts = __ballot(valid && !after) & ~(1ull << 63) & ~1ull;
         if (end - base < 62) firsts &= (2ull << (end - base)) - 1;
 
-        // The run of n rows that begins in lane l, by wavefront `sub` of `of`.
-        auto take = [&](int l, uint32_t n, uint32_t sub, auto of) {
+        // The run of n rows from row0 and `slot` on, by wavefront `sub` of `of`.
+        auto take = [&](uint32_t row0, int64_t slot, uint32_t n, uint32_t sub, auto of) {
             constexpr uint32_t kOf = of.value;
-            const uint32_t row0 = base + l - 1, my_row = sub * rows_per_wave + wave_row, step = rows_per_wave * kOf;
-            const int64_t slot = ((int64_t)__builtin_amdgcn_readlane((int)(slot_l >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)slot_l, l);
+            const uint32_t my_row = sub * rows_per_wave + wave_row, step = rows_per_wave * kOf;
             const uint32_t block = (uint32_t)(slot >> bs_log), off = (uint32_t)(slot & (bs - 1));
             float* scale = a.scale[part] + (size_t)block * a.n_heads + head;
             uint8_t* codes = a.codes[part] + ((size_t)block * a.n_heads + head) * bs * dim;
@@ -285,29 +286,47 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
             if constexpr (kOf > 1) __syncthreads();             // (all have read the old scale and the peaks)
             if (lane == 0 && sub == 0) *scale = now;
         };
-        auto run_of = [&](int l) {
-            uint32_t n = 1 + (uint32_t)__builtin_ctzll(~(follow >> (l + 1)));
-            if (l + n == 64) {                                  // the run goes on behind what the wavefront has in view
-                const int64_t slot = ((int64_t)__builtin_amdgcn_readlane((int)(slot_l >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)slot_l, l);
-                const uint32_t row0 = base + l - 1, off = (uint32_t)(slot & (bs - 1));
-                for (;;) {
-                    const uint32_t i = n + lane;
-                    const bool more = off + i < bs && (uint64_t)row0 + i < a.n_rows && a.slots[row0 + i] == slot + i;
-                    const unsigned long long more_l = __ballot(more);
-                    if (more_l != ~0ull) { n += (uint32_t)__builtin_ctzll(~more_l); break; }
-                    n += 64;
-                }
+        // the run's length, of which n rows are known
+        auto extend = [&](uint32_t row0, int64_t slot, uint32_t n) {
+            const uint32_t off = (uint32_t)(slot & (bs - 1));
+            for (;;) {
+                const uint32_t i = n + lane;
+                const bool more = off + i < bs && (uint64_t)row0 + i < a.n_rows && a.slots[row0 + i] == slot + i;
+                const unsigned long long more_l = __ballot(more);
+                if (more_l != ~0ull) return n + (uint32_t)__builtin_ctzll(~more_l);
+                n += 64;
             }
-            return n;
         };
+        auto whole = [](int64_t x, int l) { return ((int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, l); };
         // (the same runs in the same order in all four wavefronts, so that all of them meet at the barriers)
         uint32_t turn = 0;
         while (firsts) {
             const int l = __builtin_ctzll(firsts);
             firsts &= firsts - 1;
-            const uint32_t n = run_of(l);
-            if (n > 2 * rows_per_wave) take(l, n, wave, std::integral_constant<int, 4>{});
-            else if (turn++ % 4 == wave) take(l, n, 0u, std::integral_constant<int, 1>{});
+            uint32_t row0 = base + l - 1, n = 1 + (uint32_t)__builtin_ctzll(~(follow >> (l + 1)));
+            int64_t slot = whole(slot_l, l);
+            if (l + n == 64) n = extend(row0, slot, n);         // the run goes on behind what the wavefront has in view
+            // the slot of the next row of this block, -1: there is none
+            auto next = [&]() -> int64_t {
+                if ((uint32_t)(slot & (bs - 1)) + n >= bs || (uint64_t)row0 + n >= a.n_rows) return -1;
+                const int64_t x = whole(a.slots[row0 + n], 0);
+                return x >= slot + n && (x >> bs_log) == (slot >> bs_log) ? x : -1;
+            };
+            const bool gap = __builtin_expect(l + n < 64, 1) ? (behind >> (l + n)) & 1 : next() >= 0;
+            if (gap || n > 2 * rows_per_wave) {
+                for (;;) {
+                    take(row0, slot, n, wave, std::integral_constant<int, 4>{});
+                    if (__builtin_expect(!gap, 1)) break;
+                    const int64_t x = next();
+                    if (x < 0) break;
+                    row0 += n;
+                    slot = x;
+                    n = extend(row0, slot, 1);
+                    __syncthreads();                            // (scale and codes of the rows before)
+                }
+            } else if (turn++ % 4 == wave) {
+                take(row0, slot, n, 0u, std::integral_constant<int, 1>{});
+            }
         }
     }
 }

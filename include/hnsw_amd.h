@@ -333,8 +333,9 @@ int hnsw_amd_cache_plan_device(const int32_t* d_lens, const int32_t* d_grow, uin
  * the codes' range; it never shrinks while the block holds earlier tokens, and where a new token raises it the earlier codes
  * are rounded to the new scale.  Rows whose run begins at a block's first slot start the block afresh.  Codes round to
  * nearest, ties to even; infinities become the largest code, NaN becomes 0.  Slots outside the cache are skipped.  The rows
- * of one block must lie next to each other with ascending slots (as cache_plan lays them out): a block that is named in two
- * separate places of one call ends with unspecified codes and scale. */
+ * of one block must lie next to each other with ascending slots (as cache_plan lays them out); behind slots that are left out
+ * they are written as by a further call.  A block that is named in two separate places of one call, or with slots that do not
+ * ascend, ends with unspecified codes and scale. */
 int hnsw_amd_cache_append_device(const hnsw_amd_token_cache* cache, const void* d_k, const void* d_v, uint32_t n_rows, uint32_t row_type,
                                  int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, const int64_t* d_slots,
                                  int device, void* stream);
