@@ -392,7 +392,14 @@ void cache_plan(const int32_t* lens, const int32_t* grow, uint32_t n_requests, i
     if (width < 1 || (uint64_t)width * block_tokens > 0x7fffffffull) throw std::invalid_argument("cache_plan: the table's width in tokens must be 1..2^31 - 1");
     if (n_blocks < 1 || n_blocks > 0x7fffffffu) throw std::invalid_argument("cache_plan: n_blocks must be 1..2^31 - 1");
     if (n_slots > 0x7fffffffu) throw std::invalid_argument("cache_plan: n_slots must be below 2^31");
-    if (lens == lens_out || state == state_out) throw std::invalid_argument("cache_plan: the new lengths and ring state need buffers of their own");
+    // every workgroup reads the inputs, while others write
+    const uint64_t n = n_requests;
+    const struct { const void* at; uint64_t bytes; } in[] = {{lens, 4 * n}, {grow, 4 * n}, {state, 16}},
+                                                     out[] = {{slots, 8ull * n_slots}, {cu_new, 4 * (n + 1)}, {lens_out, 4 * n}, {state_out, 16}, {status, 4}};
+    for (const auto& i : in)
+        for (const auto& o : out)
+            if ((uintptr_t)i.at < (uintptr_t)o.at + o.bytes && (uintptr_t)o.at < (uintptr_t)i.at + i.bytes)
+                throw std::invalid_argument("cache_plan: the results need buffers of their own");
     const OnDevice on(device);
     // A slot a thread, or four in a row where there are more than a few workgroups of them; 512 workgroups at most.  (64 requests, one slot
     // each: 6.0 us, 7.5 with four.  1000 requests, 318000 slots: 10.7 us, 11.9 with one; 14.3 with workgroups of 1024 whose first threads do

@@ -316,7 +316,7 @@ typedef struct {
  * ends (grow[b] == -1: its blocks go back to the ring).  Blocks are taken off the ring's head in the order of the requests
  * and entered into the table behind those the request holds; blocks given back go behind the tail and can be taken by later
  * calls.  Writes slots[0 .. n_slots) (the new tokens of request 0, then 1, ...; -1 behind the last one), cu_new[0 .. n_requests]
- * (new tokens before each request), lens_out and state_out, which may not be the inputs' buffers: a call that is repeated
+ * (new tokens before each request), lens_out and state_out.  No result may overlap lens, grow or state: a call that is repeated
  * with the same inputs gives the same results.  (A request's table row keeps its entries when it ends.)  *status is 0, or
  * says with HNSW_AMD_PLAN_* bits why nothing was done: then slots are -1, cu_new 0, lengths, state, table and ring as before.
  * n_requests <= 8192. */
