@@ -112,11 +112,27 @@ struct Cache {
 
 const char* const kCapsule = "hnsw_amd.token_cache";
 
+// Nothing here has a gradient, and none is lost without a word.
+void no_gradient(const at::Tensor& t, const char* name)
+{
+    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(name) + " requires a gradient: the token cache has none");
+}
+
+void no_gradient(const Cache& c)
+{
+    no_gradient(c.k, "k_codes");
+    no_gradient(c.v, "v_codes");
+    no_gradient(c.ks, "k_scale");
+    no_gradient(c.vs, "v_scale");
+}
+
 const Cache& cache(PyObject* o)
 {
     void* p = PyCapsule_GetPointer(o, kCapsule);
     if (!p) throw Raised{};
-    return *static_cast<const Cache*>(p);
+    const Cache& c = *static_cast<const Cache*>(p);
+    no_gradient(c);
+    return c;
 }
 
 // Rows [rows, heads, dim] of one of the three types, the last dimension contiguous.
@@ -126,7 +142,7 @@ uint32_t rows_of(const Cache& c, const at::Tensor& t, const char* name, int64_t 
         refuse(std::string(name) + " must be a [rows, " + std::to_string(heads) + ", " + std::to_string(c.c.dim) + "] tensor on " + c.device.str());
     if (t.stride(2) != 1) refuse(std::string(name) + ": the last dimension must be contiguous");
     if (t.size(0) >= INT64_C(1) << 31) refuse(std::string(name) + " has too many rows");
-    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(name) + " requires a gradient: the token cache has none");
+    no_gradient(t, name);
     return row_type(t, name);
 }
 
@@ -165,6 +181,10 @@ PyObject* py_cache(PyObject*, PyObject* const* args, Py_ssize_t n)
         need(v, "v_codes", k.scalar_type(), k.sizes(), device);
         need(ks, "k_scale", at::kFloat, {k.size(0), k.size(1)}, device);
         need(vs, "v_scale", at::kFloat, {k.size(0), k.size(1)}, device);
+        no_gradient(k, "k_codes");
+        no_gradient(v, "v_codes");
+        no_gradient(ks, "k_scale");
+        no_gradient(vs, "v_scale");
         for (int i = 0; i < 4; i++)
             if (k.size(i) > 0xffffffffll) refuse("TokenCache: an extent is out of range");
         Cache* c = new Cache{{k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), (uint32_t)k.size(0), (uint32_t)k.size(1), (uint32_t)k.size(2),
