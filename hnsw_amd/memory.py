@@ -83,11 +83,11 @@ class TokenMemory:
         """(out, lse, ids) of one query row for each request, q [requests, heads, dim], over the k tokens that the indexes find for each
         query head (scores with the sign of `scale`; ef: the search's breadth, 2 k unless given) and over the tokens that are not indexed."""
         torch, c = self._torch, self.cache
-        n, heads = q.shape[0], q.shape[1]
-        if n != len(self.host_lens):
-            raise ValueError("recall: one row for each request")
+        if q.dim() != 3 or q.shape[0] != len(self.host_lens) or q.shape[1] < 1 or q.shape[1] % c.n_heads or q.shape[2] != c.dim:
+            raise ValueError(f"recall: one row for each request, [{len(self.host_lens)}, a multiple of {c.n_heads} heads, {c.dim}]")
         if k < 1:
             raise ValueError("recall: k must be positive")
+        n, heads = q.shape[0], q.shape[1]
         ef, group = max(k, ef or 2 * k), heads // c.n_heads
         known = [x[1] if x else 0 for x in self.indexes]
         tail = max(a - i for a, i in zip(self.host_lens, known))
