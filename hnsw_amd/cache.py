@@ -81,8 +81,9 @@ class TokenCache:
     def attend(self, q, table, lens, *, cu_q=None, causal: bool = True, scale: float | None = None, max_len: int = 0):
         """(out, lse) of the queries q [rows, heads, dim] over all tokens of their requests; table [n, width], lens [n] int32.  Without
         cu_q each request has one row; with it ([n + 1] int32) request b has the rows cu_q[b] .. cu_q[b + 1], its last tokens; what the
-        result holds in rows behind the last request is not defined.  scale: 1 / sqrt(dim) unless given.  max_len: the longest length, if
-        the caller knows it (a hint for splitting the work; without it the workspace is for requests as long as the table is wide)."""
+        result holds in rows behind the last request is not defined.  (Single tokens of long requests are faster in a call of their own
+        than next to prompts.)  scale: 1 / sqrt(dim) unless given.  max_len: the longest length, if the caller knows it (a hint for splitting
+        the work; without it the workspace is for requests as long as the table is wide)."""
         return self._b.attend(self._c, q, table, lens, cu_q, causal, scale, max_len, None)
 
     def attend_found(self, q, table, lens, ids, *, cu_q=None, causal: bool = True, scale: float | None = None):

@@ -69,15 +69,19 @@ static Cut cut_work(uint32_t dim, uint32_t n_rows, uint32_t q_heads, uint32_t n_
     if (c.tiles) {
         // (cut above)
     } else if (c.mt == 1 && have >= 1024 && items <= 256) {
-        // short requests (lists) in number: a wavefront for each, nothing to join (64 requests x 32 lists of 100 entries: 18.8 us, 25.7 in
-        // chunks)
+        // short requests (lists) in number: a wavefront for each, nothing to join.  (Lists of 32, 100, 200 and 256 entries in 2048 workgroups: 8.4,
+        // 18.5, 27.7 and 31.8 us, in chunks 18.5, 23.9, 31.5 and 34.7; in 1024: 6.4, 11.3, 18.0 and 19.4, in chunks 11.2, 13.9, 19.0 and
+        // 20.4; in 768: 6.2, 10.2, 15.5 and 16.7, in chunks 7.8, 10.1, 14.3 and 15.4.)
         c.waves = 1;
         chunk = 256;
     } else if (c.mt == 1 && have < 512 && items <= 1024) {
-        // few short ones: one chunk, as a second launch to join more of them would cost more than it saves (one request, 8 heads of 777
-        // tokens of 64 dims: 9.7 us, 10.2 in chunks), and eight wavefronts for it (11.1 with four) where it is not so short that they
-        // cost more in starting (100 tokens: 6.4 us, 6.0 with four) and all fit the chip at once: beyond 64 dims one such workgroup to a compute
-        // unit (48 requests of up to 1000 tokens, 8 heads of 128 dims: 23.3 us, 17.6 with four)
+        // few short ones: one chunk, as a second launch to join more of them mostly costs more than it saves (300 and 1000 tokens of 128 dims,
+        // 504 workgroups: 11.8 and 25.4 us, in chunks 19.0 and 29.5; 256: 9.0 and 16.6, in chunks 12.1 and 18.5; 64: 8.6 and 12.5, in chunks 9.2
+        // and 10.9; and it would still win at 504 of 2000 tokens, 42.3 and 48.9, but not at 64 of 2000, 21.2 and 12.9).  Eight wavefronts for
+        // it where it is not so short that they cost more in starting (64 dims, 256 workgroups: 100 tokens 6.6 us, with four 6.2; 160: 6.9 and
+        // 7.0; 500: 8.7 and 9.2; 1000: 11.4 and 13.2; at 128 dims four are 0.3 to 0.6 us faster up to 500 tokens and 0.4 slower at 1000)
+        // and all fit the chip at once, beyond 64 dims one such workgroup to a compute unit (320 of 1000 tokens of 128 dims: 26.6, with
+        // four 19.3)
         c.waves = items > 128 && have <= (dim <= 64 ? 512 : 256) ? 8 : 4;
         chunk = 1024;
     } else {

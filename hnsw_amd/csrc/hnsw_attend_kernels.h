@@ -234,13 +234,13 @@ __device__ __forceinline__ void arguments_now(const AttendArgs& a, const Partial
 // Queries are scaled by a power of two to just under 2^15 and rounded to 16-bit floats (nothing is lost of bf16 and f16 but what
 // lies 2^-29 under the row's largest element); 32-bit queries are split into two terms.  A block's key scale multiplies the
 // scores, its value scale goes into the weights by way of their exponents.  Weights as 16-bit floats in units of 2^-11 reach down to
-// 2^-35 of the row's largest: 2^-12 of each is rounded away for bf16 rows (whose outputs keep 2^-9), and a second term takes that up for
+// 2^-35 of the row's largest: 2^-11 of each is rounded away for bf16 rows (whose outputs keep 2^-8), and a second term takes that up for
 // the others.  Sums, maxima and outputs are in 32 bits.
 // A workgroup's start is a chain of loads that wait for one another (length, table, codes; for lists: ids, table, codes): the first
 // tile's codes are asked for as soon as the table is there, and queries and scales are made ready meanwhile.
-// Measured (memory bounds the long ones, that chain the short ones): 64 requests of 1 to 8192 tokens, 8 heads of 128 dims, 540 MB: 113 us,
-// 4.8 TB/s (a large copy: 4.85); 2 requests of 150000 and more, 678 MB: 126 us, 5.4 TB/s; one request of 777 tokens, 8 heads of 64 dims: 9.4 us;
-// lists of 100 tokens, 64 requests of 32 lists, 56 MB of single rows: 17.7 us, 3.2 TB/s.
+// Measured (memory bounds the long ones, that chain the short ones; reading alone reaches 6.3 TB/s here, and this kernel 5.8 over 4.3 GB):
+// 64 requests of 1 to 8192 tokens, 8 heads of 128 dims, 540 MB: 113 us and 5 of joining; 2 requests of 150000 and more, 678 MB: 126 us and 5.5;
+// one request of 777 tokens, 8 heads of 64 dims: 9.6 us; lists of 100 tokens, 64 requests of 32 lists, 56 MB of single rows: 18 us, 3.1 TB/s.
 template <class T, int CODES, int DP, int MT, int NW, bool FOUND>
 __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_kernel(AttendArgs a, Partials parts, uint32_t heads, uint32_t q_vec)
 {
@@ -711,12 +711,13 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
 // of the values' octets, so that the blocks they lie in are scalars.
 // HALVES = 2: twice the wavefronts, which take the tiles in turn and join at the end: half the steps of one after the other where
 // workgroups are too few to hide them.  (Up to 64 dims, where two such workgroups fit a compute unit: 163 rows each of eight requests over
-// 1000 tokens, 16 heads: 34.3 us, 37.4 without.  At 128 dims only one fits, and the rounds cost more than the steps: 300 rows each of four over 700
-// tokens, 43.8 -> 51.3.)
+// 1000 tokens, 16 heads: 34.3 us, 37.4 without.  At 128 dims only one fits: with more than 256 workgroups the rounds cost more than the steps, 300 rows
+// each of four requests over 700 tokens 43.8 -> 51.3; with fewer they would win, 35 -> 30, which no rule here takes.)
 // Each wavefront has 16 * MT rows and their softmax to itself.  The arithmetic is that of attend_rows_kernel.
-// What bounds it is issue: per tile and wavefront about 260 vector instructions and 32 exponentials (1400 cycles; the softmax 60 % of them, decoding
-// a third) and 64 matrix instructions (1000), of which the registers leave room for two wavefronts a SIMD to overlap.  Three prompts of 900 rows over
-// 4000 tokens, 32 query heads of 128 dims, 156 GFLOP: 264 to 280 us, 560 to 590 TFLOP/s.
+// What bounds it: per tile and wavefront 371 vector instructions (by the counters, starts included; 32 of them are exponentials; 1870 cycles of issue)
+// and 64 matrix instructions (1020 cycles), of which the registers leave room for two wavefronts a SIMD to overlap.  Three prompts of 900 rows
+// over 4000 tokens, 32 query heads of 128 dims, 156 GFLOP: 275 us, 566 TFLOP/s, the vector units busy 43 % of it and the matrix units 23 %: neither is
+// the limit, but that the two overlap little, and that 688 workgroups on 512 places leave some compute units three to do and others two.
 template <class T, int CODES, int DP, int MT, int NBUF, int HALVES>
 __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile_kernel(AttendArgs a, Partials parts, uint32_t q_vec)
 {

@@ -44,8 +44,8 @@ __device__ __forceinline__ uint32_t last_not_after(const uint32_t* pre, uint32_t
 // launch that would wait for them) and then takes its share of the slots, table entries and returned blocks.  Nothing that a
 // workgroup reads is written by another: lengths and ring state go to buffers of their own, the table is written only beyond
 // what the requests held, and the ring only behind its tail, where no free block lies.
-// What bounds it is the chain of loads that wait for one another: lengths, table or ring, slots.  (64 requests, a token each: 3.9 us;
-// 1000 requests, 318000 tokens, 2.8 MB: 8.1 us.)
+// What bounds it is the chain of loads that wait for one another: lengths, table or ring, slots.  (64 requests, a token each: 4.0 us;
+// 1000 requests, 318000 tokens, 2.8 MB: 8.2 us.)
 __global__ void plan_kernel(PlanArgs a)
 {
     extern __shared__ uint32_t lds[];
@@ -177,7 +177,7 @@ __device__ __forceinline__ int scale_exponent(float peak, float most)
 // requests) are latency: a wavefront takes each by itself.  Long runs (prompts) are memory: all four wavefronts take each, and so they do
 // with runs of one block that slots which are left out keep apart, one after the other.
 // A power of two as scale makes x / scale exact, so a code is ONE rounding of x, and moving codes to a larger scale one more.
-// (64 rows of 8 heads of 128 dims: 4.2 us.  Three prompts, 21500 rows, 132 MB: 41.5 us, 3.2 TB/s: slots, rows, largest value and codes follow
+// (64 rows of 8 heads of 128 dims: 4.4 us.  Three prompts, 21500 rows, 132 MB: 41 us, 3.2 TB/s: slots, rows, largest value and codes follow
 // one another in a workgroup, and seven workgroups a compute unit hide most of that; five, with the rows kept as 32-bit values: 45 us.)
 template <class T, int CODES, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a)
@@ -339,7 +339,7 @@ struct ReadArgs {
     uint32_t n_rows, n_blocks, n_heads, block_tokens, dim;
 };
 
-// Eight values a lane; blockIdx.y: keys or values.  Bound by memory (21500 rows in 32 bits, 220 MB: 41 us, 5.4 TB/s).
+// Eight values a lane; blockIdx.y: keys or values.  Bound by memory (21500 rows in 32 bits, 220 MB: 42 us, 5.3 TB/s).
 template <class T, int CODES>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
 {

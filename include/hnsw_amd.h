@@ -353,8 +353,12 @@ int hnsw_amd_cache_read_device(const hnsw_amd_token_cache* cache, const int64_t*
  * (lens counts them): with `causal`, row i of n sees the tokens 0 .. lens - n + i; without, all of lens.  A row that sees
  * nothing gives zeros and -infinity.  Lengths are taken within 0 .. width * block_tokens, tokens of a block number outside
  * the cache do not exist.  max_len: a hint, the longest length (0: not known), which sets how the work is split; results do
- * not depend on it beyond rounding, but without it the workspace is for lengths of width blocks.  A call that mixes prompts and
- * single tokens costs between 0.85 and 1.6 of two calls.  n_rows * n_q_heads is below 2^24 (longer prompts: several calls).
+ * not depend on it beyond rounding, but without it the workspace is for lengths of width blocks: 4 (dim + 1) bytes for each row,
+ * query head and chunk, and a long request is cut into chunks of up to 4096 tokens.  One cut is made for all of a call's rows,
+ * by their number for each request in the mean; as many rows as requests are taken as one each, whatever cu_q says.  A call that
+ * mixes prompts and single tokens costs 0.85 to 1.8 times what two calls do where the single tokens' requests are at most twice as
+ * long as the prompts', and up to 10 times where they are far longer: make two calls of these.  n_rows * n_q_heads is below 2^24 (longer
+ * prompts: several calls).
  * workspace: at least hnsw_amd_cache_attend_workspace(...) bytes, 16-byte aligned, not shared with a call that may run at
  * the same time (NULL if that is 0). */
 uint64_t hnsw_amd_cache_attend_workspace(const hnsw_amd_token_cache* cache, uint32_t n_rows, uint32_t n_q_heads, uint32_t n_requests, uint32_t width,
