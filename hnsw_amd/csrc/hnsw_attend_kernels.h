@@ -250,7 +250,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
     static_assert(FOUND || kTable / 16 <= kThreads);
     constexpr int kOutLd = DP + 4, kJoin = NW == 1 ? 1 : NW / 2;
     __shared__ uint32_t ent_row[kEntries];                      // first row of a block's (a token's) codes, in rows of dim bytes; ~0: of no block
-    // its key scale (-1: of no block), its value scale in base 2, and that one's inverse
+    // its key scale (-1: of no block; the sign says so, a scale of -0 is made 0), its value scale in base 2, and that one's inverse
     __shared__ __align__(16) float ent_k[FOUND ? kEntries : 1], ent_v[FOUND ? kEntries : 1], ent_z[FOUND ? kEntries : 1];
     __shared__ __align__(16) float4 ent[FOUND ? 1 : kEntries];
     __shared__ __align__(16) float join[kJoin][16 * MT][kOutLd];
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
                     }
                 } else if (tid <= ((c1 - 1) >> bs_log) - e0) {
                     const float sv = bh[0] != ~0u ? a.v_scale[bh[0]] : 1.0f;
-                    ent[tid] = make_float4(bh[0] != ~0u ? a.k_scale[bh[0]] : -1.0f, log2_of_scale(sv), inverse_of_scale(sv), 0.0f);
+                    ent[tid] = make_float4(bh[0] != ~0u ? a.k_scale[bh[0]] + 0.0f : -1.0f, log2_of_scale(sv), inverse_of_scale(sv), 0.0f);
                 }
             }
             __syncthreads();
@@ -997,7 +997,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
     while (c0 < end) {
         if (has) {
             // the entries' scales
-            const float sk = bh != ~0u ? a.k_scale[bh] : -1.0f, sv = bh != ~0u ? a.v_scale[bh] : 1.0f;
+            const float sk = bh != ~0u ? a.k_scale[bh] + 0.0f : -1.0f, sv = bh != ~0u ? a.v_scale[bh] : 1.0f;
             if (tid <= ((c1 - 1) >> bs_log) - e0) ent[tid] = make_float4(sk, log2_of_scale(sv), inverse_of_scale(sv), 0.0f);
             const int own = NBUF * half;                        // this half's buffers
             store(own);

@@ -148,3 +148,16 @@ def test_rows_before_a_block_whose_scales_are_none(rows, dim, none):
     s.cache.k_scale[last], s.cache.v_scale[last] = none, none
     out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=cu)
     _check(s, q, out, lse, lambda r, h: (0, np.arange(length - rows + r + 1)), dim ** -0.5, range(0, rows - 14, 1 if rows < 50 else 17))
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (40, 128), (200, 64), (300, 128)])
+def test_scales_that_are_minus_zero(rows, dim):
+    """-0 is a scale of 0: scores of 0 for a key scale, values of zeros for a value scale."""
+    length = 430
+    s = Setup([length], 1, 16, dim, I8)
+    q, cu = _queries(rows, 1, dim, F32), _gpu([0, rows])
+    some = s.table[0, 2::3].long()
+    s.cache.k_scale[some], s.cache.v_scale[s.table[0, 1::3].long()] = -0.0, -0.0
+    s.k64, s.v64 = (c.cpu().double() * x.cpu().double()[:, :, None, None] for c, x in ((s.cache.k_codes, s.cache.k_scale), (s.cache.v_codes, s.cache.v_scale)))
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=cu)
+    _check(s, q, out, lse, lambda r, h: (0, np.arange(length - rows + r + 1)), dim ** -0.5, sorted({0, rows // 2, rows - 1}))
