@@ -161,3 +161,35 @@ def test_scales_that_are_minus_zero(rows, dim):
     s.k64, s.v64 = (c.cpu().double() * x.cpu().double()[:, :, None, None] for c, x in ((s.cache.k_codes, s.cache.k_scale), (s.cache.v_codes, s.cache.v_scale)))
     out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=cu)
     _check(s, q, out, lse, lambda r, h: (0, np.arange(length - rows + r + 1)), dim ** -0.5, sorted({0, rows // 2, rows - 1}))
+
+
+@pytest.mark.parametrize("codes,dtype", [(I8, F32), (E4, BF16)])
+@pytest.mark.parametrize("rows,group,dim", FORMS)
+@pytest.mark.parametrize("at", [0, 70, 150, 215, 280, 330, 400, 470])
+def test_one_block_of_large_values_anywhere(rows, group, dim, codes, dtype, at):
+    """Wavefronts take the tokens' tiles in turn: any one of them, and no other, meets the block, and their sums become one."""
+    length, block = 500, 16
+    s = Setup([length], 1, block, dim, codes)
+    vs = s.cache.v_scale.cpu()
+    vs[s.table[0, at // block].long()] *= 2.0 ** 60
+    _set(s, vs)
+    q, cu = _queries(rows, group, dim, dtype), _gpu([0, rows])
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=cu)
+    _check(s, q, out, lse, lambda r, h: (0, np.arange(length - rows + r + 1)), dim ** -0.5, sorted({0, rows // 3, rows // 2, rows - 1}))
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (40, 128), (200, 64), (300, 128)])
+def test_values_of_zeros_and_scores_far_below_zero(rows, dim):
+    """Scores around -600 (in base e), and nothing but scales of 0 among the values."""
+    length = 430
+    s = Setup([length], 1, 16, dim, I8)
+    _set(s, torch.zeros_like(s.cache.v_scale.cpu()), torch.full((s.cache.n_blocks, 1, 16), -96.0))
+    s.cache.k_scale.fill_(600 / 96)
+    s.k64 = s.cache.k_codes.cpu().double() * s.cache.k_scale.cpu().double()[:, :, None, None]
+    q = _queries(rows, 1, dim, F32) / 4096
+    q[..., 0] = 1.0
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens, cu_q=_gpu([0, rows]), scale=1.0)
+    _check(s, q, out, lse, lambda r, h: (0, np.arange(length - rows + r + 1)), 1.0, sorted({0, rows // 2, rows - 1}))
+    ids = _gpu(np.broadcast_to(np.arange(0, length, 3, dtype=np.int32), (rows, 1, 144)).copy())
+    out, lse = s.cache.attend_found(q, s.d_table, s.d_lens, ids, cu_q=_gpu([0, rows]), causal=False, scale=1.0)
+    _check(s, q, out, lse, lambda r, h: (0, np.arange(0, length, 3)), 1.0, sorted({0, rows // 2, rows - 1}))
