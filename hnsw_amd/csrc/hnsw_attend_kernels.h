@@ -396,7 +396,8 @@ __global__ __launch_bounds__(64 * NW, rows_waves(DP, MT, NW)) void attend_rows_k
             bh[0] = blk < a.n_blocks ? blk * a.n_heads + kv : ~0u;
             if (mine) ent_row[tid] = bh[0] == ~0u ? ~0u : bh[0] << bs_log;
             const unsigned long long fine = __ballot(bh[0] != ~0u);
-            if (lane == 0) red_n[wave] = fine ? (__builtin_amdgcn_readlane(bh[0], __builtin_ctzll(fine)) << bs_log) + 1 : 0;
+            const uint32_t live = fine ? (__builtin_amdgcn_readlane(bh[0], __builtin_ctzll(fine)) << bs_log) + 1 : 0;    // (all lanes take part)
+            if (lane == 0) red_n[wave] = live;
             __syncthreads();
             safe = 0;
 #pragma unroll
@@ -982,7 +983,8 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 4 : 2) void attend_tile
         bh = blk < a.n_blocks ? blk * a.n_heads + kv : ~0u;
         if (mine) ent_row[tid] = bh == ~0u ? ~0u : bh << bs_log;
         const unsigned long long fine = __ballot(bh != ~0u);
-        if (lane == 0) some[of_all] = fine ? (__builtin_amdgcn_readlane(bh, __builtin_ctzll(fine)) << bs_log) + 1 : 0;
+        const uint32_t live = fine ? (__builtin_amdgcn_readlane(bh, __builtin_ctzll(fine)) << bs_log) + 1 : 0;        // (all lanes take part)
+        if (lane == 0) some[of_all] = live;
         __syncthreads();
         safe = 0;
 #pragma unroll
