@@ -299,7 +299,9 @@ int hnsw_amd_vector_data(hnsw_amd_index* h, const float** out);
  * touch different buffers may overlap.  What lies in device memory cannot be refused by the host: each call says what it
  * does with block numbers, slots and lengths that are out of range (none of them reads or writes outside the buffers).
  * The codes and scales of a request's tokens are numbers, and scales are finite and not negative (append writes no others);
- * what a row gives that sees others is not defined. */
+ * what a row gives that sees others is not defined.  Attention takes a value scale by its logarithm in 32 bits: one that is no power of
+ * two (append writes none) counts with a relative error of up to 2^-23 of |log2 scale|.  Where the largest product of probability and
+ * value scale that a row has is below 2^-115 of its largest probability, its outputs are 0. */
 enum { HNSW_AMD_CODES_I8 = 0,         /* signed bytes, -127..127 */
        HNSW_AMD_CODES_E4M3 = 1 };     /* 8-bit floats (4 exponent, 3 mantissa bits; largest 448, no infinities) */
 enum { HNSW_AMD_TYPE_F32 = 0, HNSW_AMD_TYPE_F16 = 1, HNSW_AMD_TYPE_BF16 = 2 };   /* of rows, queries and outputs */
